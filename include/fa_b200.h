@@ -61,7 +61,8 @@ enum {
   FA_ERR_NO_DEVICE = 8,            /* no sm_100 device is current */
   FA_ERR_SCRATCH_LIMIT = 9,        /* the call needs more than FA_NOALLOC_SCRATCH_BYTES */
   FA_ERR_OUT_OF_MEMORY = 10,       /* the device had no memory for the library's scratch array */
-  FA_ERR_CUDA = 11                 /* another CUDA runtime call failed (fa_status_string names it) */
+  FA_ERR_CUDA = 11,                /* another CUDA runtime call failed (fa_status_string names it) */
+  FA_ERR_BAD_INDEX = 12            /* device status only: a position, slot, page or length out of range */
 };
 
 /* Forward: O = softmax(scale * Q K^T [+ causal mask]) V and the base-2 LSE.
@@ -468,9 +469,144 @@ FA_API int fa_bwd_dropout_bf16(const void* q, const void* k, const void* v, cons
                                const int64_t* dk_strides, const int64_t* dv_strides,
                                float dropout_p, uint64_t seed, float softmax_scale, int causal, void* stream);
 
+/* Query/key preparation.  No counterpart in the reference, which takes
+ * queries and keys as they enter the product.  For every row x of D values
+ * (one head of one token): r = 1 / sqrt(mean(x^2) + eps), y = x r w, and the
+ * first rotary_dim columns of y turn in pairs (a, b) by the angle of the
+ * token's position: a' = a cos - b sin, b' = b cos + a sin.  Pair i is
+ * columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved != 0.
+ * wq and wk are D weights each, in the operand type or fp32 (w_fp32), or both
+ * NULL: no norm.  table is (max_positions, rotary_dim) fp32, contiguous:
+ * rotary_dim / 2 cosines, then as many sines, of each position.  positions is
+ * int32, positions[b * pos_batch_stride + n]; NULL: token n is at position n.
+ * A position outside the table gives NaN in the turned columns and sets the
+ * device status to FA_ERR_BAD_INDEX.  Arithmetic is fp32, rounded once.
+ * q, q_out: (B, Hq, N, D), k, k_out: (B, Hkv, N, D) by element strides
+ * {batch, head, seq} (inputs may have zero strides); packed (total, H, D)
+ * tensors are B = 1, N = total.  rotary_dim is a multiple of 16, at most D. */
+FA_API int fa_qk_norm_rotary(const void* q, const void* k, void* q_out, void* k_out, const float* table,
+                        const int* positions, const void* wq, const void* wk, int B, int Hq, int Hkv, int
+                        N, int D, int max_positions, int rotary_dim, int interleaved, int w_fp32, const
+                        int64_t* q_strides, const int64_t* k_strides, const int64_t* qo_strides, const
+                        int64_t* ko_strides, int64_t pos_batch_stride, float eps, void* stream);
+FA_API int fa_qk_norm_rotary_bf16(const void* q, const void* k, void* q_out, void* k_out, const float*
+                        table, const int* positions, const void* wq, const void* wk, int B, int Hq, int
+                        Hkv, int N, int D, int max_positions, int rotary_dim, int interleaved, int
+                        w_fp32, const int64_t* q_strides, const int64_t* k_strides, const int64_t*
+                        qo_strides, const int64_t* ko_strides, int64_t pos_batch_stride, float eps, void*
+                        stream);
+/* Its backward: dq, dk from q, k and the outputs' gradients gq, gk, and with
+ * weights dwq and dwk (in the weights' type; NULL both: not wanted).  w_part
+ * is caller scratch of FA_ROTARY_PARTIALS * D floats (NULL without dwq).
+ * Sums run in an order fixed by the sizes: gradients repeat bit for bit. */
+#define FA_ROTARY_PARTIALS 592
+FA_API int fa_qk_norm_rotary_bwd(const void* q, const void* k, const void* gq, const void* gk, void* dq,
+                        void* dk, void* dwq, void* dwk, float* w_part, const float* table, const int*
+                        positions, const void* wq, const void* wk, int B, int Hq, int Hkv, int N, int D,
+                        int max_positions, int rotary_dim, int interleaved, int w_fp32, const int64_t*
+                        q_strides, const int64_t* k_strides, const int64_t* gq_strides, const int64_t*
+                        gk_strides, const int64_t* dq_strides, const int64_t* dk_strides, int64_t
+                        pos_batch_stride, float eps, void* stream);
+FA_API int fa_qk_norm_rotary_bwd_bf16(const void* q, const void* k, const void* gq, const void* gk, void*
+                        dq, void* dk, void* dwq, void* dwk, float* w_part, const float* table, const int*
+                        positions, const void* wq, const void* wk, int B, int Hq, int Hkv, int N, int D,
+                        int max_positions, int rotary_dim, int interleaved, int w_fp32, const int64_t*
+                        q_strides, const int64_t* k_strides, const int64_t* gq_strides, const int64_t*
+                        gk_strides, const int64_t* dq_strides, const int64_t* dk_strides, int64_t
+                        pos_batch_stride, float eps, void* stream);
+
+/* The same preparation for serving: packed q (total, Hq, D), k and v (total,
+ * Hkv, D) by element strides {batch (unused), head, row}; q is written to
+ * q_out (total, Hq, D), contiguous, the prepared k and v as it is to row
+ * slots[t] of the (num_slots, Hkv, D) caches, contiguous.  slots[t] < 0:
+ * nothing of token t is written to the caches; slots[t] >= num_slots: the
+ * same, and the device status is FA_ERR_BAD_INDEX.  Slots of one call must
+ * differ from each other.  positions is an int32 array of total. */
+FA_API int fa_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void*
+                        v_cache, const int* slots, const float* table, const int* positions, const void*
+                        wq, const void* wk, int total, int Hq, int Hkv, int D, int num_slots, int
+                        max_positions, int rotary_dim, int interleaved, int w_fp32, const int64_t*
+                        q_strides, const int64_t* k_strides, const int64_t* v_strides, float eps, void*
+                        stream);
+FA_API int fa_paged_append_bf16(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                        void* v_cache, const int* slots, const float* table, const int* positions, const
+                        void* wq, const void* wk, int total, int Hq, int Hkv, int D, int num_slots, int
+                        max_positions, int rotary_dim, int interleaved, int w_fp32, const int64_t*
+                        q_strides, const int64_t* k_strides, const int64_t* v_strides, float eps, void*
+                        stream);
+
+/* A serving step's tables from the requests' lengths.  Request r has
+ * cached[r] tokens in the cache and brings fresh[r] (int32, negative counts
+ * as 0).  Its row of block_table (requests, max_pages) holds
+ * ceil(cached / page_size) pages; the ones it lacks for cached + fresh tokens
+ * are appended, taken in the order of the requests from free_pages[start ..
+ * n_free), start = *free_start.  Written: cu_seqlens_q (requests + 1),
+ * offsets of the requests' new tokens, none above total_q; positions and
+ * slots (total_q), each new token's position in its sequence and its cache
+ * row page * page_size + position % page_size, 0 and -1 in rows behind the
+ * last request; seqlens_k (requests), cached + fresh; fits (requests, bytes);
+ * *free_next, the start for the next step.  A request whose pages would pass
+ * max_pages or whose tokens total_q takes no pages; one whose pages the free
+ * list lacks, and all after it, take none.  Such a request has fits = 0,
+ * slots of -1 and seqlens_k = cached.  Other entries of block_table stay as
+ * they are.  page_size is a power of two of at least 16. */
+FA_API int fa_extend_block_table(int* block_table, const int* cached, const int* fresh, const int*
+                        free_pages, const int* free_start, int* cu_seqlens_q, int* seqlens_k, int*
+                        positions, int* slots, uint8_t* fits, int* free_next, int requests, int
+                        max_pages, int n_free, int page_size, int total_q, void* stream);
+
+/* Attention of new tokens over chosen pages of a paged cache, in three calls.
+ * Layouts as in fa_fwd_paged: caches (num_pages, page_size, Hkv, D),
+ * block_table (B, max_pages_per_seq), row i of the nq a sequence brings is at
+ * position nk - nq + i of its nk keys and sees the keys up to it.  Pages are
+ * named by their index in the sequence.
+ *
+ * fa_page_means: the mean key, summed in 64 bits, of every page that the
+ * step's tokens completed, to page_means (num_pages, Hkv, D) in the cache's
+ * type; other rows stay as they are. */
+FA_API int fa_page_means(const void* k_cache, void* page_means, const int* block_table, const int*
+                        cu_seqlens_q, const int* seqlens_k, int B, int Hkv, int D, int num_pages, int
+                        page_size, int max_pages_per_seq, int total_q, void* stream);
+FA_API int fa_page_means_bf16(const void* k_cache, void* page_means, const int* block_table, const int*
+                        cu_seqlens_q, const int* seqlens_k, int B, int Hkv, int D, int num_pages, int
+                        page_size, int max_pages_per_seq, int total_q, void* stream);
+/* fa_select_pages: for each row and K/V head, top pages of those up to the
+ * row's own: the first sink, the last local (the own page is the last) and
+ * those with the highest max over the group's heads of q . page mean (64-bit
+ * sums, rounded to fp32; of equal scores the lower page; NaN is lowest).
+ * selected is (total_q, Hkv, top) int32, ascending, -1 behind a row's last
+ * page; all pages when there are no more than top.  1 <= local,
+ * 0 <= sink, sink + local <= top; max_pages_per_seq <= FA_MAX_SELECT_PAGES. */
+#define FA_MAX_SELECT_PAGES 16384
+FA_API int fa_select_pages(const void* q, const void* page_means, const int* block_table, const int*
+                        cu_seqlens_q, const int* seqlens_k, int* selected, int B, int Hq, int Hkv, int D,
+                        int total_q, int num_pages, int page_size, int max_pages_per_seq, int top, int
+                        sink, int local, const int64_t* q_strides, void* stream);
+FA_API int fa_select_pages_bf16(const void* q, const void* page_means, const int* block_table, const int*
+                        cu_seqlens_q, const int* seqlens_k, int* selected, int B, int Hq, int Hkv, int D,
+                        int total_q, int num_pages, int page_size, int max_pages_per_seq, int top, int
+                        sink, int local, const int64_t* q_strides, void* stream);
+/* fa_fwd_paged_sparse: o = softmax(scale * q k^T) v over the keys of the
+ * listed pages that the row sees; entries of -1 are skipped, as are pages
+ * behind the row's own.  A page listed twice counts twice.  Rows that see no
+ * listed key, and rows behind the last sequence, get zeros.  Nothing behind
+ * a row's position is used, whatever it holds.  o is (total_q, Hq, D),
+ * contiguous; q by element strides {batch (unused), head, row}. */
+FA_API int fa_fwd_paged_sparse(const void* q, const void* k_cache, const void* v_cache, void* o, const
+                        int* block_table, const int* cu_seqlens_q, const int* seqlens_k, const int*
+                        pages, int B, int Hq, int Hkv, int D, int total_q, int num_pages, int page_size,
+                        int max_pages_per_seq, int top, float softmax_scale, const int64_t* q_strides,
+                        void* stream);
+FA_API int fa_fwd_paged_sparse_bf16(const void* q, const void* k_cache, const void* v_cache, void* o,
+                        const int* block_table, const int* cu_seqlens_q, const int* seqlens_k, const int*
+                        pages, int B, int Hq, int Hkv, int D, int total_q, int num_pages, int page_size,
+                        int max_pages_per_seq, int top, float softmax_scale, const int64_t* q_strides,
+                        void* stream);
+
 /* Reads (and with reset != 0 clears) the device status word that kernels set
- * when a bounded wait gives up: 0 = healthy, else FA_ERR_DEVICE_TIMEOUT in the
- * low byte and the barrier site in bits 8..15.  Synchronises the device. */
+ * when a bounded wait gives up or an index is out of range: 0 = healthy, else
+ * FA_ERR_DEVICE_TIMEOUT or FA_ERR_BAD_INDEX in the low byte and the site in
+ * bits 8..15.  Synchronises the device. */
 FA_API int fa_device_status(int reset);
 
 /* Human-readable text of an FA_ERR_* code. */
@@ -479,7 +615,8 @@ FA_API const char* fa_status_string(int code);
 /* Library version: major * 10000 + minor * 100 + patch (1.1.0 adds bf16,
  * 1.2.0 the fused backward, 1.3.0 packed variable-length batches and the
  * paged K/V forward, 1.4.0 value head sizes different from D, 1.5.0 dense
- * boolean masks, 1.6.0 attention dropout). */
+ * boolean masks, 1.6.0 attention dropout, 1.7.0 query/key norm with rotation,
+ * cache append, block tables and page-sparse attention). */
 FA_API int fa_version(void);
 
 #ifdef __cplusplus

@@ -505,3 +505,145 @@ def attention_block_grads(q, k, v, do, lse2, delta, *, causal: bool, scale: floa
     dke = np.einsum("bhqk,bhqd->bhkd", ds, q) * scale
     dve = np.einsum("bhqk,bhqd->bhkd", p, do)
     return dq, _reduce_kv(dke, hkv), _reduce_kv(dve, hkv)
+
+
+# ------------------------------------------------------------------
+# Query/key preparation and the paged cache's step (no counterpart in the
+# reference): plain float64 restatements.
+def _rotate(y, table, pos, interleaved: bool, sign: float):
+    """Rows y (tokens, heads, D) turned by sign * their positions' angles."""
+    rd = table.shape[1]
+    t = np.asarray(table, np.float64)[pos]
+    cos, sin = t[:, None, :rd // 2], sign * t[:, None, rd // 2:]
+    z = y.copy()
+    a, b = (slice(0, rd, 2), slice(1, rd, 2)) if interleaved else (slice(0, rd // 2), slice(rd // 2, rd))
+    z[..., a] = y[..., a] * cos - y[..., b] * sin
+    z[..., b] = y[..., b] * cos + y[..., a] * sin
+    return z
+
+
+def norm_rotary_reference(x, weight, table, pos, eps: float, interleaved: bool, grad=None):
+    """Norm (unless weight is None) and rotation of packed rows x (tokens,
+    heads, D) at int positions pos; with ``grad`` also dx and dw (None without
+    a weight).  Returns a dict."""
+    x = np.asarray(x, np.float64)
+    if weight is None:
+        out = {"z": _rotate(x, table, pos, interleaved, 1.0)}
+        if grad is not None:
+            out.update(dx=_rotate(np.asarray(grad, np.float64), table, pos, interleaved, -1.0), dw=None)
+        return out
+    w = np.asarray(weight, np.float64)
+    r = 1.0 / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
+    out = {"z": _rotate(x * r * w, table, pos, interleaved, 1.0)}
+    if grad is not None:
+        dy = _rotate(np.asarray(grad, np.float64), table, pos, interleaved, -1.0)
+        g = dy * w
+        out["dx"] = r * (g - x * r * r * (g * x).mean(-1, keepdims=True))
+        out["dw"] = (dy * x * r).sum((0, 1))
+    return out
+
+
+def extend_block_table_reference(block_table, cached, new, free_pages, free_start: int, page_size: int, total_q: int):
+    """One request after the other; returns a dict of fa_extend_block_table's
+    outputs (the table a new array)."""
+    table = np.array(block_table, np.int32)
+    requests, width = table.shape
+    cu, seqlens, fits = [0], [], []
+    pos, slots = np.zeros(total_q, np.int32), np.full(total_q, -1, np.int32)
+    start = max(0, int(free_start))
+    left = len(free_pages) - start
+    want_sum, used, row = 0, 0, 0
+    for r in range(requests):
+        c, f = max(0, int(cached[r])), max(0, int(new[r]))
+        have, want = -(-c // page_size), -(-(c + f) // page_size)
+        placed = want <= width and row + f <= total_q
+        need = want - have if placed else 0
+        want_sum += need
+        ok = placed and want_sum <= left
+        if ok:
+            first = start + want_sum - need
+            table[r, have:want] = free_pages[first:first + need]
+            used = want_sum
+        for i in range(max(0, min(f, total_q - row))):
+            p = c + i
+            pos[row + i] = min(p, 2 ** 31 - 1)
+            if ok and table[r, p // page_size] >= 0:
+                slots[row + i] = table[r, p // page_size] * page_size + p % page_size
+        row += f
+        cu.append(min(row, total_q))
+        seqlens.append(c + f if ok else c)
+        fits.append(ok)
+    return {"block_table": table, "cu_seqlens_q": np.array(cu, np.int32), "seqlens_k": np.array(seqlens, np.int32),
+            "positions": pos, "slot_mapping": slots, "fits": np.array(fits),
+            "free_next": np.array([start + used], np.int32)}
+
+
+def _rows(cu, seqlens_k):
+    """(row, sequence, position) of every packed row."""
+    for b in range(len(seqlens_k)):
+        for t in range(cu[b], cu[b + 1]):
+            yield t, b, int(seqlens_k[b]) - int(cu[b + 1] - t)
+
+
+def page_means_reference(k_cache, means, block_table, cu, seqlens_k):
+    """means (num_pages, Hkv, D) float64 with the rows of the pages that the
+    step completed replaced."""
+    out = np.array(means, np.float64)
+    page = k_cache.shape[1]
+    for b in range(len(seqlens_k)):
+        nk, nq = int(seqlens_k[b]), int(cu[b + 1] - cu[b])
+        if nq > 0:
+            for p in range(max(nk - nq, 0) // page, nk // page):
+                out[block_table[b, p]] = np.asarray(k_cache[block_table[b, p]], np.float64).mean(0)
+    return out
+
+
+def select_pages_reference(q, means, block_table, cu, seqlens_k, page_size: int, top: int, sink: int, local: int):
+    """int32 (total, Hkv, top): the kept pages of each row and K/V head."""
+    q, means = np.asarray(q, np.float64), np.asarray(means, np.float64)
+    total, hq, _ = q.shape
+    hkv = means.shape[1]
+    out = np.full((total, hkv, top), -1, np.int32)
+    for t, b, pos in _rows(cu, seqlens_k):
+        if pos < 0:
+            continue
+        n = pos // page_size + 1
+        for h in range(hkv):
+            if n <= top:
+                keep = np.arange(n)
+            else:
+                g = q[t, h * (hq // hkv):(h + 1) * (hq // hkv)]
+                s = (means[block_table[b, :n], h] @ g.T).max(1).astype(np.float32)
+                s = np.where(np.isnan(s), -np.inf, s)
+                s[:sink] = np.inf
+                s[n - local:] = np.inf
+                keep = np.sort(np.argsort(-s, kind="stable")[:top])
+            out[t, h, :len(keep)] = keep
+    return out
+
+
+def sparse_paged_reference(q, k_cache, v_cache, block_table, cu, seqlens_k, pages, scale: float):
+    """(o, a): attention over the listed pages in float64, and the same
+    weights over |v| (what a rounding of the weights is measured by)."""
+    q = np.asarray(q, np.float64)
+    total, hq, d = q.shape
+    page, hkv = k_cache.shape[1], k_cache.shape[2]
+    o, a = np.zeros((total, hq, d)), np.zeros((total, hq, d))
+    for t, b, pos in _rows(cu, seqlens_k):
+        for h in range(hkv):
+            ks, vs = [], []
+            for p in map(int, pages[t, h]):
+                seen = min(page, pos - p * page + 1)
+                if p >= 0 and seen > 0:
+                    ks.append(np.asarray(k_cache[block_table[b, p], :seen, h], np.float64))
+                    vs.append(np.asarray(v_cache[block_table[b, p], :seen, h], np.float64))
+            if not ks:
+                continue
+            k, v = np.concatenate(ks), np.concatenate(vs)
+            g = hq // hkv
+            s = scale * q[t, h * g:(h + 1) * g] @ k.T
+            w = np.exp(s - s.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            o[t, h * g:(h + 1) * g] = w @ v
+            a[t, h * g:(h + 1) * g] = w @ np.abs(v)
+    return o, a

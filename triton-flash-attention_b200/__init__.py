@@ -35,6 +35,21 @@ from .masks import (
     attention_forward_masked,
     pack_attention_mask,
 )
+from .paging import (
+    PagedStep,
+    extend_block_table,
+    paged_append,
+    scaled_dot_product_attention_paged_sparse,
+    select_pages,
+    update_page_means,
+)
+from .rotary import (
+    B200QKNormRotary,
+    qk_norm_rotary,
+    qk_norm_rotary_backward,
+    qk_norm_rotary_forward,
+    rotary_table,
+)
 from .varlen import (
     B200VarlenAttention,
     paged_attention_forward,
@@ -48,8 +63,10 @@ __all__ = [
     "B200Attention",
     "B200DropoutAttention",
     "B200MaskedAttention",
+    "B200QKNormRotary",
     "B200VarlenAttention",
     "DispatchDecision",
+    "PagedStep",
     "SUPPORTED_HEAD_DIMS",
     "FUSED_BWD_HEAD_DIMS",
     "TritonAttention",
@@ -67,13 +84,22 @@ __all__ = [
     "attention_forward_vdim",
     "delta_bytes",
     "explain_dispatch",
+    "extend_block_table",
     "fused_backward_enabled",
     "memory_model",
     "pack_attention_mask",
+    "paged_append",
     "paged_attention_forward",
+    "qk_norm_rotary",
+    "qk_norm_rotary_backward",
+    "qk_norm_rotary_forward",
+    "rotary_table",
     "scaled_dot_product_attention",
     "scaled_dot_product_attention_paged",
+    "scaled_dot_product_attention_paged_sparse",
     "scaled_dot_product_attention_varlen",
+    "select_pages",
+    "update_page_means",
     "varlen_attention_backward",
     "varlen_attention_forward",
 ]

@@ -27,6 +27,7 @@ FA_ERR_NO_DEVICE = 8
 FA_ERR_SCRATCH_LIMIT = 9
 FA_ERR_OUT_OF_MEMORY = 10
 FA_ERR_CUDA = 11
+FA_ERR_BAD_INDEX = 12
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -76,6 +77,18 @@ SIGNATURES.update({
 SIGNATURES.update({name + "_bf16": SIGNATURES[name]
                    for name in ("fa_fwd_vdim", "fa_bwd_vdim", "fa_fwd_masked", "fa_bwd_masked",
                                 "fa_fwd_dropout", "fa_bwd_dropout")})
+SIGNATURES.update({
+    "fa_qk_norm_rotary": (_i, [_p] * 8 + [_i] * 9 + [_s] * 4 + [ctypes.c_int64, _f, _p]),
+    "fa_qk_norm_rotary_bwd": (_i, [_p] * 13 + [_i] * 9 + [_s] * 6 + [ctypes.c_int64, _f, _p]),
+    "fa_paged_append": (_i, [_p] * 11 + [_i] * 9 + [_s] * 3 + [_f, _p]),
+    "fa_page_means": (_i, [_p] * 5 + [_i] * 7 + [_p]),
+    "fa_select_pages": (_i, [_p] * 6 + [_i] * 11 + [_s, _p]),
+    "fa_fwd_paged_sparse": (_i, [_p] * 8 + [_i] * 9 + [_f, _s, _p]),
+})
+SIGNATURES.update({name + "_bf16": SIGNATURES[name]
+                   for name in ("fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_paged_append", "fa_page_means",
+                                "fa_select_pages", "fa_fwd_paged_sparse")})
+SIGNATURES["fa_extend_block_table"] = (_i, [_p] * 11 + [_i] * 5 + [_p])
 SIGNATURES.update({
     "fa_bwd_fused_noalloc": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i,
                                   _s, _s, _s, _s, _s, _s, _s, _s, _f, _i, _p]),
@@ -145,7 +158,12 @@ def strides3(t) -> ctypes.Array:
     s = t.stride()
     if s[3] != 1:
         raise ValueError("the head dimension must be contiguous (unit stride)")
-    key = s[:3]
+    return strides_of(s[:3])
+
+
+def strides_of(key: tuple) -> ctypes.Array:
+    """Three element strides as a ctypes array, shared by every call with the
+    same ones."""
     arr = _strides_cache.get(key)
     if arr is None:
         if len(_strides_cache) > 1024:
@@ -155,5 +173,6 @@ def strides3(t) -> ctypes.Array:
 
 
 def device_status(reset: bool = False) -> int:
-    """The device status word (0 = healthy); synchronises the device."""
+    """The device status word (0 = healthy; its low byte is an ``FA_ERR_*``
+    code); synchronises the device."""
     return int(lib().fa_device_status(1 if reset else 0))

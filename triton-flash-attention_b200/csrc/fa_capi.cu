@@ -702,6 +702,12 @@ int bwd_dense_impl(const void* q, const void* k, const void* v, const void* o, c
 }
 
 }  // namespace
+
+int* device_status_word() { return status_ptr(); }
+int make_cache_map(CUtensorMap* map, const void* cache, int cache_rows, int Hkv, int D, int rows, int dtype) {
+  const PackedStrides sk(cache_rows, Hkv, D);
+  return make_map(map, cache, 1, Hkv, cache_rows, D, sk.v, rows, dtype);
+}
 }  // namespace fa
 
 using namespace fa;
@@ -933,6 +939,7 @@ extern "C" const char* fa_status_string(int code) {
     case FA_ERR_SCRATCH_LIMIT: return "the call needs more scratch than FA_NOALLOC_SCRATCH_BYTES (32 MiB)";
     case FA_ERR_OUT_OF_MEMORY: return "out of device memory for the library's scratch array";
     case FA_ERR_CUDA: return last_cuda_error_text();
+    case FA_ERR_BAD_INDEX: return "a position, cache slot, page or length is out of range";
     default: return "unknown error";
   }
 }
@@ -1120,4 +1127,4 @@ extern "C" int fa_bwd_dropout_bf16(const void* q, const void* k, const void* v, 
                            softmax_scale, causal, stream, DT_BF16);
 }
 
-extern "C" int fa_version(void) { return 10600; }
+extern "C" int fa_version(void) { return 10700; }

@@ -91,6 +91,97 @@ int launch_combine_splits(const void* o_part, const float* lse_part, void* o, fl
 int launch_merge_partial(float* o_acc, float* lse_acc, const void* o_part, const float* lse_part, long long rows,
                          int D, int dtype, cudaStream_t stream);
 
+// ---------------------------------------------------------------------------
+// Query/key preparation and the paged cache (fa_rotary.cu, fa_tables.cu,
+// fa_sparse.cu; no counterpart in the reference).
+
+// Sites of FA_ERR_BAD_INDEX in the device status word (bits 8..15): a
+// position, a slot, a page or a length that a kernel refused.
+enum : int { FA_SITE_POSITION = 224, FA_SITE_SLOT = 225, FA_SITE_PAGE = 226 };
+
+struct RowStrides {
+  long long b, h, n;  // elements
+};
+// Norm and rotation of query and key rows (B batches x N tokens x heads).
+struct RotaryArgs {
+  const void *q, *k, *v;  // v: append only
+  RowStrides qs, ks, vs;
+  const void *gq, *gk;  // backward: gradients of the outputs
+  RowStrides gqs, gks;
+  void *qo, *ko, *vo;  // outputs; append: packed q, k cache, v cache
+  RowStrides qos, kos;
+  const float* table;  // (max_pos, rd): cosines, then sines
+  const int* pos;      // nullptr: the token's index
+  long long pos_sb;
+  const int* slots;  // append: a cache row for each token, -1 for none
+  const void *wq, *wk;  // nullptr: no norm
+  void *dwq, *dwk;
+  float* w_part;  // (ROTARY_BWD_CTAS, D) partial weight gradients
+  float eps;
+  int max_pos, rd, interleaved, w_fp32, n_slots;
+  int B, N, Hq, Hkv, dtype;
+  int q_ctas;
+  int* status;
+  cudaStream_t stream;
+};
+constexpr int ROTARY_BWD_CTAS = FA_ROTARY_PARTIALS;
+void rotary_bwd_ctas(int Hq, int Hkv, long long rows, int D, int* q_ctas, int* k_ctas);
+int launch_rotary_fwd(const RotaryArgs& a, int D);
+int launch_rotary_bwd(const RotaryArgs& a, int D);
+int launch_paged_append(const RotaryArgs& a, int D);
+
+struct TableArgs {
+  int* table;  // (requests, width)
+  const int *cached, *fresh;
+  const int *free_pages, *free_start;
+  int *cu, *seqlens, *pos, *slots;
+  unsigned char* fits;
+  int* free_next;
+  int requests, width, n_free, page_log2, total;
+  cudaStream_t stream;
+};
+int launch_extend_table(const TableArgs& a);
+
+struct PageArgs {
+  const void* k_cache;
+  void* means;  // (num_pages, Hkv, D)
+  const int *table, *cu, *seqlens;
+  int B, Hkv, D, num_pages, page_log2, width, dtype;
+  int* status;
+  cudaStream_t stream;
+};
+int launch_page_means(const PageArgs& a, int total_q);
+
+struct SelectArgs {
+  const void *q, *means;
+  long long q_sh, q_st;  // element strides of heads and rows
+  const int *table, *cu, *seqlens;
+  int* out;  // (total_q, Hkv, top)
+  int B, Hq, Hkv, total_q, num_pages, page_log2, width, top, sink, local, dtype;
+  int cluster, share;  // set by the launch
+  int* status;
+  cudaStream_t stream;
+};
+int launch_select_pages(SelectArgs a, int D);
+
+struct SparseArgs {
+  const void* q;
+  void* o;
+  long long q_sh, q_st;
+  const int *table, *cu, *seqlens, *idx;
+  int B, Hq, Hkv, total_q, num_pages, page_log2, width, top, dtype;
+  int cluster;  // set by the launch
+  float scale_log2;
+  int* status;
+  cudaStream_t stream;
+};
+int launch_sparse_decode(SparseArgs a, const CUtensorMap& k, const CUtensorMap& v, int D);
+
+// The device status word, and a tensor map over a (num_pages, page_size, Hkv,
+// D) cache whose box is `rows` rows of one head (fa_capi.cu).
+int* device_status_word();
+int make_cache_map(CUtensorMap* map, const void* cache, int cache_rows, int Hkv, int D, int rows, int dtype);
+
 // Query-tile / key-tile sizes the host needs for TMA box shapes.
 namespace dq_cfg {
 constexpr int BM = 128;  // query rows per tile

@@ -1,0 +1,826 @@
+// fa_sparse.cu -- attention of new tokens over a few pages of a paged K/V
+// cache, chosen for each token and K/V head by a cheap score.
+//
+//  * fa_page_means_kernel: the mean key of every page that a step's tokens
+//    completed;
+//  * fa_select_pages_kernel: score(p) = max over the group's query heads of
+//    q . mean key of page p, and the top pages by it;
+//  * fa_sparse_decode_kernel: softmax attention over the keys of the listed
+//    pages that the token may see.
+//
+// Means and scores decide which pages are kept, and two pages' scores may be
+// as near as their roundings, so both are summed in 64 bits and rounded once
+// to what they are kept in (means: to fp32 and then the cache's type; scores:
+// to fp32).  The kept pages then depend on the inputs alone, not on the order
+// of a sum.
+#include "fa_kernels.h"
+
+namespace fa {
+namespace {
+
+// Sequence of packed row t: the last b with cu[b] <= t, by 32 probes a step.
+// Every lane of the warp calls and gets it.
+__device__ __forceinline__ int warp_find_seq(const int* __restrict__ cu, int B, int t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = B;
+  while (len > 1) {
+    const int step = (len + 31) / 32;
+    const int i = lane * step;
+    const bool ok = i < len && __ldg(cu + lo + i) <= t;
+    const int c = __popc(__ballot_sync(0xffffffffu, ok));
+    const int at = c > 0 ? (c - 1) * step : 0;
+    lo += at;
+    len = min(step, len - at);
+  }
+  return lo;
+}
+
+template <int DT>
+__device__ __forceinline__ float to_f32(uint16_t v) {
+  return unpack2<DT>(uint32_t(v)).x;
+}
+
+// ---------------------------------------------------------------------------
+// Means of completed pages.
+//
+// Sequence b brings rows cu[b] .. cu[b+1] - 1, its last keys, and so completes
+// pages (nk - nq) / P .. nk / P - 1: at most floor(nq / P) + 1 of them.  Unit
+// u of the launch is page u - off(b) of them with off(b) = cu[b] / P + b, which
+// leaves room enough for every b and needs no sum over the sequences.
+//
+// A block takes one page: P rows of W = Hkv D neighbouring columns.  A thread
+// sums 8 columns of every n-th row; the partial sums meet in shared memory.
+constexpr int MEAN_THREADS = 512;
+
+template <int DT>
+__global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __grid_constant__ PageArgs a, int units) {
+  extern __shared__ double part[];  // [row groups][8 * columns of a pass]
+  const int W8 = a.Hkv * a.D / 8;   // 16-byte column chunks of a row
+  const int cols = min(W8, MEAN_THREADS);
+  const int groups = min(MEAN_THREADS / cols, 8);
+  const int P = 1 << a.page_log2;
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    // last b with off(b) <= u
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = a.B;
+    while (len > 1) {
+      const int step = (len + 31) / 32;
+      const int i = lane * step;
+      const bool ok = i < len && (__ldg(a.cu + lo + i) >> a.page_log2) + lo + i <= u;
+      const int c = __popc(__ballot_sync(0xffffffffu, ok));
+      const int at = c > 0 ? (c - 1) * step : 0;
+      lo += at;
+      len = min(step, len - at);
+    }
+    const int b = lo;
+    const int q0 = __ldg(a.cu + b), nq = __ldg(a.cu + b + 1) - q0, nk = __ldg(a.seqlens + b);
+    if (nq <= 0 || nk <= 0) continue;
+    const int from = max(nk - nq, 0) >> a.page_log2;
+    const long long p = (long long)from + (u - ((q0 >> a.page_log2) + b));
+    if (p < from || p >= (nk >> a.page_log2) || p >= a.width) continue;  // uniform in the block
+    const int id = __ldg(a.table + (long long)b * a.width + p);
+    if (id < 0 || id >= a.num_pages) {
+      if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+      continue;
+    }
+    const uint16_t* src = static_cast<const uint16_t*>(a.k_cache) + (long long)id * P * a.Hkv * a.D;
+    uint16_t* dst = static_cast<uint16_t*>(a.means) + (long long)id * a.Hkv * a.D;
+    const int g = threadIdx.x / cols, c0 = threadIdx.x % cols;
+    for (int base = 0; base < W8; base += cols) {
+      const int c = base + c0;
+      const bool mine = g < groups && c < W8;
+      double s[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = 0.0;
+      if (mine) {
+#pragma unroll 8
+        for (int r = g; r < P; r += groups) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + (long long)r * a.Hkv * a.D) + c);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<DT>(w[j]);
+            s[2 * j] += double(f.x);
+            s[2 * j + 1] += double(f.y);
+          }
+        }
+      }
+      __syncthreads();  // the last pass's sums are read
+      if (mine && g > 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[((g - 1) * 8 + j) * cols + c0] = s[j];
+      __syncthreads();
+      if (mine && g == 0) {
+        for (int o = 1; o < groups; ++o)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[j] += part[((o - 1) * 8 + j) * cols + c0];
+        float f[8];
+        const double inv = 1.0 / double(P);  // a power of two: exact
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __double2float_rn(s[j] * inv);
+        reinterpret_cast<uint4*>(dst)[c] = make_uint4(pack2<DT>(f[0], f[1]), pack2<DT>(f[2], f[3]),
+                                                      pack2<DT>(f[4], f[5]), pack2<DT>(f[6], f[7]));
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Cluster helpers: `S` blocks of one launch cluster share a unit's work.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// All threads of all blocks of the cluster; shared-memory writes before it
+// are seen after it.  It ends as soon as every block has come to it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of this block's shared variable at saddr in block `rank`.
+__device__ __forceinline__ uint32_t cluster_map(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// The packed row's sequence and its position there: keys 0 .. pos are seen.
+// pos < 0: a row behind the last sequence, or one whose sequence has no key
+// for it.  Every lane of the warp calls.
+struct RowPlace {
+  int b;
+  int pos;
+};
+__device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens, int B, int t, int key_cap,
+                                              int* status) {
+  RowPlace r;
+  r.b = warp_find_seq(cu, B, t);
+  const int q0 = __ldg(cu + r.b), q1 = __ldg(cu + r.b + 1);
+  const int nk = __ldg(seqlens + r.b);
+  const long long pos = (long long)nk - (q1 - t);  // the rows are the sequence's last
+  const bool too_long = nk > key_cap;  // its table row cannot hold it
+  if (too_long && status) atomicCAS(status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+  r.pos = (t < q0 || t >= q1 || too_long) ? -1 : int(pos < 0 ? -1 : pos);
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// Page selection.  A cluster of S blocks takes one (token, K/V head): every
+// block scores its share of the pages into the first block's shared memory,
+// which then finds the top ones.
+//
+// Scoring: D / 8 lanes own a page, 8 columns a lane, SEL_PAGES pages at once
+// for their loads in flight.  The group's queries lie in shared memory in 64
+// bits.  Lanes swap halves of their page sums until each holds whole ones.
+//
+// Selection: keys are the scores' bits in an order that whole numbers have,
+// SEL_KEYS neighbouring ones a thread.  The kk-th largest key is found bit by
+// bit, a block-wide count for each; the pages above it, and of the pages at
+// it the first ones, are written in order of their index.
+constexpr int SEL_THREADS = 512;
+constexpr int SEL_PAGES = 4;
+
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0u;  // NaN: behind everything
+  const uint32_t u = __float_as_uint(f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(SEL_THREADS) fa_select_pages_kernel(const __grid_constant__ SelectArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int LP = D / 8;  // lanes of a page
+  const int S = a.cluster;
+  const int rank = S > 1 ? int(cluster_rank()) : 0;
+  const int unit = blockIdx.x / S;
+  const int t = unit / a.Hkv, h = unit - t * a.Hkv;
+  const int G = a.Hq / a.Hkv;
+  const int lane = threadIdx.x & 31;
+  // [G][4][LP] pairs of a query's columns in 64 bits, then ids, then keys
+  double2* qd = reinterpret_cast<double2*>(smem);
+  int* ids = reinterpret_cast<int*>(smem + size_t(G) * D * 8);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(ids + a.share);
+  __shared__ int warp_gt[SEL_THREADS / 32], warp_eq[SEL_THREADS / 32];
+
+  const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
+  int* out = a.out + (long long)unit * a.top;
+  const int n = row.pos < 0 ? 0 : (row.pos >> a.page_log2) + 1;  // pages up to the token's own
+  if (n <= a.top) {  // all of them (uniform over the cluster)
+    if (rank == 0)
+      for (int i = threadIdx.x; i < a.top; i += SEL_THREADS) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int M = n - a.sink - a.local;  // pages to choose from, the first at index sink
+  const int kk = a.top - a.sink - a.local;
+  if (rank == 0)
+    for (int i = threadIdx.x; i < a.sink + a.local; i += SEL_THREADS) {
+      if (i < a.sink) out[i] = i;
+      else out[a.top - a.local + (i - a.sink)] = n - a.local + (i - a.sink);
+    }
+  if (kk == 0) return;
+
+  // this block's pages: a contiguous share
+  const int share = (M + S - 1) / S;
+  const int p0 = rank * share, pn = max(0, min(share, M - p0));
+  for (int i = threadIdx.x; i < pn; i += SEL_THREADS) {
+    const int id = __ldg(a.table + (long long)row.b * a.width + a.sink + p0 + i);
+    const bool ok = id >= 0 && id < a.num_pages;
+    if (!ok && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+    ids[i] = ok ? id : -1;
+  }
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
+  for (int i = threadIdx.x; i < G * D / 2; i += SEL_THREADS) {
+    const int g = i / (D / 2), d = i % (D / 2) * 2;  // columns d, d + 1: lane d / 8, pair (d % 8) / 2
+    const float2 f = unpack2<DT>(__ldg(reinterpret_cast<const uint32_t*>(q + g * a.q_sh + d)));
+    qd[(g * 4 + (d % 8) / 2) * LP + d / 8] = make_double2(double(f.x), double(f.y));
+  }
+  if (S > 1) cluster_sync();  // and the first block has begun, so that its shared memory may be written
+  else __syncthreads();
+  const uint32_t keys0 = smem_u32(keys);
+  const uint32_t keys_at = S > 1 ? cluster_map(keys0, 0) : keys0;
+  {
+    const int sub = threadIdx.x / LP, l = threadIdx.x % LP;
+    constexpr int SUBS = SEL_THREADS / LP;
+    // the trip count is the warp's, for the shuffles
+    for (int base = (sub - lane / LP) * SEL_PAGES; base < pn; base += SUBS * SEL_PAGES) {
+      const int first = base + lane / LP * SEL_PAGES;
+      double kd[SEL_PAGES][8];
+      uint4 v[SEL_PAGES];
+#pragma unroll
+      for (int i = 0; i < SEL_PAGES; ++i) {
+        const int id = first + i < pn ? ids[first + i] : -1;
+        v[i] = id >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.means) +
+                                                              ((long long)id * a.Hkv + h) * D) + l)
+                       : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < SEL_PAGES; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack2<DT>(w[j]);
+          kd[i][2 * j] = double(f.x);
+          kd[i][2 * j + 1] = double(f.y);
+        }
+      }
+      float best = -INFINITY;
+      bool nan = false;
+      for (int g = 0; g < G; ++g) {
+        double s[SEL_PAGES];
+#pragma unroll
+        for (int i = 0; i < SEL_PAGES; ++i) s[i] = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const double2 x = qd[(g * 4 + j) * LP + l];
+#pragma unroll
+          for (int i = 0; i < SEL_PAGES; ++i) s[i] = fma(x.y, kd[i][2 * j + 1], fma(x.x, kd[i][2 * j], s[i]));
+        }
+        // 4 page sums over LP lanes: keep 2, then 1, then add it up
+        const bool up0 = (l & (LP / 2)) != 0;
+        double e0 = up0 ? s[2] : s[0], e1 = up0 ? s[3] : s[1];
+        e0 += __shfl_xor_sync(0xffffffffu, up0 ? s[0] : s[2], LP / 2);
+        e1 += __shfl_xor_sync(0xffffffffu, up0 ? s[1] : s[3], LP / 2);
+        const bool up1 = (l & (LP / 4)) != 0;
+        double e = up1 ? e1 : e0;
+        e += __shfl_xor_sync(0xffffffffu, up1 ? e0 : e1, LP / 4);
+#pragma unroll
+        for (int m = LP / 8; m > 0; m >>= 1) e += __shfl_xor_sync(0xffffffffu, e, m);
+        const float f = __double2float_rn(e);
+        nan |= f != f;
+        best = fmaxf(best, f);
+      }
+      // this lane's page of the four
+      const int mine = first + ((l & (LP / 2)) ? 2 : 0) + ((l & (LP / 4)) ? 1 : 0);
+      if ((l & (LP / 4 - 1)) == 0 && mine < pn) {
+        const uint32_t key = ids[mine] < 0 || nan ? 0u : order_key(best);
+        st_cluster_u32(keys_at + 4u * uint32_t(p0 + mine), key);
+      }
+    }
+  }
+  if (S > 1) {
+    cluster_sync();
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+
+  // thread i owns keys [i E, (i + 1) E)
+  const int E = (M + SEL_THREADS - 1) / SEL_THREADS;
+  const int k0 = min(M, int(threadIdx.x) * E), k1 = min(M, k0 + E);
+  uint32_t T = 0;  // the kk-th largest key
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t cand = T | (1u << bit);
+    int c = 0;
+    for (int i = k0; i < k1; ++i) c += keys[i] >= cand;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) warp_gt[threadIdx.x >> 5] = c;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < SEL_THREADS / 32; ++w) all += warp_gt[w];
+    __syncthreads();
+    if (all >= kk) T = cand;
+  }
+  int gt = 0, eq = 0;
+  for (int i = k0; i < k1; ++i) gt += keys[i] > T, eq += keys[i] == T;
+  int gs = gt, es = eq;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, gs, m), y = __shfl_up_sync(0xffffffffu, es, m);
+    if (lane >= m) gs += x, es += y;
+  }
+  if (lane == 31) warp_gt[threadIdx.x >> 5] = gs, warp_eq[threadIdx.x >> 5] = es;
+  __syncthreads();
+  gs -= gt;
+  es -= eq;
+  int total_gt = 0;
+  for (int w = 0; w < SEL_THREADS / 32; ++w) {
+    if (w < int(threadIdx.x >> 5)) gs += warp_gt[w], es += warp_eq[w];
+    total_gt += warp_gt[w];
+  }
+  const int want_eq = kk - total_gt;
+  for (int i = k0; i < k1; ++i) {
+    const uint32_t key = keys[i];
+    if (key > T || (key == T && es < want_eq)) out[a.sink + gs + min(es, want_eq)] = a.sink + i;
+    gs += key > T;
+    es += key == T;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention over the listed pages.
+//
+// A cluster of S blocks takes one (token, K/V head, up to 16 of its query
+// heads).  The list is cut into 64-key tiles; block r takes tiles r, r + S,
+// ...  A producer warp copies a tile's K and V rows by TMA, a piece of a page
+// and 64 columns a copy, into a ring of DEC_STAGES tiles.  Four warps take 16
+// keys of every tile each, with softmax state of their own: S = Q K^T and
+// O += P V by m16n8k16 matrix instructions with the query heads as the 16
+// rows, so nothing is exchanged until the end.  Then the warps' states are
+// joined in shared memory and the blocks' over the cluster's.
+//
+// Bound: HBM, 4 D bytes a key.  For a key the two products are 2 matrix
+// instructions, 4 of the 22 clocks that its bytes take an SM's share of HBM;
+// tcgen05's 128 rows would be 7 of 8 parts empty for a group's heads.
+constexpr int DEC_WARPS = 4;
+constexpr int DEC_THREADS = (DEC_WARPS + 1) * 32;
+constexpr int DEC_TILE = 64;
+constexpr int NO_KEY = 0x7fffffff;
+
+template <int D>
+constexpr int dec_stages() {
+  return D == 128 ? 3 : D == 64 ? 6 : 8;
+}
+template <int D>
+constexpr int dec_tile_bytes() {
+  return DEC_TILE * D * 2;
+}
+template <int D>
+struct DecSmem {
+  static constexpr int ST = dec_stages<D>();
+  static constexpr int RING = ST * 2 * dec_tile_bytes<D>();
+  static constexpr int BASE = RING;                      // first logical key of each 16 of a tile
+  static constexpr int BARS = BASE + ST * 4 * 4;         // full, empty
+  static constexpr int BYTES = BARS + ST * 2 * 8 + 64 + 1024;  // control block; room to align the ring
+  // after the last tile: joined state of the block, then the warps' states
+  static constexpr int O_BLOCK = 0;                      // [16][D] fp32
+  static constexpr int ML_BLOCK = 16 * D * 4;            // [2][16]
+  static constexpr int O_WARP = ML_BLOCK + 128;          // [4][16][D]
+  static constexpr int ML_WARP = O_WARP + 4 * 16 * D * 4;  // [4][2][16]
+  static_assert(ML_WARP + 4 * 128 <= RING, "the states reuse the ring");
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <int DT>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == 0) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+// Byte offset of 16-byte chunk c (8 columns) of row r in a 64-row tile as the
+// TMA's swizzle leaves it.
+template <int D>
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  if constexpr (D == 32) return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  else return uint32_t((c >> 3) * (DEC_TILE * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(DEC_THREADS)
+    fa_sparse_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                            const __grid_constant__ SparseArgs a) {
+  using M = DecSmem<D>;
+  constexpr int ST = M::ST;
+  constexpr int NBOX = D == 128 ? 2 : 1;
+  constexpr int KS = D / 16;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  int* key_base = reinterpret_cast<int*>(smem + M::BASE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + M::BARS);
+  uint64_t* empty = full + ST;
+  CtaCtl* ctl = reinterpret_cast<CtaCtl*>(empty + ST);
+  const int S = a.cluster;
+  const int rank = S > 1 ? int(cluster_rank()) : 0;
+  const int G = a.Hq / a.Hkv;
+  const int hblocks = (G + 15) / 16;
+  const int unit = blockIdx.x / S;  // (token, K/V head, block of 16 heads)
+  const int hb = unit % hblocks;
+  const int th = unit / hblocks;
+  const int t = th / a.Hkv, h = th - t * a.Hkv;
+  const int rows = min(16, G - hb * 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    ctl->abort = 0;
+    ctl->status = a.status;
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, DEC_WARPS);
+    }
+    fence_mbar_init();
+  }
+  const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
+  const int pos = row.pos;
+  __syncthreads();
+
+  const int g8 = lane >> 2, t4 = lane & 3;
+  float o[D / 8][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+  if (warp == DEC_WARPS) {
+    // ---- producer ----
+    const int PR = min(1 << a.page_log2, DEC_TILE);  // rows of a piece
+    const int PT = DEC_TILE / PR;                    // pieces of a tile
+    const int sub_log2 = max(0, a.page_log2 - 6);    // pieces of a page
+    const int pieces = pos < 0 ? 0 : a.top << sub_log2;
+    const int tiles = (pieces + PT - 1) / PT;
+    const int mine = tiles > rank ? (tiles - rank + S - 1) / S : 0;  // tiles rank, rank + S, ...
+    const int* list = a.idx + ((long long)t * a.Hkv + h) * a.top;
+    const int per_batch = 32 / PT;  // tiles whose pieces the warp's lanes look up at once
+    int it = 0;
+    bool ok = true;
+    for (int t0 = 0; t0 < mine && ok; t0 += per_batch) {
+      // lane j: piece j % PT of tile t0 + j / PT
+      const int lt = t0 + lane / PT;
+      const int piece = (lt * S + rank) * PT + lane % PT;
+      int base = NO_KEY, at = 0;  // first logical key; row in the cache
+      if (lt < mine && piece < pieces) {
+        const int e = __ldg(list + (piece >> sub_log2));
+        const int sub = piece & ((1 << sub_log2) - 1);
+        if (e >= 0 && e < a.width) {
+          const int first = (e << a.page_log2) + sub * DEC_TILE;
+          if (first <= pos) {
+            const int id = __ldg(a.table + (long long)row.b * a.width + e);
+            if (id >= 0 && id < a.num_pages) {
+              base = first;
+              at = (id << a.page_log2) + sub * DEC_TILE;
+            } else if (a.status) {
+              atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+            }
+          }
+        }
+      }
+      const uint32_t there = __ballot_sync(0xffffffffu, base != NO_KEY);
+      for (int i = 0; i < per_batch && t0 + i < mine; ++i) {
+        const uint32_t have = (there >> (i * PT)) & ((1u << PT) - 1u);
+        if (have == 0) continue;
+        const int s = it % ST;
+        if (it >= ST && !mbar_wait_warp(empty + s, uint32_t(it / ST - 1) & 1, ctl, 96)) {
+          ok = false;
+          break;
+        }
+        // lane j: copy j % (2 NBOX) of piece j / (2 NBOX): K or V, 64 columns
+        const int pc = lane / (2 * NBOX);
+        const int src = i * PT + min(pc, PT - 1);
+        const int pb = __shfl_sync(0xffffffffu, base, src);
+        const int pa = __shfl_sync(0xffffffffu, at, src);
+        const int b16 = __shfl_sync(0xffffffffu, base, i * PT + min(lane * 16 / PR, PT - 1));
+        if (lane < 4) key_base[s * 4 + lane] = b16 == NO_KEY ? NO_KEY : b16 + (lane * 16) % PR;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(full + s, uint32_t(__popc(have)) * uint32_t(PR * D * 2 * 2));
+        __syncwarp();
+        if (pc < PT && pb != NO_KEY) {
+          const int what = lane % (2 * NBOX);
+          const int box = what % NBOX;
+          unsigned char* tile = smem + (s * 2 + (what / NBOX)) * dec_tile_bytes<D>();
+          tma_load_4d(tile + box * (DEC_TILE * 128) + pc * PR * (D >= 64 ? 128 : 64), what < NBOX ? &tmap_k : &tmap_v,
+                      full + s, box * 64, pa, h, 0);
+        }
+        ++it;
+      }
+    }
+    // one more turn of the ring that says there is nothing more
+    if (ok) {
+      const int s = it % ST;
+      if (it < ST || mbar_wait_warp(empty + s, uint32_t(it / ST - 1) & 1, ctl, 97)) {
+        if (lane < 4) key_base[s * 4 + lane] = -1;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + s);
+      } else {
+        ok = false;
+      }
+    }
+    if (!ok || *(volatile int*)&ctl->abort) {
+      for (int i = it > ST ? it - ST : 0; i < it; ++i)  // its copies land before the block goes
+        mbar_wait_drain(full + i % ST, uint32_t(i / ST) & 1, ctl, 98);
+      __syncwarp();
+    }
+  } else {
+    // ---- consumer: keys 16 warp .. of each tile ----
+    uint32_t qf[KS][4];
+    {
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + ((long long)h * G + hb * 16) * a.q_sh;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = g8 + (j & 1) * 8, c = ks * 16 + (j >> 1) * 8 + t4 * 2;
+          qf[ks][j] = r < rows && pos >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_sh + c)) : 0u;
+        }
+    }
+    const int row0 = warp * 16;
+    for (int it = 0;; ++it) {
+      const int s = it % ST;
+      if (!mbar_wait_warp(full + s, uint32_t(it / ST) & 1, ctl, 99)) break;
+      const int base = key_base[s * 4 + warp];
+      if (base == -1) break;
+      const int seen = base == NO_KEY ? 0 : max(0, min(16, pos - base + 1));
+      if (seen > 0) {
+        unsigned char* kt = smem + s * 2 * dec_tile_bytes<D>();
+        unsigned char* vt = kt + dec_tile_bytes<D>();
+        const uint32_t ka = smem_u32(kt), va = smem_u32(vt);
+        float sc[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[0][j] = sc[1][j] = 0.f;
+        const int mi = lane >> 3, mr = lane & 7;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t b[4];
+          ldmatrix4(ka + tile_off<D>(row0 + (mi >> 1) * 8 + mr, ks * 2 + (mi & 1)), b);
+          mma16816<DT>(sc[0], qf[ks], b[0], b[1]);
+          mma16816<DT>(sc[1], qf[ks], b[2], b[3]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[nt][j] *= a.scale_log2;
+        if (seen < 16) {
+          // keys past the token's position: no score, and zeros for their
+          // values, which may be anything and would meet a zero weight
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (nt * 8 + t4 * 2 + (j & 1) >= seen) sc[nt][j] = -INFINITY;
+          for (int i = lane; i < (16 - seen) * (D / 8); i += 32)
+            *reinterpret_cast<uint4*>(vt + tile_off<D>(row0 + seen + i / (D / 8), i % (D / 8))) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
+        float mx[2], al[2];
+        bool same = true;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          x = fmaxf(m[r], x);
+          same = same && x == m[r];
+          const float ref = x == -INFINITY ? 0.f : x;  // no finite score so far: weights of zero
+          al[r] = ex2(m[r] - ref);
+          m[r] = x;
+          mx[r] = ref;
+        }
+        if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) l[r] *= al[r];
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][0] *= al[0], o[i][1] *= al[0];
+            o[i][2] *= al[1], o[i][3] *= al[1];
+          }
+        }
+        float p[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            p[nt][j] = ex2(sc[nt][j] - mx[j >> 1]);
+            l[j >> 1] += p[nt][j];
+          }
+        // the weights as the second product's operand: rounded to its type,
+        // at most half a step of a value in [0, 1]
+        const uint32_t pf[4] = {pack2<DT>(p[0][0], p[0][1]), pack2<DT>(p[0][2], p[0][3]), pack2<DT>(p[1][0], p[1][1]),
+                                pack2<DT>(p[1][2], p[1][3])};
+#pragma unroll
+        for (int np = 0; np < D / 16; ++np) {
+          uint32_t b[4];
+          ldmatrix4_t(va + tile_off<D>(row0 + (mi & 1) * 8 + mr, np * 2 + (mi >> 1)), b);
+          mma16816<DT>(o[2 * np], pf, b[0], b[1]);
+          mma16816<DT>(o[2 * np + 1], pf, b[2], b[3]);
+        }
+        if (seen < 16) fence_proxy_async_smem();  // zeros written before the next copy lands there
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + s);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+  }
+  __syncthreads();  // the ring is free
+  float* ml_warp = reinterpret_cast<float*>(smem + M::ML_WARP);
+  float* o_warp = reinterpret_cast<float*>(smem + M::O_WARP);
+  float* ml_block = reinterpret_cast<float*>(smem + M::ML_BLOCK);
+  float* o_block = reinterpret_cast<float*>(smem + M::O_BLOCK);
+  if (warp < DEC_WARPS) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      if (g8 + r * 8 < rows) {
+        if (t4 == 0) {
+          ml_warp[warp * 32 + g8 + r * 8] = m[r];
+          ml_warp[warp * 32 + 16 + g8 + r * 8] = l[r];
+        }
+        float* dst = o_warp + (warp * 16 + g8 + r * 8) * D + t4 * 2;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+      }
+  }
+  __syncthreads();
+  // the block's state: rows x D / 4 vectors over the threads
+  for (int i = threadIdx.x; i < rows * (D / 4); i += DEC_THREADS) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < DEC_WARPS; ++w) mm = fmaxf(mm, ml_warp[w * 32 + r]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < DEC_WARPS; ++w) {
+      const float x = ex2(ml_warp[w * 32 + r] - ref);
+      ll += x * ml_warp[w * 32 + 16 + r];
+      const float4 v = *reinterpret_cast<const float4*>(o_warp + (w * 16 + r) * D + c);
+      acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
+    }
+    *reinterpret_cast<float4*>(o_block + r * D + c) = acc;
+    if (c == 0) {
+      ml_block[r] = mm;
+      ml_block[16 + r] = ll;
+    }
+  }
+  if (S > 1) cluster_sync();
+  else __syncthreads();
+  // the cluster's state: each block joins its share of the columns
+  uint16_t* out = static_cast<uint16_t*>(a.o) + ((long long)t * a.Hq + h * G + hb * 16) * D;
+  const uint32_t o_addr = smem_u32(o_block), ml_addr = smem_u32(ml_block);
+  const int vecs = rows * (D / 4);
+  for (int i = rank + S * int(threadIdx.x); i < vecs; i += S * DEC_THREADS) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float mm = -INFINITY;
+    for (int k = 0; k < S; ++k)
+      mm = fmaxf(mm, S > 1 ? ld_cluster_f32(cluster_map(ml_addr + r * 4, k)) : ml_block[r]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < S; ++k) {
+      const float mk = S > 1 ? ld_cluster_f32(cluster_map(ml_addr + r * 4, k)) : ml_block[r];
+      const float lk = S > 1 ? ld_cluster_f32(cluster_map(ml_addr + 64 + r * 4, k)) : ml_block[16 + r];
+      const float4 v = S > 1 ? ld_cluster_f4(cluster_map(o_addr + (r * D + c) * 4, k))
+                             : *reinterpret_cast<const float4*>(o_block + r * D + c);
+      const float x = ex2(mk - ref);
+      ll += x * lk;
+      acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
+    }
+    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);  // no key: zeros; NaN stays
+    *reinterpret_cast<uint2*>(out + r * D + c) =
+        make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+  }
+  if (S > 1) cluster_sync();  // the others have read this block's state
+}
+
+// A launch in clusters of S blocks (1: none).
+template <class... Params, class... Args>
+int launch_clustered(void (*kernel)(Params...), unsigned blocks, unsigned threads, size_t smem, int S,
+                     cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = unsigned(S);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+template <int D, int DT>
+int run_sparse(const SparseArgs& a, const CUtensorMap& k, const CUtensorMap& v) {
+  auto* kernel = fa_sparse_decode_kernel<D, DT>;
+  const int smem = DecSmem<D>::BYTES;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return FA_ERR_LAUNCH;
+  const int G = a.Hq / a.Hkv;
+  const long long units = (long long)a.total_q * a.Hkv * ((G + 15) / 16);
+  if (units * a.cluster > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
+  return launch_clustered(kernel, unsigned(units * a.cluster), DEC_THREADS, size_t(smem), a.cluster, a.stream, k, v, a);
+}
+
+template <int D, int DT>
+int run_select(const SelectArgs& a) {
+  auto* kernel = fa_select_pages_kernel<D, DT>;
+  const int G = a.Hq / a.Hkv;
+  const size_t smem = size_t(G) * D * 8 + size_t(a.share) * 4 + size_t(a.width) * 4;
+  if (smem > size_t(200) << 10) return FA_ERR_BAD_SHAPE;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
+    return FA_ERR_LAUNCH;
+  const long long units = (long long)a.total_q * a.Hkv;
+  if (units * a.cluster > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
+  return launch_clustered(kernel, unsigned(units * a.cluster), SEL_THREADS, smem, a.cluster, a.stream, a);
+}
+
+// Largest power of two up to 8 that still leaves every block `least` pieces
+// of a unit's work and does not go past what the GPU holds at once.
+int cluster_for(long long units, long long pieces, int least, int per_sm) {
+  const long long slots = (long long)device_sm_count() * per_sm;
+  int S = 1;
+  while (S < 8 && units * S < slots && pieces >= 2LL * S * least) S *= 2;
+  return S;
+}
+
+}  // namespace
+
+int launch_page_means(const PageArgs& a, int total_q) {
+  const long long units = (long long)(total_q >> a.page_log2) + a.B;
+  const long long cap = (long long)device_sm_count() * 4;
+  const unsigned ctas = unsigned(units < cap ? units : cap);
+  const int W8 = a.Hkv * a.D / 8;
+  const int cols = W8 < MEAN_THREADS ? W8 : MEAN_THREADS;
+  const int groups = MEAN_THREADS / cols < 8 ? MEAN_THREADS / cols : 8;
+  const size_t smem = size_t(groups - 1) * 8 * cols * 8;
+  if (units > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
+  if (a.dtype == DT_BF16) fa_page_means_kernel<DT_BF16><<<ctas, MEAN_THREADS, smem, a.stream>>>(a, int(units));
+  else fa_page_means_kernel<DT_F16><<<ctas, MEAN_THREADS, smem, a.stream>>>(a, int(units));
+  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int launch_select_pages(SelectArgs a, int D) {
+  a.cluster = cluster_for((long long)a.total_q * a.Hkv, a.width, 64, 2);
+  a.share = (a.width + a.cluster - 1) / a.cluster;
+  if (a.dtype == DT_BF16)
+    return D == 32 ? run_select<32, DT_BF16>(a) : D == 64 ? run_select<64, DT_BF16>(a) : run_select<128, DT_BF16>(a);
+  return D == 32 ? run_select<32, DT_F16>(a) : D == 64 ? run_select<64, DT_F16>(a) : run_select<128, DT_F16>(a);
+}
+
+int launch_sparse_decode(SparseArgs a, const CUtensorMap& k, const CUtensorMap& v, int D) {
+  const int G = a.Hq / a.Hkv;
+  const long long tiles = (((long long)a.top << a.page_log2) + DEC_TILE - 1) / DEC_TILE;
+  a.cluster = cluster_for((long long)a.total_q * a.Hkv * ((G + 15) / 16), tiles, 2, 2);
+  if (a.dtype == DT_BF16)
+    return D == 32 ? run_sparse<32, DT_BF16>(a, k, v)
+                   : D == 64 ? run_sparse<64, DT_BF16>(a, k, v) : run_sparse<128, DT_BF16>(a, k, v);
+  return D == 32 ? run_sparse<32, DT_F16>(a, k, v)
+                 : D == 64 ? run_sparse<64, DT_F16>(a, k, v) : run_sparse<128, DT_F16>(a, k, v);
+}
+
+}  // namespace fa

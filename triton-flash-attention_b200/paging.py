@@ -1,0 +1,368 @@
+"""A serving step over a paged K/V cache, around the paged attention call.
+
+No counterpart in the reference, which has no cache.  In the order of a step:
+
+* ``extend_block_table`` gives the step's new tokens their pages, cache slots,
+  positions and offsets, on the GPU, from the requests' lengths;
+* ``paged_append`` norms and rotates the new queries and keys
+  (``rotary.py``) and writes keys and values into the cache;
+* then ``scaled_dot_product_attention_paged`` (``varlen.py``) over all of the
+  cache, or attention over a part of it: ``update_page_means`` keeps the mean
+  key of every full page, ``select_pages`` scores the pages by it for each
+  token and K/V head, and ``scaled_dot_product_attention_paged_sparse``
+  attends to the selected pages only.
+
+All are forward only and capture into CUDA graphs: nothing is read back, and
+rows of a padded batch behind the last request are left alone.  Indices that
+would reach outside a tensor are refused on the GPU (nothing is read or
+written there) and set the device status (``_abi.device_status``).
+"""
+
+from __future__ import annotations
+
+import math
+from numbers import Real
+from typing import NamedTuple
+
+import torch
+
+from . import _abi
+from .attention import _stream_handle
+from .rotary import _ptr, _strides, check_backend, check_eps, check_table, check_weights, on_device, vector_rows
+
+# block-table width that select_pages takes (FA_MAX_SELECT_PAGES of include/fa_b200.h)
+MAX_SELECT_PAGES = 16384
+
+
+def _check_page_size(page_size) -> None:
+    if isinstance(page_size, bool) or not isinstance(page_size, int) or page_size < 16 or page_size & (page_size - 1):
+        raise ValueError("page_size must be a power of two of at least 16")
+
+
+def _check_int32(name: str, t, ndim: int, device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.ndim != ndim or t.dtype != torch.int32 or t.device != device:
+        raise ValueError(f"{name} must be a {ndim}-D int32 tensor on the same device as the others")
+
+
+def _check_cache(name: str, t, like=None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.ndim != 4 or 0 in t.shape:
+        raise ValueError(f"{name} must have shape (num_pages, page_size, heads, head_dim); got {tuple(t.shape)}")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be contiguous and start on a 16-byte boundary")
+    if t.shape[0] * t.shape[1] > 0x7fffffff:
+        raise ValueError(f"{name} must have fewer than 2**31 slots")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise ValueError("k_cache and v_cache must have the same shape, dtype and device")
+
+
+def _check_no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the paged K/V path is forward only; run it under torch.no_grad()")
+
+
+class PagedStep(NamedTuple):
+    """What ``extend_block_table`` returns; all on the GPU.  ``cu_seqlens_q``
+    (requests + 1,), ``seqlens_k`` (requests,), ``positions`` and
+    ``slot_mapping`` (total_q,), ``free_next`` (1,) int32; ``fits``
+    (requests,) bool."""
+
+    cu_seqlens_q: torch.Tensor
+    seqlens_k: torch.Tensor
+    positions: torch.Tensor
+    slot_mapping: torch.Tensor
+    fits: torch.Tensor
+    free_next: torch.Tensor
+
+
+def extend_block_table(block_table, seqlens_cached, seqlens_new, free_pages, free_start, *, page_size: int,
+                       total_q: int) -> PagedStep:
+    """Make room in the cache for a step's new tokens.
+
+    ``block_table``: int32 ``(requests, max_pages)``, the first
+    ``ceil(seqlens_cached / page_size)`` entries of a row its pages; the new
+    ones are appended in place, other entries stay as they are.
+    ``seqlens_cached``, ``seqlens_new``: int32 ``(requests,)``, tokens in the
+    cache and new ones (either may be 0; negative counts as 0).
+    ``free_pages``: int32 page ids; those from entry ``free_start[0]`` on are
+    free and are taken in order, ``free_next`` is the start for the next step.
+    ``total_q``: rows of the packed batch, at least the sum of
+    ``seqlens_new``; rows behind the last request get position 0 and slot -1.
+
+    A request that needs more pages than its row has, or rows behind
+    ``total_q``, takes nothing; when the free pages run out, the request that
+    lacks them and all after it take nothing.  Such a request has ``fits``
+    False, slots of -1 and the ``seqlens_k`` it had."""
+    if not isinstance(block_table, torch.Tensor):
+        raise TypeError("block_table must be a torch.Tensor")
+    dev = block_table.device
+    _check_int32("block_table", block_table, 2, dev)
+    for name, t in (("seqlens_cached", seqlens_cached), ("seqlens_new", seqlens_new), ("free_pages", free_pages),
+                    ("free_start", free_start)):
+        _check_int32(name, t, 1, dev)
+    requests, width = block_table.shape
+    if requests == 0 or width == 0:
+        raise ValueError("block_table dimensions must all be greater than zero")
+    if not block_table.is_contiguous():
+        raise ValueError("block_table must be contiguous (it is extended in place)")
+    if seqlens_cached.shape[0] != requests or seqlens_new.shape[0] != requests:
+        raise ValueError("seqlens_cached and seqlens_new must have one entry per row of block_table")
+    if free_start.shape[0] != 1:
+        raise ValueError("free_start must have one entry")
+    _check_page_size(page_size)
+    if width * page_size > 0x7fffffff:
+        raise ValueError("max_pages * page_size must be below 2**31")
+    if isinstance(total_q, bool) or not isinstance(total_q, int) or not 0 <= total_q <= 0x7fffffff:
+        raise ValueError("total_q must be a non-negative int")
+    if dev.type != "cuda":
+        raise RuntimeError("B200 CUDA backend is unavailable: the B200 kernel requires a CUDA tensor")
+    seqlens_cached, seqlens_new, free_pages = (t.contiguous() for t in (seqlens_cached, seqlens_new, free_pages))
+    with on_device(block_table):
+        # one allocation for the int32 outputs, each part on a 16-byte boundary
+        a, b, c = (requests + 4) // 4 * 4, (requests + 3) // 4 * 4, (total_q + 3) // 4 * 4
+        out = torch.empty(a + b + 2 * c + 1, device=dev, dtype=torch.int32)
+        cu, sk, pos, slots, nxt = (out[:requests + 1], out[a:a + requests], out[a + b:a + b + total_q],
+                                   out[a + b + c:a + b + c + total_q], out[a + b + 2 * c:])
+        fits = torch.empty(requests, device=dev, dtype=torch.bool)
+        at = out.data_ptr()
+        rc = _abi.lib().fa_extend_block_table(
+            block_table.data_ptr(), seqlens_cached.data_ptr(), seqlens_new.data_ptr(),
+            free_pages.data_ptr(), free_start.data_ptr(), at, at + 4 * a, at + 4 * (a + b),
+            at + 4 * (a + b + c), fits.data_ptr(), at + 4 * (a + b + 2 * c), requests, width, free_pages.shape[0],
+            page_size, total_q, _stream_handle(dev))
+    _abi.check(rc, "fa_extend_block_table")
+    return PagedStep(cu, sk, pos, slots, fits, nxt)
+
+
+def paged_append(query, key, value, k_cache, v_cache, slot_mapping, table, positions, *, query_weight=None,
+                 key_weight=None, eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+    """Norm and rotate a step's packed queries and keys as ``qk_norm_rotary``
+    does, write keys and values to the cache and return the queries, all in
+    one pass.
+
+    ``query``: ``(total, Hq, D)``; ``key``, ``value``: ``(total, Hkv, D)``;
+    views of a fused projection are read in place.  ``k_cache``, ``v_cache``:
+    contiguous ``(num_pages, page_size, Hkv, D)``, written in place at row
+    ``slot_mapping[t]`` (int32, ``page * page_size + row``) of their
+    ``num_pages * page_size`` rows; a slot of -1 writes nothing.  Slots of one
+    call must differ.  ``positions``: int32 ``(total,)``.  The weights, ``eps``
+    and ``interleaved`` as in ``qk_norm_rotary``."""
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.ndim != 3 or 0 in t.shape:
+            raise ValueError(f"{name} must have shape (total, heads, head_dim), no dimension zero; "
+                             f"got {tuple(t.shape)}")
+        if t.dtype != query.dtype or t.device != query.device:
+            raise ValueError("query, key, and value must have the same dtype and device")
+    total, hq, d = query.shape
+    if key.shape != value.shape:
+        raise ValueError("key and value must have the same shape")
+    if key.shape[0] != total or key.shape[2] != d:
+        raise ValueError("query and key must have the same number of rows and head dimension")
+    _check_cache("k_cache", k_cache)
+    _check_cache("v_cache", v_cache, k_cache)
+    if k_cache.shape[2:] != key.shape[1:] or k_cache.dtype != query.dtype or k_cache.device != query.device:
+        raise ValueError("the caches must have the key's heads, head dimension, dtype and device")
+    for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):
+        _check_int32(name, t, 1, query.device)
+        if t.shape[0] != total:
+            raise ValueError(f"{name} must have one entry per row of query")
+    if not isinstance(interleaved, bool):
+        raise TypeError("interleaved must be a bool")
+    check_eps(eps)
+    check_table(table, d, query.device)
+    check_weights(query_weight, key_weight, query)
+    _check_no_grad(query, key, value, query_weight, key_weight)
+    check_backend(query)
+    q, k, v = vector_rows(query), vector_rows(key), vector_rows(value)
+    slots, pos = slot_mapping.contiguous(), positions.contiguous()
+    if query_weight is not None:
+        query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
+    with on_device(q):
+        out = torch.empty((total, hq, d), device=q.device, dtype=q.dtype)
+        rc = _abi.entry("fa_paged_append", q.dtype)(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            slots.data_ptr(), table.data_ptr(), pos.data_ptr(), _ptr(query_weight), _ptr(key_weight), total, hq,
+            k.shape[1], d, k_cache.shape[0] * k_cache.shape[1], table.shape[0], table.shape[1], interleaved,
+            query_weight is not None and query_weight.dtype == torch.float32, _strides(q), _strides(k), _strides(v),
+            float(eps), _stream_handle(q.device))
+    _abi.check(rc, "fa_paged_append")
+    return out
+
+
+def _check_step(block_table, cu_seqlens_q, seqlens_k, device) -> None:
+    _check_int32("block_table", block_table, 2, device)
+    _check_int32("cu_seqlens_q", cu_seqlens_q, 1, device)
+    _check_int32("seqlens_k", seqlens_k, 1, device)
+    if 0 in block_table.shape:
+        raise ValueError("block_table dimensions must all be greater than zero")
+    if cu_seqlens_q.shape[0] != block_table.shape[0] + 1 or seqlens_k.shape[0] != block_table.shape[0]:
+        raise ValueError("block_table and seqlens_k must have one row per sequence of cu_seqlens_q")
+
+
+def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k, *, total_q: int | None = None):
+    """Write the mean key of every page that a step's tokens completed.
+
+    ``k_cache``: contiguous ``(num_pages, page_size, Hkv, D)``, the step's keys
+    included; ``page_means``: contiguous ``(num_pages, Hkv, D)`` in the cache's
+    type, updated in place at the completed pages and returned.
+    ``block_table``, ``cu_seqlens_q``, ``seqlens_k`` as in
+    ``scaled_dot_product_attention_paged``: the rows of a sequence are its
+    last keys.  ``total_q``: rows of the packed batch when the caller has it;
+    None takes room for a step that fills the table.  Means are summed in 64
+    bits and do not depend on the order of the sum."""
+    _check_cache("k_cache", k_cache)
+    num_pages, page_size, hkv, d = k_cache.shape
+    _check_page_size(page_size)
+    if not isinstance(page_means, torch.Tensor):
+        raise TypeError("page_means must be a torch.Tensor")
+    if (tuple(page_means.shape) != (num_pages, hkv, d) or page_means.dtype != k_cache.dtype
+            or page_means.device != k_cache.device or not page_means.is_contiguous() or page_means.data_ptr() % 16):
+        raise ValueError("page_means must be a contiguous (num_pages, heads, head_dim) tensor of the cache's dtype "
+                         "and device")
+    _check_step(block_table, cu_seqlens_q, seqlens_k, k_cache.device)
+    batch, width = block_table.shape
+    if width * page_size > 0x7fffffff:
+        raise ValueError("max_pages_per_seq * page_size must be below 2**31")
+    if total_q is None:
+        total_q = min(batch * width * page_size, 0x7fffffff)
+    elif isinstance(total_q, bool) or not isinstance(total_q, int) or not 0 < total_q <= 0x7fffffff:
+        raise ValueError("total_q must be a positive int or None")
+    _check_no_grad(k_cache, page_means)
+    check_backend(k_cache)
+    table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
+    with on_device(k_cache):
+        rc = _abi.entry("fa_page_means", k_cache.dtype)(
+            k_cache.data_ptr(), page_means.data_ptr(), table.data_ptr(),
+            cu.data_ptr(), lens.data_ptr(), batch, hkv, d, num_pages,
+            page_size, width, total_q, _stream_handle(k_cache.device))
+    _abi.check(rc, "fa_page_means")
+    return page_means
+
+
+def _check_query(query) -> None:
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a torch.Tensor")
+    if query.ndim != 3:
+        raise ValueError(f"query must have shape (total, heads, head_dim); got {tuple(query.shape)}")
+    if 0 in query.shape:
+        raise ValueError("query dimensions must all be greater than zero")
+
+
+def select_pages(query, page_means, block_table, cu_seqlens_q, seqlens_k, *, page_size: int, num_selected: int,
+                 sink_pages: int = 1, local_pages: int = 1) -> torch.Tensor:
+    """Choose the pages that each new token attends to.
+
+    ``query``: packed ``(total_q, Hq, D)``, as it enters the attention;
+    ``page_means``: ``update_page_means``'s, up to date for every full page.
+    A page's score for a token and K/V head is the highest dot product of one
+    of the group's query heads with the page's mean key, summed in 64 bits and
+    rounded to fp32.  Kept are the first ``sink_pages`` pages of the sequence,
+    the ``local_pages`` up to and with the token's own, and those of the
+    highest score (of equal ones the lower page; NaN is the lowest) up to
+    ``num_selected`` in all.  Returns int32 ``(total_q, Hkv, num_selected)``:
+    page indices in the sequence, ascending, -1 behind the last; all pages up
+    to the token's own when there are no more than ``num_selected``."""
+    _check_query(query)
+    if not isinstance(page_means, torch.Tensor):
+        raise TypeError("page_means must be a torch.Tensor")
+    total, hq, d = query.shape
+    if (page_means.ndim != 3 or 0 in page_means.shape or page_means.shape[2] != d or page_means.dtype != query.dtype
+            or page_means.device != query.device or not page_means.is_contiguous() or page_means.data_ptr() % 16):
+        raise ValueError("page_means must be a contiguous (num_pages, heads, head_dim) tensor of the query's head "
+                         "dimension, dtype and device")
+    hkv = page_means.shape[1]
+    if hq % hkv:
+        raise ValueError("the number of query heads must be divisible by the number of key/value heads")
+    _check_step(block_table, cu_seqlens_q, seqlens_k, query.device)
+    _check_page_size(page_size)
+    batch, width = block_table.shape
+    if width > MAX_SELECT_PAGES:
+        raise ValueError(f"block_table may be {MAX_SELECT_PAGES} pages wide for page selection; got {width}")
+    if width * page_size > 0x7fffffff or page_means.shape[0] * page_size > 0x7fffffff:
+        raise ValueError("page counts times page_size must be below 2**31")
+    for name, v, least in (("num_selected", num_selected, 1), ("sink_pages", sink_pages, 0),
+                           ("local_pages", local_pages, 1)):
+        if isinstance(v, bool) or not isinstance(v, int) or v < least:
+            raise ValueError(f"{name} must be an int of at least {least}")
+    if sink_pages + local_pages > num_selected:
+        raise ValueError("sink_pages + local_pages must not be above num_selected")
+    if num_selected * page_size > 0x3fffffff:
+        raise ValueError("num_selected * page_size must be below 2**30")
+    _check_no_grad(query, page_means)
+    check_backend(query)
+    q = vector_rows(query)
+    table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
+    with on_device(q):
+        out = torch.empty((total, hkv, num_selected), device=q.device, dtype=torch.int32)
+        rc = _abi.entry("fa_select_pages", q.dtype)(
+            q.data_ptr(), page_means.data_ptr(), table.data_ptr(),
+            cu.data_ptr(), lens.data_ptr(), out.data_ptr(), batch, hq, hkv,
+            d, total, page_means.shape[0], page_size, width, num_selected, sink_pages, local_pages, _strides(q),
+            _stream_handle(q.device))
+    _abi.check(rc, "fa_select_pages")
+    return out
+
+
+def scaled_dot_product_attention_paged_sparse(query, k_cache, v_cache, block_table, cu_seqlens_q, seqlens_k,
+                                              page_indices, *, scale: float | None = None,
+                                              enable_gqa: bool = False) -> torch.Tensor:
+    """Attention of packed queries over listed pages of a paged K/V cache
+    (forward only; made for decode, where each sequence brings one query or a
+    few).
+
+    ``query``, the caches, ``block_table``, ``cu_seqlens_q`` and ``seqlens_k``
+    as in ``scaled_dot_product_attention_paged`` with ``is_causal=True``: row
+    ``i`` of a sequence's ``nq`` sees its keys ``j <= i + nk - nq``.
+    ``page_indices``: int32 ``(total_q, Hkv, n)``, for each row and K/V head
+    the pages it attends to by their index in the sequence, as
+    ``select_pages`` returns them; -1 and pages behind the row's own are
+    skipped, and a page listed twice counts twice.  Rows that see no listed
+    key, and rows behind the last sequence, get zeros.  Cache rows behind a
+    token's position may hold anything.  The default ``scale`` is
+    ``D ** -0.5``."""
+    _check_query(query)
+    if not isinstance(enable_gqa, bool):
+        raise TypeError("enable_gqa must be a bool")
+    if scale is not None and (not isinstance(scale, Real) or not math.isfinite(float(scale))):
+        raise ValueError("scale must be a finite real number or None")
+    _check_cache("k_cache", k_cache)
+    _check_cache("v_cache", v_cache, k_cache)
+    total, hq, d = query.shape
+    num_pages, page_size, hkv, cache_d = k_cache.shape
+    _check_page_size(page_size)
+    if cache_d != d or k_cache.dtype != query.dtype or k_cache.device != query.device:
+        raise ValueError("the caches must have the query's head dimension, dtype and device")
+    if hq != hkv and not enable_gqa:
+        raise ValueError(
+            "query has a different number of heads from key/value; pass "
+            "enable_gqa=True to use grouped-query attention")
+    if hq % hkv:
+        raise ValueError("the number of query heads must be divisible by the number of key/value heads")
+    _check_step(block_table, cu_seqlens_q, seqlens_k, query.device)
+    _check_int32("page_indices", page_indices, 3, query.device)
+    batch, width = block_table.shape
+    n = page_indices.shape[2]
+    if tuple(page_indices.shape[:2]) != (total, hkv) or n == 0:
+        raise ValueError("page_indices must have shape (total_q, key/value heads, n)")
+    if width * page_size > 0x7fffffff or n * page_size > 0x3fffffff:
+        raise ValueError("block_table and page_indices are too wide for this page_size")
+    _check_no_grad(query, k_cache, v_cache)
+    check_backend(query)
+    q = vector_rows(query)
+    table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
+    pages = page_indices.contiguous()
+    with on_device(q):
+        out = torch.empty((total, hq, d), device=q.device, dtype=q.dtype)
+        rc = _abi.entry("fa_fwd_paged_sparse", q.dtype)(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+            table.data_ptr(), cu.data_ptr(),
+            lens.data_ptr(), pages.data_ptr(), batch, hq, hkv, d, total,
+            num_pages, page_size, width, n, float(scale) if scale is not None else d ** -0.5, _strides(q),
+            _stream_handle(q.device))
+    _abi.check(rc, "fa_fwd_paged_sparse")
+    return out

@@ -1,0 +1,258 @@
+"""Queries and keys on their way into the attention: a root-mean-square norm
+of every head and the rotation by the token's position, in one pass.
+
+No counterpart in the reference, whose API takes queries and keys as they
+enter the product (triton_flash_attention/attention.py:584-626).  For a row
+``x`` of ``D`` values (one head of one token)::
+
+    y = x / sqrt(mean(x^2) + eps) * weight
+    y'[a] = y[a] cos - y[b] sin,   y'[b] = y[b] cos + y[a] sin
+
+for the column pairs ``(a, b)`` of the first ``rotary_dim`` columns; columns
+behind them keep ``y``.  Both steps run in fp32 and the result is rounded
+once.  ``qk_norm_rotary`` supports autograd; ``paged_append`` (``paging.py``)
+is the same preparation for serving, with keys and values written to a paged
+cache.
+"""
+
+from __future__ import annotations
+
+import math
+from numbers import Real
+
+import torch
+
+from . import _abi
+from .attention import SUPPORTED_DTYPES, SUPPORTED_HEAD_DIMS, _device_capability, _stream_handle
+
+# rows of the partial weight gradients (FA_ROTARY_PARTIALS of include/fa_b200.h)
+ROTARY_PARTIALS = 592
+
+
+def rotary_table(max_positions: int, rotary_dim: int, *, base: float = 10000.0, device=None) -> torch.Tensor:
+    """The ``(max_positions, rotary_dim)`` fp32 table that the rotating calls
+    take: for each position the ``rotary_dim / 2`` cosines, then the sines, of
+    ``position * base ** (-2 i / rotary_dim)``, from 64-bit angles (far
+    positions need them).  Made once and kept; any other frequencies can be
+    put in a table of the same layout."""
+    for name, v in (("max_positions", max_positions), ("rotary_dim", rotary_dim)):
+        if isinstance(v, bool) or not isinstance(v, int) or v <= 0:
+            raise ValueError(f"{name} must be a positive int")
+    if rotary_dim % 16:
+        raise ValueError("rotary_dim must be a multiple of 16")
+    if isinstance(base, bool) or not isinstance(base, Real) or not math.isfinite(base) or base <= 0:
+        raise ValueError("base must be a finite positive number")
+    freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def check_backend(tensor: torch.Tensor) -> None:
+    """Raises unless the B200 kernels serve tensors of this device, type and
+    head dim, with the messages of the attention calls."""
+    if tensor.device.type != "cuda":
+        raise RuntimeError("B200 CUDA backend is unavailable: the B200 kernel requires a CUDA tensor")
+    if tensor.dtype not in SUPPORTED_DTYPES:
+        raise RuntimeError("B200 CUDA backend is unavailable: the custom mixed-precision path currently "
+                           "supports float16 and bfloat16")
+    if tensor.shape[-1] not in SUPPORTED_HEAD_DIMS:
+        supported = ", ".join(str(dim) for dim in SUPPORTED_HEAD_DIMS)
+        raise RuntimeError(f"B200 CUDA backend is unavailable: head_dim must be one of ({supported}) "
+                           "for the B200 path")
+    if _device_capability(tensor.device) != (10, 0):
+        raise RuntimeError("B200 CUDA backend is unavailable: the kernels are built for sm_100a (B200) GPUs only")
+
+
+def on_device(tensor: torch.Tensor):
+    """Context in which launches go to the tensor's device: nothing when it is
+    current already."""
+    return torch.cuda.device(tensor.device.index)
+
+
+def vector_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when its rows can be read 16 bytes at a time -- unit
+    stride over the last dimension, the others and the start multiples of 16
+    bytes -- and else a contiguous copy."""
+    s = t.stride()
+    if s[-1] == 1 and not any(x % 8 for x in s[:-1]) and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _strides(t: torch.Tensor):
+    """{batch, head, seq} strides of a (B, H, N, D) or packed (total, H, D)
+    tensor.  Dimensions of one entry get a stride of no consequence."""
+    s = t.stride()
+    key = s[:3] if t.ndim == 4 else (t.shape[0] * t.shape[1] * t.shape[2], s[1], s[0])
+    return _abi.strides_of(key)
+
+
+def check_table(table, rotary_max: int, device) -> None:
+    if not isinstance(table, torch.Tensor):
+        raise TypeError("table must be a torch.Tensor")
+    if table.ndim != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.shape[0] == 0:
+        raise ValueError("table must be a contiguous (max_positions, rotary_dim) float32 tensor")
+    if table.shape[1] == 0 or table.shape[1] % 16 or table.shape[1] > rotary_max:
+        raise ValueError(f"the table's rotary_dim must be a multiple of 16 up to the head dim {rotary_max}; "
+                         f"got {table.shape[1]}")
+    if table.device != device:
+        raise ValueError("table must be on the same device as query")
+    if table.data_ptr() % 16:
+        raise ValueError("table must start on a 16-byte boundary")
+
+
+def check_weights(query_weight, key_weight, query) -> None:
+    if (query_weight is None) != (key_weight is None):
+        raise ValueError("pass both query_weight and key_weight, or neither for the rotation alone")
+    if query_weight is None:
+        return
+    for name, w in (("query_weight", query_weight), ("key_weight", key_weight)):
+        if not isinstance(w, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if w.ndim != 1 or w.shape[0] != query.shape[-1] or w.device != query.device:
+            raise ValueError(f"{name} must be a 1-D tensor of head_dim weights on the query's device")
+        if w.dtype not in (query.dtype, torch.float32):
+            raise ValueError(f"{name} must have the query's dtype or float32")
+    if query_weight.dtype != key_weight.dtype:
+        raise ValueError("query_weight and key_weight must have the same dtype")
+
+
+def check_eps(eps) -> None:
+    if isinstance(eps, bool) or not isinstance(eps, Real) or not 0.0 <= eps < math.inf:
+        raise ValueError("eps must be a finite non-negative number")
+
+
+def _validate(query, key, table, positions, query_weight, key_weight, eps, interleaved) -> None:
+    for name, t in (("query", query), ("key", key)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.ndim not in (3, 4):
+            raise ValueError(f"{name} must have shape (batch, heads, sequence, head_dim) or (total, heads, head_dim); "
+                             f"got {tuple(t.shape)}")
+        if 0 in t.shape:
+            raise ValueError(f"{name} dimensions must all be greater than zero")
+    if query.ndim != key.ndim:
+        raise ValueError("query and key must have the same layout")
+    if query.device != key.device:
+        raise ValueError("query and key must be on the same device")
+    if query.dtype != key.dtype:
+        raise ValueError("query and key must have the same dtype")
+    if query.shape[-1] != key.shape[-1]:
+        raise ValueError("query and key head dimensions must match")
+    dense = query.ndim == 4
+    if dense and (query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]):
+        raise ValueError("query and key batch and sequence dimensions must match")
+    if not dense and query.shape[0] != key.shape[0]:
+        raise ValueError("query and key must have the same number of rows")
+    if not isinstance(interleaved, bool):
+        raise TypeError("interleaved must be a bool")
+    check_eps(eps)
+    check_table(table, query.shape[-1], query.device)
+    check_weights(query_weight, key_weight, query)
+    if positions is None:
+        if not dense:
+            raise ValueError("packed (total, heads, head_dim) tensors need positions")
+    else:
+        if not isinstance(positions, torch.Tensor):
+            raise TypeError("positions must be a torch.Tensor")
+        n = query.shape[2] if dense else query.shape[0]
+        shapes = ((n,), (query.shape[0], n)) if dense else ((n,),)
+        if positions.dtype != torch.int32 or positions.device != query.device or tuple(positions.shape) not in shapes:
+            raise ValueError("positions must be an int32 tensor of the token dimension, or of (batch, sequence) for "
+                             "4-D tensors, on the query's device")
+    check_backend(query)
+
+
+def _sizes(q, k):
+    """(B, Hq, Hkv, N, D)"""
+    if q.ndim == 4:
+        return q.shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[3]
+    return 1, q.shape[1], k.shape[1], q.shape[0], q.shape[2]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def qk_norm_rotary_forward(q, k, table, positions, query_weight, key_weight, eps: float, interleaved: bool):
+    """Launch the forward: contiguous outputs in the inputs' layout."""
+    b, hq, hkv, n, d = _sizes(q, k)
+    with on_device(q):
+        qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        ko = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        rc = _abi.entry("fa_qk_norm_rotary", q.dtype)(
+            q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), table.data_ptr(), _ptr(positions),
+            _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n, d, table.shape[0], table.shape[1],
+            interleaved, query_weight is not None and query_weight.dtype == torch.float32,
+            _strides(q), _strides(k), _strides(qo), _strides(ko),
+            n if positions is not None and positions.ndim == 2 else 0, eps, _stream_handle(q.device))
+    _abi.check(rc, "fa_qk_norm_rotary")
+    return qo, ko
+
+
+def qk_norm_rotary_backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, eps: float,
+                            interleaved: bool, weight_grads: bool = True):
+    """dQ, dK and, with weights and ``weight_grads``, the weights' gradients
+    (else None).  Gradients repeat bit for bit."""
+    b, hq, hkv, n, d = _sizes(q, k)
+    wants = weight_grads and query_weight is not None
+    with on_device(q):
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        dwq = torch.empty_like(query_weight) if wants else None
+        dwk = torch.empty_like(key_weight) if wants else None
+        part = torch.empty(ROTARY_PARTIALS * d, device=q.device, dtype=torch.float32) if wants else None
+        rc = _abi.entry("fa_qk_norm_rotary_bwd", q.dtype)(
+            q.data_ptr(), k.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+            _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions), _ptr(query_weight),
+            _ptr(key_weight), b, hq, hkv, n, d, table.shape[0], table.shape[1], interleaved,
+            query_weight is not None and query_weight.dtype == torch.float32,
+            _strides(q), _strides(k), _strides(grad_q), _strides(grad_k), _strides(dq), _strides(dk),
+            n if positions is not None and positions.ndim == 2 else 0, eps, _stream_handle(q.device))
+    _abi.check(rc, "fa_qk_norm_rotary_bwd")
+    return dq, dk, dwq, dwk
+
+
+class B200QKNormRotary(torch.autograd.Function):
+    """Autograd bridge; saves the inputs only (a row's norm is found again
+    from its values, which the backward reads anyhow)."""
+
+    @staticmethod
+    def forward(ctx, query, key, table, positions, query_weight, key_weight, eps, interleaved):
+        ctx.save_for_backward(query, key, table, positions, query_weight, key_weight)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return qk_norm_rotary_forward(query, key, table, positions, query_weight, key_weight, eps, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_query, grad_key):
+        query, key, table, positions, query_weight, key_weight = ctx.saved_tensors
+        dq, dk, dwq, dwk = qk_norm_rotary_backward(
+            query, key, vector_rows(grad_query), vector_rows(grad_key), table, positions, query_weight, key_weight,
+            ctx.eps, ctx.interleaved, ctx.needs_input_grad[4] or ctx.needs_input_grad[5])
+        return dq, dk, None, None, dwq, dwk, None, None
+
+
+def qk_norm_rotary(query, key, table, positions=None, *, query_weight=None, key_weight=None, eps: float = 1e-6,
+                   interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm and rotate queries and keys for the attention calls.
+
+    ``query``, ``key``: ``(B, Hq, N, D)`` and ``(B, Hkv, N, D)``, or packed
+    ``(total, Hq, D)`` and ``(total, Hkv, D)``; views of a fused projection
+    are read in place.  ``table``: ``rotary_table``'s; its width is the number
+    of columns that turn.  ``positions``: int32, ``(N,)`` or ``(B, N)``, or
+    ``(total,)`` when packed; None counts from 0 (4-D only).  ``query_weight``,
+    ``key_weight``: ``D`` weights each, in the operand type or float32; with
+    both None there is no norm.  ``interleaved`` pairs columns ``(2 i, 2 i +
+    1)`` instead of ``(i, i + rotary_dim / 2)``.  Returns contiguous tensors
+    in the inputs' layout and supports autograd for the queries, keys and
+    weights.
+
+    A position outside the table is found on the GPU: its turned columns are
+    NaN and the device status (``_abi.device_status``) names the error."""
+    _validate(query, key, table, positions, query_weight, key_weight, eps, interleaved)
+    return B200QKNormRotary.apply(
+        vector_rows(query), vector_rows(key), table, None if positions is None else positions.contiguous(),
+        None if query_weight is None else query_weight.contiguous(),
+        None if key_weight is None else key_weight.contiguous(), float(eps), interleaved)
