@@ -705,8 +705,22 @@ int bwd_dense_impl(const void* q, const void* k, const void* v, const void* o, c
 
 int* device_status_word() { return status_ptr(); }
 int make_cache_map(CUtensorMap* map, const void* cache, int cache_rows, int Hkv, int D, int rows, int dtype) {
-  const PackedStrides sk(cache_rows, Hkv, D);
-  return make_map(map, cache, 1, Hkv, cache_rows, D, sk.v, rows, dtype);
+  // as make_map, with the runs of 64 columns as the third dimension and the
+  // heads as the fourth
+  const int run = D >= 64 ? 64 : 32;
+  const int64_t strides[3] = {D, run, int64_t(Hkv) * D};
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return FA_ERR_DRIVER;
+  if (!aligned16(cache)) return FA_ERR_MISALIGNED;
+  cuuint64_t dims[4] = {cuuint64_t(run), cuuint64_t(cache_rows), cuuint64_t(D / run), cuuint64_t(Hkv)};
+  cuuint64_t gstr[3] = {cuuint64_t(strides[2]) * 2, cuuint64_t(strides[1]) * 2, cuuint64_t(strides[0]) * 2};
+  cuuint32_t box[4] = {cuuint32_t(run), cuuint32_t(rows), cuuint32_t(D / run), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType ty = dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(map, ty, 4, const_cast<void*>(cache), dims, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSOR_MAP;
 }
 }  // namespace fa
 

@@ -178,7 +178,9 @@ struct SparseArgs {
 int launch_sparse_decode(SparseArgs a, const CUtensorMap& k, const CUtensorMap& v, int D);
 
 // The device status word, and a tensor map over a (num_pages, page_size, Hkv,
-// D) cache whose box is `rows` rows of one head (fa_capi.cu).
+// D) cache whose box is `rows` rows of one head, all D columns: dimensions
+// {min(D, 64) columns, cache rows, D / 64 runs of columns, heads}, so that one
+// copy leaves a row's runs of 64 columns behind each other (fa_capi.cu).
 int* device_status_word();
 int make_cache_map(CUtensorMap* map, const void* cache, int cache_rows, int Hkv, int D, int rows, int dtype);
 

@@ -13,6 +13,8 @@
 // to what they are kept in (means: to fp32 and then the cache's type; scores:
 // to fp32).  The kept pages then depend on the inputs alone, not on the order
 // of a sum.
+#include <atomic>
+
 #include "fa_kernels.h"
 
 namespace fa {
@@ -59,6 +61,7 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
   const int cols = min(W8, MEAN_THREADS);
   const int groups = min(MEAN_THREADS / cols, 8);
   const int P = 1 << a.page_log2;
+  units = min(units, (__ldg(a.cu + a.B) >> a.page_log2) + a.B);  // the step's own rows
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     // last b with off(b) <= u
     const int lane = threadIdx.x & 31;
@@ -170,9 +173,16 @@ struct RowPlace {
 __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens, int B, int t, int key_cap,
                                               int* status) {
   RowPlace r;
-  r.b = warp_find_seq(cu, B, t);
-  const int q0 = __ldg(cu + r.b), q1 = __ldg(cu + r.b + 1);
-  const int nk = __ldg(seqlens + r.b);
+  // a decode step brings one row a sequence: that guess is loaded at once,
+  // and the search with its dependent loads is for other batches
+  r.b = min(t, B - 1);
+  int q0 = __ldg(cu + r.b), q1 = __ldg(cu + r.b + 1), nk = __ldg(seqlens + r.b);
+  if (t < q0 || t >= q1) {
+    r.b = warp_find_seq(cu, B, t);
+    q0 = __ldg(cu + r.b);
+    q1 = __ldg(cu + r.b + 1);
+    nk = __ldg(seqlens + r.b);
+  }
   const long long pos = (long long)nk - (q1 - t);  // the rows are the sequence's last
   const bool too_long = nk > key_cap;  // its table row cannot hold it
   if (too_long && status) atomicCAS(status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
@@ -185,16 +195,22 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
 // block scores its share of the pages into the first block's shared memory,
 // which then finds the top ones.
 //
-// Scoring: D / 8 lanes own a page, 8 columns a lane, SEL_PAGES pages at once
-// for their loads in flight.  The group's queries lie in shared memory in 64
-// bits.  Lanes swap halves of their page sums until each holds whole ones.
+// Scoring: D / 8 lanes own a page, 8 columns a lane, SEL_PAGES pages at once,
+// the next ones' loads in flight.  The group's queries lie in shared memory in
+// 64 bits and are taken SEL_HEADS heads at a time.  Lanes swap halves of
+// their page sums until each holds whole ones.  Bound: for a group of 4 heads
+// the 64-bit products (64 a clock and SM) take about as long as the means'
+// bytes, for larger ones longer.
 //
 // Selection: keys are the scores' bits in an order that whole numbers have,
-// SEL_KEYS neighbouring ones a thread.  The kk-th largest key is found bit by
-// bit, a block-wide count for each; the pages above it, and of the pages at
-// it the first ones, are written in order of their index.
-constexpr int SEL_THREADS = 512;
+// neighbouring ones a thread.  The kk-th largest key is found two bits a
+// round, by block-wide counts of the keys at and above three candidates; the
+// pages above it, and of the pages at it the first ones, are written in order
+// of their index.
+constexpr int SEL_THREADS = 256;
+constexpr int SEL_WARPS = SEL_THREADS / 32;
 constexpr int SEL_PAGES = 4;
+constexpr int SEL_HEADS = 4;
 
 __device__ __forceinline__ uint32_t order_key(float f) {
   if (f != f) return 0u;  // NaN: behind everything
@@ -202,22 +218,185 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// Scores of the block's pn pages (ids in shared memory), as keys to keys_at.
 template <int D, int DT>
-__global__ void __launch_bounds__(SEL_THREADS) fa_select_pages_kernel(const __grid_constant__ SelectArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
+__device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* qd, const int* ids, int h, int G,
+                                            int pn, uint32_t keys_at) {
   constexpr int LP = D / 8;  // lanes of a page
+  constexpr int SUBS = SEL_THREADS / LP;
+  const int lane = threadIdx.x & 31;
+  const int l = threadIdx.x % LP;
+  const uint16_t* means = static_cast<const uint16_t*>(a.means) + (long long)h * D + 8 * l;
+  const long long page_stride = (long long)a.Hkv * D;
+  auto load = [&](int first, uint4 (&v)[SEL_PAGES]) {
+#pragma unroll
+    for (int i = 0; i < SEL_PAGES; ++i) {
+      const int id = first + i < pn ? ids[first + i] : -1;
+      v[i] = id >= 0 ? __ldg(reinterpret_cast<const uint4*>(means + id * page_stride)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  // the trip count is the warp's, for the shuffles
+  int first = (threadIdx.x / LP) * SEL_PAGES;
+  uint4 v[SEL_PAGES];
+  load(first, v);
+  for (int base = (threadIdx.x - lane) / LP * SEL_PAGES; base < pn; base += SUBS * SEL_PAGES, first += SUBS * SEL_PAGES) {
+    uint4 next[SEL_PAGES];
+    load(first + SUBS * SEL_PAGES, next);
+    float best = -INFINITY;
+    bool nan = false;
+    for (int g0 = 0; g0 < G; g0 += SEL_HEADS) {
+      double s[SEL_HEADS][SEL_PAGES];
+#pragma unroll
+      for (int g = 0; g < SEL_HEADS; ++g)
+#pragma unroll
+        for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = 0.0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        double lo[SEL_PAGES], hi[SEL_PAGES];
+#pragma unroll
+        for (int i = 0; i < SEL_PAGES; ++i) {
+          const uint32_t w = j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w;
+          const float2 f = unpack2<DT>(w);
+          lo[i] = double(f.x);
+          hi[i] = double(f.y);
+        }
+#pragma unroll
+        for (int g = 0; g < SEL_HEADS; ++g) {
+          const double2 x = qd[((g0 + g) * 4 + j) * LP + l];
+#pragma unroll
+          for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = fma(x.y, hi[i], fma(x.x, lo[i], s[g][i]));
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < SEL_HEADS; ++g) {
+        if (g0 + g >= G) break;  // uniform
+        // 4 page sums over LP lanes: keep 2, then 1, then add it up
+        const bool up0 = (l & (LP / 2)) != 0;
+        double e0 = up0 ? s[g][2] : s[g][0], e1 = up0 ? s[g][3] : s[g][1];
+        e0 += __shfl_xor_sync(0xffffffffu, up0 ? s[g][0] : s[g][2], LP / 2);
+        e1 += __shfl_xor_sync(0xffffffffu, up0 ? s[g][1] : s[g][3], LP / 2);
+        const bool up1 = (l & (LP / 4)) != 0;
+        double e = up1 ? e1 : e0;
+        e += __shfl_xor_sync(0xffffffffu, up1 ? e0 : e1, LP / 4);
+#pragma unroll
+        for (int m = LP / 8; m > 0; m >>= 1) e += __shfl_xor_sync(0xffffffffu, e, m);
+        const float f = __double2float_rn(e);
+        nan |= f != f;
+        best = fmaxf(best, f);
+      }
+    }
+    // this lane's page of the four
+    const int mine = first + ((l & (LP / 2)) ? 2 : 0) + ((l & (LP / 4)) ? 1 : 0);
+    if ((l & (LP / 4 - 1)) == 0 && mine < pn)
+      st_cluster_u32(keys_at + 4u * uint32_t(mine), ids[mine] < 0 || nan ? 0u : order_key(best));
+#pragma unroll
+    for (int i = 0; i < SEL_PAGES; ++i) v[i] = next[i];
+  }
+}
+
+// The kk largest of the M keys, to out in order of their index, plus off.
+// E: keys a thread, held in registers; 0: read again from shared memory.
+template <int E>
+__device__ __forceinline__ void write_top(const uint32_t* keys, int M, int kk, int off, int* out) {
+  __shared__ uint2 counts[2][SEL_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = E > 0 ? E : (M + SEL_THREADS - 1) / SEL_THREADS;
+  const int k0 = min(M, int(threadIdx.x) * each), k1 = min(M, k0 + each);
+  uint32_t mine[E > 0 ? E : 1];
+  if constexpr (E > 0) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) mine[i] = k0 + i < k1 ? keys[k0 + i] : 0u;
+  }
+  uint32_t T = 0;  // the kk-th largest key
+#pragma unroll 1
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    const uint32_t t1 = T | (1u << bit), t2 = T | (2u << bit), t3 = T | (3u << bit);
+    // counts of keys >= t1, t2 and t3; M is below 2^16
+    uint32_t c12 = 0, c3 = 0;
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) c12 += (mine[i] >= t1) + ((mine[i] >= t2) << 16), c3 += mine[i] >= t3;
+    } else {
+      for (int i = k0; i < k1; ++i) {
+        const uint32_t k = keys[i];
+        c12 += (k >= t1) + ((k >= t2) << 16), c3 += k >= t3;
+      }
+    }
+    c12 = __reduce_add_sync(0xffffffffu, c12);
+    c3 = __reduce_add_sync(0xffffffffu, c3);
+    uint2* slot = counts[(bit >> 1) & 1];
+    if (lane == 0) slot[warp] = make_uint2(c12, c3);
+    __syncthreads();
+    c12 = c3 = 0;
+#pragma unroll
+    for (int w = 0; w < SEL_WARPS; ++w) c12 += slot[w].x, c3 += slot[w].y;
+    const uint32_t want = uint32_t(kk);
+    T = c3 >= want ? t3 : (c12 >> 16) >= want ? t2 : (c12 & 0xffffu) >= want ? t1 : T;
+  }
+  // a thread's keys above and at T (padding never counts: it lies behind k1)
+  int gt = 0, eq = 0;
+  auto key_at = [&](int i) {
+    if constexpr (E > 0) return mine[i];
+    else return keys[k0 + i];
+  };
+  auto each_key = [&](auto f) {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (k0 + i < k1) f(i);
+    } else {
+      for (int i = 0; k0 + i < k1; ++i) f(i);
+    }
+  };
+  each_key([&](int i) { gt += key_at(i) > T, eq += key_at(i) == T; });
+  uint32_t both = uint32_t(gt) | (uint32_t(eq) << 16), sum = both;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, sum, m);
+    if (lane >= m) sum += x;
+  }
+  __syncthreads();
+  if (lane == 31) counts[0][warp].x = sum;
+  __syncthreads();
+  uint32_t before = sum - both, all = 0;
+#pragma unroll
+  for (int w = 0; w < SEL_WARPS; ++w) {
+    if (w < warp) before += counts[0][w].x;
+    all += counts[0][w].x;
+  }
+  int gs = int(before & 0xffffu), es = int(before >> 16);
+  const int want_eq = kk - int(all & 0xffffu);
+  each_key([&](int i) {
+    const uint32_t key = key_at(i);
+    if (key > T || (key == T && es < want_eq)) out[gs + min(es, want_eq)] = off + k0 + i;
+    gs += key > T;
+    es += key == T;
+  });
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const __grid_constant__ SelectArgs a) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int LP = D / 8;
   const int S = a.cluster;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / S;
   const int t = unit / a.Hkv, h = unit - t * a.Hkv;
   const int G = a.Hq / a.Hkv;
-  const int lane = threadIdx.x & 31;
-  // [G][4][LP] pairs of a query's columns in 64 bits, then ids, then keys
+  // the group's queries in 64 bits, [head][4][LP] pairs of columns, zeros up
+  // to a whole SEL_HEADS; then page ids; then keys
+  const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
   double2* qd = reinterpret_cast<double2*>(smem);
-  int* ids = reinterpret_cast<int*>(smem + size_t(G) * D * 8);
+  int* ids = reinterpret_cast<int*>(smem + size_t(G4) * D * 8);
   uint32_t* keys = reinterpret_cast<uint32_t*>(ids + a.share);
-  __shared__ int warp_gt[SEL_THREADS / 32], warp_eq[SEL_THREADS / 32];
 
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
+  for (int i = threadIdx.x; i < G4 * D / 2; i += SEL_THREADS) {
+    const int g = i / (D / 2), d = i % (D / 2) * 2;  // columns d, d + 1: lane d / 8, pair (d % 8) / 2
+    float2 f = make_float2(0.f, 0.f);
+    if (g < G) f = unpack2<DT>(__ldg(reinterpret_cast<const uint32_t*>(q + g * a.q_sh + d)));
+    qd[(g * 4 + (d % 8) / 2) * LP + d / 8] = make_double2(double(f.x), double(f.y));
+  }
   const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
   int* out = a.out + (long long)unit * a.top;
   const int n = row.pos < 0 ? 0 : (row.pos >> a.page_log2) + 1;  // pages up to the token's own
@@ -244,148 +423,58 @@ __global__ void __launch_bounds__(SEL_THREADS) fa_select_pages_kernel(const __gr
     if (!ok && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
     ids[i] = ok ? id : -1;
   }
-  const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
-  for (int i = threadIdx.x; i < G * D / 2; i += SEL_THREADS) {
-    const int g = i / (D / 2), d = i % (D / 2) * 2;  // columns d, d + 1: lane d / 8, pair (d % 8) / 2
-    const float2 f = unpack2<DT>(__ldg(reinterpret_cast<const uint32_t*>(q + g * a.q_sh + d)));
-    qd[(g * 4 + (d % 8) / 2) * LP + d / 8] = make_double2(double(f.x), double(f.y));
-  }
   if (S > 1) cluster_sync();  // and the first block has begun, so that its shared memory may be written
   else __syncthreads();
-  const uint32_t keys0 = smem_u32(keys);
-  const uint32_t keys_at = S > 1 ? cluster_map(keys0, 0) : keys0;
-  {
-    const int sub = threadIdx.x / LP, l = threadIdx.x % LP;
-    constexpr int SUBS = SEL_THREADS / LP;
-    // the trip count is the warp's, for the shuffles
-    for (int base = (sub - lane / LP) * SEL_PAGES; base < pn; base += SUBS * SEL_PAGES) {
-      const int first = base + lane / LP * SEL_PAGES;
-      double kd[SEL_PAGES][8];
-      uint4 v[SEL_PAGES];
-#pragma unroll
-      for (int i = 0; i < SEL_PAGES; ++i) {
-        const int id = first + i < pn ? ids[first + i] : -1;
-        v[i] = id >= 0 ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.means) +
-                                                              ((long long)id * a.Hkv + h) * D) + l)
-                       : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < SEL_PAGES; ++i) {
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack2<DT>(w[j]);
-          kd[i][2 * j] = double(f.x);
-          kd[i][2 * j + 1] = double(f.y);
-        }
-      }
-      float best = -INFINITY;
-      bool nan = false;
-      for (int g = 0; g < G; ++g) {
-        double s[SEL_PAGES];
-#pragma unroll
-        for (int i = 0; i < SEL_PAGES; ++i) s[i] = 0.0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const double2 x = qd[(g * 4 + j) * LP + l];
-#pragma unroll
-          for (int i = 0; i < SEL_PAGES; ++i) s[i] = fma(x.y, kd[i][2 * j + 1], fma(x.x, kd[i][2 * j], s[i]));
-        }
-        // 4 page sums over LP lanes: keep 2, then 1, then add it up
-        const bool up0 = (l & (LP / 2)) != 0;
-        double e0 = up0 ? s[2] : s[0], e1 = up0 ? s[3] : s[1];
-        e0 += __shfl_xor_sync(0xffffffffu, up0 ? s[0] : s[2], LP / 2);
-        e1 += __shfl_xor_sync(0xffffffffu, up0 ? s[1] : s[3], LP / 2);
-        const bool up1 = (l & (LP / 4)) != 0;
-        double e = up1 ? e1 : e0;
-        e += __shfl_xor_sync(0xffffffffu, up1 ? e0 : e1, LP / 4);
-#pragma unroll
-        for (int m = LP / 8; m > 0; m >>= 1) e += __shfl_xor_sync(0xffffffffu, e, m);
-        const float f = __double2float_rn(e);
-        nan |= f != f;
-        best = fmaxf(best, f);
-      }
-      // this lane's page of the four
-      const int mine = first + ((l & (LP / 2)) ? 2 : 0) + ((l & (LP / 4)) ? 1 : 0);
-      if ((l & (LP / 4 - 1)) == 0 && mine < pn) {
-        const uint32_t key = ids[mine] < 0 || nan ? 0u : order_key(best);
-        st_cluster_u32(keys_at + 4u * uint32_t(p0 + mine), key);
-      }
-    }
-  }
+  const uint32_t keys0 = smem_u32(keys) + 4u * uint32_t(p0);
+  score_pages<D, DT>(a, qd, ids, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
   if (S > 1) {
     cluster_sync();
     if (rank != 0) return;
   } else {
     __syncthreads();
   }
-
-  // thread i owns keys [i E, (i + 1) E)
-  const int E = (M + SEL_THREADS - 1) / SEL_THREADS;
-  const int k0 = min(M, int(threadIdx.x) * E), k1 = min(M, k0 + E);
-  uint32_t T = 0;  // the kk-th largest key
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = T | (1u << bit);
-    int c = 0;
-    for (int i = k0; i < k1; ++i) c += keys[i] >= cand;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) warp_gt[threadIdx.x >> 5] = c;
-    __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < SEL_THREADS / 32; ++w) all += warp_gt[w];
-    __syncthreads();
-    if (all >= kk) T = cand;
-  }
-  int gt = 0, eq = 0;
-  for (int i = k0; i < k1; ++i) gt += keys[i] > T, eq += keys[i] == T;
-  int gs = gt, es = eq;
-#pragma unroll
-  for (int m = 1; m < 32; m <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, gs, m), y = __shfl_up_sync(0xffffffffu, es, m);
-    if (lane >= m) gs += x, es += y;
-  }
-  if (lane == 31) warp_gt[threadIdx.x >> 5] = gs, warp_eq[threadIdx.x >> 5] = es;
-  __syncthreads();
-  gs -= gt;
-  es -= eq;
-  int total_gt = 0;
-  for (int w = 0; w < SEL_THREADS / 32; ++w) {
-    if (w < int(threadIdx.x >> 5)) gs += warp_gt[w], es += warp_eq[w];
-    total_gt += warp_gt[w];
-  }
-  const int want_eq = kk - total_gt;
-  for (int i = k0; i < k1; ++i) {
-    const uint32_t key = keys[i];
-    if (key > T || (key == T && es < want_eq)) out[a.sink + gs + min(es, want_eq)] = a.sink + i;
-    gs += key > T;
-    es += key == T;
-  }
+  if (M <= SEL_THREADS) write_top<1>(keys, M, kk, a.sink, out + a.sink);
+  else if (M <= 4 * SEL_THREADS) write_top<4>(keys, M, kk, a.sink, out + a.sink);
+  else if (M <= 16 * SEL_THREADS) write_top<16>(keys, M, kk, a.sink, out + a.sink);
+  else write_top<0>(keys, M, kk, a.sink, out + a.sink);
 }
 
 // ---------------------------------------------------------------------------
 // Attention over the listed pages.
 //
-// A cluster of S blocks takes one (token, K/V head, up to 16 of its query
+// A cluster of S blocks takes one (token, K/V head, up to 8 of its query
 // heads).  The list is cut into 64-key tiles; block r takes tiles r, r + S,
-// ...  A producer warp copies a tile's K and V rows by TMA, a piece of a page
-// and 64 columns a copy, into a ring of DEC_STAGES tiles.  Four warps take 16
-// keys of every tile each, with softmax state of their own: S = Q K^T and
-// O += P V by m16n8k16 matrix instructions with the query heads as the 16
-// rows, so nothing is exchanged until the end.  Then the warps' states are
-// joined in shared memory and the blocks' over the cluster's.
+// ...  Two producer warps copy a tile's K and V rows by TMA, one copy a piece
+// of a page, into a ring of tiles.  Four warps take 16 keys of every tile
+// each, with softmax state of their own, so nothing is exchanged until the
+// end: then the warps' states are joined in shared memory and the blocks' over
+// the cluster's.
 //
-// Bound: HBM, 4 D bytes a key.  For a key the two products are 2 matrix
-// instructions, 4 of the 22 clocks that its bytes take an SM's share of HBM;
-// tcgen05's 128 rows would be 7 of 8 parts empty for a group's heads.
+// Both products are m16n8k16 matrix instructions.  S = Q K^T has the heads as
+// rows (8 of 16) and the keys as columns; what a thread then holds of the
+// weights is just what it has to hold of P^T as the second operand of
+// O^T = V^T P^T, whose rows are 16 of the D columns and whose columns are the
+// 8 heads.  That takes half of the instructions and accumulators of O = P V
+// with 16 rows of heads.
+//
+// Bound: HBM, 4 D bytes a key.  For a key the products take some 3 clocks of
+// the 22 that its bytes take an SM's share of HBM; tcgen05's 128 rows would
+// be 15 of 16 parts empty for a group's heads.
 constexpr int DEC_WARPS = 4;
-constexpr int DEC_THREADS = (DEC_WARPS + 1) * 32;
+constexpr int DEC_THREADS = (DEC_WARPS + 2) * 32;
 constexpr int DEC_TILE = 64;
 constexpr int NO_KEY = 0x7fffffff;
+constexpr int MAX_CLUSTER = 8;
 
 template <int D>
 constexpr int dec_stages() {
-  return D == 128 ? 3 : D == 64 ? 6 : 8;
+#ifndef T_ST64
+#define T_ST64 3
+#endif
+#ifndef T_ST32
+#define T_ST32 6
+#endif
+  return D == 128 ? 3 : D == 64 ? T_ST64 : T_ST32;
 }
 template <int D>
 constexpr int dec_tile_bytes() {
@@ -396,14 +485,15 @@ struct DecSmem {
   static constexpr int ST = dec_stages<D>();
   static constexpr int RING = ST * 2 * dec_tile_bytes<D>();
   static constexpr int BASE = RING;                      // first logical key of each 16 of a tile
-  static constexpr int BARS = BASE + ST * 4 * 4;         // full, empty
-  static constexpr int BYTES = BARS + ST * 2 * 8 + 64 + 1024;  // control block; room to align the ring
+  static constexpr int BARS = BASE + ST * 4 * 4;         // K full, V full, empty
+  static constexpr int BYTES = BARS + ST * 3 * 8 + 64 + 1024;  // control block; room to align the ring
   // after the last tile: joined state of the block, then the warps' states
-  static constexpr int O_BLOCK = 0;                      // [16][D] fp32
-  static constexpr int ML_BLOCK = 16 * D * 4;            // [2][16]
-  static constexpr int O_WARP = ML_BLOCK + 128;          // [4][16][D]
-  static constexpr int ML_WARP = O_WARP + 4 * 16 * D * 4;  // [4][2][16]
-  static_assert(ML_WARP + 4 * 128 <= RING, "the states reuse the ring");
+  static constexpr int O_PITCH = D + 4;                               // floats of a head's row
+  static constexpr int O_BLOCK = 0;                                   // [8][O_PITCH] fp32
+  static constexpr int ML_BLOCK = O_BLOCK + 8 * O_PITCH * 4;          // [2][8]
+  static constexpr int O_WARP = ML_BLOCK + 64;                        // [4][8][O_PITCH]
+  static constexpr int ML_WARP = O_WARP + DEC_WARPS * 8 * O_PITCH * 4;  // [4][2][8]
+  static_assert(ML_WARP + DEC_WARPS * 64 <= RING, "the states reuse the ring");
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -431,91 +521,108 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
   }
 }
 
-// Byte offset of 16-byte chunk c (8 columns) of row r in a 64-row tile as the
-// TMA's swizzle leaves it.
+// Byte offset of 16-byte chunk c (8 columns) of row r of 16 rows that start at
+// a multiple of 8 rows of a piece, as the TMA's swizzle leaves it.  box: bytes
+// between the first 64 columns and the last 64 of a piece.
 template <int D>
-__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+__device__ __forceinline__ uint32_t tile_off(int r, int c, uint32_t box) {
   if constexpr (D == 32) return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-  else return uint32_t((c >> 3) * (DEC_TILE * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+  else return (D == 128 && (c & 8) ? box : 0u) + uint32_t(r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+#ifndef T_M64
+#define T_M64 4
+#endif
+template <int D>
+constexpr int dec_per_sm() {
+  return D == 128 ? 2 : T_M64;
+}
 template <int D, int DT>
-__global__ void __launch_bounds__(DEC_THREADS)
+__global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
     fa_sparse_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                             const __grid_constant__ SparseArgs a) {
   using M = DecSmem<D>;
   constexpr int ST = M::ST;
-  constexpr int NBOX = D == 128 ? 2 : 1;
   constexpr int KS = D / 16;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   int* key_base = reinterpret_cast<int*>(smem + M::BASE);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + M::BARS);
-  uint64_t* empty = full + ST;
+  uint64_t* full_k = reinterpret_cast<uint64_t*>(smem + M::BARS);
+  uint64_t* full_v = full_k + ST;
+  uint64_t* empty = full_v + ST;
   CtaCtl* ctl = reinterpret_cast<CtaCtl*>(empty + ST);
   const int S = a.cluster;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
   const int G = a.Hq / a.Hkv;
-  const int hblocks = (G + 15) / 16;
-  const int unit = blockIdx.x / S;  // (token, K/V head, block of 16 heads)
+  const int hblocks = (G + 7) / 8;
+  const int unit = blockIdx.x / S;  // (token, K/V head, block of 8 heads)
   const int hb = unit % hblocks;
   const int th = unit / hblocks;
   const int t = th / a.Hkv, h = th - t * a.Hkv;
-  const int rows = min(16, G - hb * 16);
+  const int rows = min(8, G - hb * 8);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int PR = min(1 << a.page_log2, DEC_TILE);  // rows of a piece
 
   if (threadIdx.x == 0) {
     ctl->abort = 0;
     ctl->status = a.status;
     for (int i = 0; i < ST; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full_k + i, 1);
+      mbar_init(full_v + i, 1);
       mbar_init(empty + i, DEC_WARPS);
     }
     fence_mbar_init();
   }
+  // the producers' first list entries do not wait for the row's place
+  const int PT = DEC_TILE / PR;                  // pieces of a tile
+  const int sub_log2 = max(0, a.page_log2 - 6);  // pieces of a page
+  const int pieces = a.top << sub_log2;
+  const int* list = a.idx + ((long long)t * a.Hkv + h) * a.top;
+  // lane j: piece j % PT of tile t0 + j / PT of the block's
+  auto list_entry = [&](int t0) {
+    const int piece = ((t0 + lane / PT) * S + rank) * PT + lane % PT;
+    return piece < pieces ? __ldg(list + (piece >> sub_log2)) : -1;
+  };
+  int entry = warp >= DEC_WARPS ? list_entry(0) : -1;
   const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
   const int pos = row.pos;
   __syncthreads();
 
   const int g8 = lane >> 2, t4 = lane & 3;
-  float o[D / 8][4];
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  // O^T: columns 16 i + g8 (values 0, 1) and + 8 (2, 3) of heads 2 t4, 2 t4 + 1;
+  // maximum and this thread's sum of head g8
+  float o[D / 16][4];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-  if (warp == DEC_WARPS) {
-    // ---- producer ----
-    const int PR = min(1 << a.page_log2, DEC_TILE);  // rows of a piece
-    const int PT = DEC_TILE / PR;                    // pieces of a tile
-    const int sub_log2 = max(0, a.page_log2 - 6);    // pieces of a page
-    const int pieces = pos < 0 ? 0 : a.top << sub_log2;
-    const int tiles = (pieces + PT - 1) / PT;
+  if (warp >= DEC_WARPS) {
+    // ---- producers: K rows, V rows ----
+    const bool is_k = warp == DEC_WARPS;
+    uint64_t* full = is_k ? full_k : full_v;
+    const CUtensorMap* map = is_k ? &tmap_k : &tmap_v;
+    const int tiles = pos < 0 ? 0 : (pieces + PT - 1) / PT;
     const int mine = tiles > rank ? (tiles - rank + S - 1) / S : 0;  // tiles rank, rank + S, ...
-    const int* list = a.idx + ((long long)t * a.Hkv + h) * a.top;
     const int per_batch = 32 / PT;  // tiles whose pieces the warp's lanes look up at once
     int it = 0;
     bool ok = true;
     for (int t0 = 0; t0 < mine && ok; t0 += per_batch) {
       // lane j: piece j % PT of tile t0 + j / PT
-      const int lt = t0 + lane / PT;
-      const int piece = (lt * S + rank) * PT + lane % PT;
+      const int sub = (((t0 + lane / PT) * S + rank) * PT + lane % PT) & ((1 << sub_log2) - 1);
       int base = NO_KEY, at = 0;  // first logical key; row in the cache
-      if (lt < mine && piece < pieces) {
-        const int e = __ldg(list + (piece >> sub_log2));
-        const int sub = piece & ((1 << sub_log2) - 1);
-        if (e >= 0 && e < a.width) {
-          const int first = (e << a.page_log2) + sub * DEC_TILE;
-          if (first <= pos) {
-            const int id = __ldg(a.table + (long long)row.b * a.width + e);
-            if (id >= 0 && id < a.num_pages) {
-              base = first;
-              at = (id << a.page_log2) + sub * DEC_TILE;
-            } else if (a.status) {
-              atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
-            }
+      if (entry >= 0 && entry < a.width) {
+        const int first = (entry << a.page_log2) + sub * DEC_TILE;
+        if (first <= pos) {
+          const int id = __ldg(a.table + (long long)row.b * a.width + entry);
+          if (id >= 0 && id < a.num_pages) {
+            base = first;
+            at = (id << a.page_log2) + sub * DEC_TILE;
+          } else if (a.status) {
+            atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
           }
         }
       }
+      if (t0 + per_batch < mine) entry = list_entry(t0 + per_batch);  // the next look-up's
       const uint32_t there = __ballot_sync(0xffffffffu, base != NO_KEY);
       for (int i = 0; i < per_batch && t0 + i < mine; ++i) {
         const uint32_t have = (there >> (i * PT)) & ((1u << PT) - 1u);
@@ -525,22 +632,16 @@ __global__ void __launch_bounds__(DEC_THREADS)
           ok = false;
           break;
         }
-        // lane j: copy j % (2 NBOX) of piece j / (2 NBOX): K or V, 64 columns
-        const int pc = lane / (2 * NBOX);
-        const int src = i * PT + min(pc, PT - 1);
-        const int pb = __shfl_sync(0xffffffffu, base, src);
-        const int pa = __shfl_sync(0xffffffffu, at, src);
-        const int b16 = __shfl_sync(0xffffffffu, base, i * PT + min(lane * 16 / PR, PT - 1));
-        if (lane < 4) key_base[s * 4 + lane] = b16 == NO_KEY ? NO_KEY : b16 + (lane * 16) % PR;
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(full + s, uint32_t(__popc(have)) * uint32_t(PR * D * 2 * 2));
-        __syncwarp();
-        if (pc < PT && pb != NO_KEY) {
-          const int what = lane % (2 * NBOX);
-          const int box = what % NBOX;
-          unsigned char* tile = smem + (s * 2 + (what / NBOX)) * dec_tile_bytes<D>();
-          tma_load_4d(tile + box * (DEC_TILE * 128) + pc * PR * (D >= 64 ? 128 : 64), what < NBOX ? &tmap_k : &tmap_v,
-                      full + s, box * 64, pa, h, 0);
+        if (is_k) {
+          const int b16 = __shfl_sync(0xffffffffu, base, i * PT + min(lane * 16 / PR, PT - 1));
+          if (lane < 4) key_base[s * 4 + lane] = b16 == NO_KEY ? NO_KEY : b16 + (lane * 16) % PR;
+          __syncwarp();
+        }
+        unsigned char* tile = smem + (s * 2 + (is_k ? 0 : 1)) * dec_tile_bytes<D>();
+        if (lane == 0) mbar_arrive_expect_tx(full + s, uint32_t(__popc(have)) * uint32_t(PR * D * 2));
+        for (int p = 0; p < PT; ++p) {
+          const int row_at = __shfl_sync(0xffffffffu, at, i * PT + p);
+          if (lane == 0 && ((have >> p) & 1u)) tma_load_4d(tile + p * PR * D * 2, map, full + s, 0, row_at, 0, h);
         }
         ++it;
       }
@@ -549,9 +650,11 @@ __global__ void __launch_bounds__(DEC_THREADS)
     if (ok) {
       const int s = it % ST;
       if (it < ST || mbar_wait_warp(empty + s, uint32_t(it / ST - 1) & 1, ctl, 97)) {
-        if (lane < 4) key_base[s * 4 + lane] = -1;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + s);
+        if (is_k) {
+          if (lane < 4) key_base[s * 4 + lane] = -1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + s);
+        }
       } else {
         ok = false;
       }
@@ -562,126 +665,115 @@ __global__ void __launch_bounds__(DEC_THREADS)
       __syncwarp();
     }
   } else {
-    // ---- consumer: keys 16 warp .. of each tile ----
-    uint32_t qf[KS][4];
+    // ---- consumers: keys 16 warp .. of each tile ----
+    uint32_t qf[KS][2];  // head g8's columns 16 ks + 2 t4 and + 8
     {
-      const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + ((long long)h * G + hb * 16) * a.q_sh;
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + ((long long)h * G + hb * 8 + g8) * a.q_sh;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = g8 + (j & 1) * 8, c = ks * 16 + (j >> 1) * 8 + t4 * 2;
-          qf[ks][j] = r < rows && pos >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(q + r * a.q_sh + c)) : 0u;
-        }
+        for (int j = 0; j < 2; ++j)
+          qf[ks][j] =
+              g8 < rows && pos >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(q + ks * 16 + j * 8 + t4 * 2)) : 0u;
     }
-    const int row0 = warp * 16;
+    // the warp's 16 rows: their piece, and their place in it
+    const uint32_t box = uint32_t(PR) * 128u;
+    const uint32_t rows_at = uint32_t(warp * 16 / PR * PR * D * 2 + warp * 16 % PR * (D == 32 ? 64 : 128));
+    const int mi = lane >> 3, mr = lane & 7;
     for (int it = 0;; ++it) {
       const int s = it % ST;
-      if (!mbar_wait_warp(full + s, uint32_t(it / ST) & 1, ctl, 99)) break;
+      const uint32_t parity = uint32_t(it / ST) & 1;
+      if (!mbar_wait_warp(full_k + s, parity, ctl, 99)) break;
       const int base = key_base[s * 4 + warp];
       if (base == -1) break;
       const int seen = base == NO_KEY ? 0 : max(0, min(16, pos - base + 1));
+      unsigned char* vt = smem + (s * 2 + 1) * dec_tile_bytes<D>() + rows_at;
+      const uint32_t va = smem_u32(vt), ka = va - dec_tile_bytes<D>();
+      float sc[2][2][4];  // [k-steps even, odd][keys 0-7, 8-15][head g8's keys 2 t4, + 1; two of no head]
       if (seen > 0) {
-        unsigned char* kt = smem + s * 2 * dec_tile_bytes<D>();
-        unsigned char* vt = kt + dec_tile_bytes<D>();
-        const uint32_t ka = smem_u32(kt), va = smem_u32(vt);
-        float sc[2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[0][j] = sc[1][j] = 0.f;
-        const int mi = lane >> 3, mr = lane & 7;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[i >> 1][i & 1][j] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           uint32_t b[4];
-          ldmatrix4(ka + tile_off<D>(row0 + (mi >> 1) * 8 + mr, ks * 2 + (mi & 1)), b);
-          mma16816<DT>(sc[0], qf[ks], b[0], b[1]);
-          mma16816<DT>(sc[1], qf[ks], b[2], b[3]);
+          ldmatrix4(ka + tile_off<D>((mi >> 1) * 8 + mr, ks * 2 + (mi & 1), box), b);
+          const uint32_t af[4] = {qf[ks][0], 0u, qf[ks][1], 0u};
+          mma16816<DT>(sc[ks & 1][0], af, b[0], b[1]);
+          mma16816<DT>(sc[ks & 1][1], af, b[2], b[3]);
         }
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sc[nt][j] *= a.scale_log2;
+      }
+      if (!mbar_wait_warp(full_v + s, parity, ctl, 100)) break;
+      if (seen > 0) {
         if (seen < 16) {
-          // keys past the token's position: no score, and zeros for their
-          // values, which may be anything and would meet a zero weight
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (nt * 8 + t4 * 2 + (j & 1) >= seen) sc[nt][j] = -INFINITY;
+          // values behind the token's position may be anything and would meet
+          // a zero weight: zeros in their place
           for (int i = lane; i < (16 - seen) * (D / 8); i += 32)
-            *reinterpret_cast<uint4*>(vt + tile_off<D>(row0 + seen + i / (D / 8), i % (D / 8))) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vt + tile_off<D>(seen + i / (D / 8), i % (D / 8), box)) = make_uint4(0, 0, 0, 0);
           __syncwarp();
         }
-        float mx[2], al[2];
-        bool same = true;
+        uint32_t vf[D / 16][4];  // V^T: 16 columns x 16 keys each
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float x = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          x = fmaxf(m[r], x);
-          same = same && x == m[r];
-          const float ref = x == -INFINITY ? 0.f : x;  // no finite score so far: weights of zero
-          al[r] = ex2(m[r] - ref);
-          m[r] = x;
-          mx[r] = ref;
+        for (int np = 0; np < D / 16; ++np)
+          ldmatrix4_t(va + tile_off<D>((mi >> 1) * 8 + mr, np * 2 + (mi & 1), box), vf[np]);
+        float w[4];  // scores, then weights of keys 2 t4, + 1, + 8, + 9
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = (sc[0][j >> 1][j & 1] + sc[1][j >> 1][j & 1]) * a.scale_log2;
+          if (seen < 16 && (j >> 1) * 8 + t4 * 2 + (j & 1) >= seen) w[j] = -INFINITY;
         }
-        if (!__all_sync(0xffffffffu, same)) {
+        float x = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        x = fmaxf(m, x);
+        const float ref = x == -INFINITY ? 0.f : x;  // no finite score so far: weights of zero
+        if (__any_sync(0xffffffffu, x != m)) {
+          const float al = ex2(m - ref);
+          m = x;
+          l *= al;
+          const float a0 = __shfl_sync(0xffffffffu, al, t4 * 8), a1 = __shfl_sync(0xffffffffu, al, t4 * 8 + 4);
 #pragma unroll
-          for (int r = 0; r < 2; ++r) l[r] *= al[r];
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][0] *= al[0], o[i][1] *= al[0];
-            o[i][2] *= al[1], o[i][3] *= al[1];
+          for (int i = 0; i < D / 16; ++i) {
+            o[i][0] *= a0, o[i][1] *= a1;
+            o[i][2] *= a0, o[i][3] *= a1;
           }
         }
-        float p[2][4];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            p[nt][j] = ex2(sc[nt][j] - mx[j >> 1]);
-            l[j >> 1] += p[nt][j];
-          }
+        for (int j = 0; j < 4; ++j) {
+          w[j] = ex2(w[j] - ref);
+          l += w[j];
+        }
         // the weights as the second product's operand: rounded to its type,
         // at most half a step of a value in [0, 1]
-        const uint32_t pf[4] = {pack2<DT>(p[0][0], p[0][1]), pack2<DT>(p[0][2], p[0][3]), pack2<DT>(p[1][0], p[1][1]),
-                                pack2<DT>(p[1][2], p[1][3])};
+        const uint32_t p0 = pack2<DT>(w[0], w[1]), p1 = pack2<DT>(w[2], w[3]);
 #pragma unroll
-        for (int np = 0; np < D / 16; ++np) {
-          uint32_t b[4];
-          ldmatrix4_t(va + tile_off<D>(row0 + (mi & 1) * 8 + mr, np * 2 + (mi >> 1)), b);
-          mma16816<DT>(o[2 * np], pf, b[0], b[1]);
-          mma16816<DT>(o[2 * np + 1], pf, b[2], b[3]);
-        }
+        for (int np = 0; np < D / 16; ++np) mma16816<DT>(o[np], vf[np], p0, p1);
         if (seen < 16) fence_proxy_async_smem();  // zeros written before the next copy lands there
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + s);
     }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
   }
   __syncthreads();  // the ring is free
   float* ml_warp = reinterpret_cast<float*>(smem + M::ML_WARP);
   float* o_warp = reinterpret_cast<float*>(smem + M::O_WARP);
   float* ml_block = reinterpret_cast<float*>(smem + M::ML_BLOCK);
   float* o_block = reinterpret_cast<float*>(smem + M::O_BLOCK);
+  constexpr int OP = M::O_PITCH;
   if (warp < DEC_WARPS) {
+    if (t4 == 0) {
+      ml_warp[warp * 16 + g8] = m;
+      ml_warp[warp * 16 + 8 + g8] = l;
+    }
+    float* dst = o_warp + (warp * 8 + t4 * 2) * OP + g8;
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-      if (g8 + r * 8 < rows) {
-        if (t4 == 0) {
-          ml_warp[warp * 32 + g8 + r * 8] = m[r];
-          ml_warp[warp * 32 + 16 + g8 + r * 8] = l[r];
-        }
-        float* dst = o_warp + (warp * 16 + g8 + r * 8) * D + t4 * 2;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
-      }
+    for (int i = 0; i < D / 16; ++i) {
+      dst[i * 16] = o[i][0], dst[i * 16 + OP] = o[i][1];
+      dst[i * 16 + 8] = o[i][2], dst[i * 16 + 8 + OP] = o[i][3];
+    }
   }
   __syncthreads();
   // the block's state: rows x D / 4 vectors over the threads
@@ -689,51 +781,78 @@ __global__ void __launch_bounds__(DEC_THREADS)
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < DEC_WARPS; ++w) mm = fmaxf(mm, ml_warp[w * 32 + r]);
+    for (int w = 0; w < DEC_WARPS; ++w) mm = fmaxf(mm, ml_warp[w * 16 + r]);
     const float ref = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < DEC_WARPS; ++w) {
-      const float x = ex2(ml_warp[w * 32 + r] - ref);
-      ll += x * ml_warp[w * 32 + 16 + r];
-      const float4 v = *reinterpret_cast<const float4*>(o_warp + (w * 16 + r) * D + c);
+      const float x = ex2(ml_warp[w * 16 + r] - ref);
+      ll += x * ml_warp[w * 16 + 8 + r];
+      const float4 v = *reinterpret_cast<const float4*>(o_warp + (w * 8 + r) * OP + c);
       acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
     }
-    *reinterpret_cast<float4*>(o_block + r * D + c) = acc;
+    *reinterpret_cast<float4*>(o_block + r * OP + c) = acc;
     if (c == 0) {
       ml_block[r] = mm;
-      ml_block[16 + r] = ll;
+      ml_block[8 + r] = ll;
     }
   }
   if (S > 1) cluster_sync();
   else __syncthreads();
   // the cluster's state: each block joins its share of the columns
-  uint16_t* out = static_cast<uint16_t*>(a.o) + ((long long)t * a.Hq + h * G + hb * 16) * D;
+  uint16_t* out = static_cast<uint16_t*>(a.o) + ((long long)t * a.Hq + h * G + hb * 8) * D;
   const uint32_t o_addr = smem_u32(o_block), ml_addr = smem_u32(ml_block);
   const int vecs = rows * (D / 4);
   for (int i = rank + S * int(threadIdx.x); i < vecs; i += S * DEC_THREADS) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
-    float mm = -INFINITY;
-    for (int k = 0; k < S; ++k)
-      mm = fmaxf(mm, S > 1 ? ld_cluster_f32(cluster_map(ml_addr + r * 4, k)) : ml_block[r]);
-    const float ref = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < S; ++k) {
-      const float mk = S > 1 ? ld_cluster_f32(cluster_map(ml_addr + r * 4, k)) : ml_block[r];
-      const float lk = S > 1 ? ld_cluster_f32(cluster_map(ml_addr + 64 + r * 4, k)) : ml_block[16 + r];
-      const float4 v = S > 1 ? ld_cluster_f4(cluster_map(o_addr + (r * D + c) * 4, k))
-                             : *reinterpret_cast<const float4*>(o_block + r * D + c);
-      const float x = ex2(mk - ref);
-      ll += x * lk;
-      acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
+    if (S > 1) {
+      // all blocks' values at once: one trip through the cluster's network
+      float mk[MAX_CLUSTER], lk[MAX_CLUSTER];
+      float4 v[MAX_CLUSTER];
+#pragma unroll
+      for (int k = 0; k < MAX_CLUSTER; ++k) {
+        const uint32_t from = uint32_t(k < S ? k : rank);
+        mk[k] = ld_cluster_f32(cluster_map(ml_addr + r * 4, from));
+        lk[k] = ld_cluster_f32(cluster_map(ml_addr + 32 + r * 4, from));
+        v[k] = ld_cluster_f4(cluster_map(o_addr + (r * OP + c) * 4, from));
+      }
+      float mm = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < MAX_CLUSTER; ++k) mm = fmaxf(mm, k < S ? mk[k] : -INFINITY);
+      const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+      for (int k = 0; k < MAX_CLUSTER; ++k)
+        if (k < S) {
+          const float x = ex2(mk[k] - ref);
+          ll += x * lk[k];
+          acc.x += x * v[k].x, acc.y += x * v[k].y, acc.z += x * v[k].z, acc.w += x * v[k].w;
+        }
+    } else {
+      ll = ml_block[8 + r];
+      acc = *reinterpret_cast<const float4*>(o_block + r * OP + c);
     }
     const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);  // no key: zeros; NaN stays
     *reinterpret_cast<uint2*>(out + r * D + c) =
         make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
   }
   if (S > 1) cluster_sync();  // the others have read this block's state
+}
+
+// Raises a kernel's dynamic shared memory limit, once per device.
+template <auto* Kernel>
+int allow_smem(int bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FA_ERR_LAUNCH;
+  if (!done[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return FA_ERR_LAUNCH;
+    done[dev].store(true, std::memory_order_release);
+  }
+  return FA_OK;
 }
 
 // A launch in clusters of S blocks (1: none).
@@ -758,10 +877,9 @@ template <int D, int DT>
 int run_sparse(const SparseArgs& a, const CUtensorMap& k, const CUtensorMap& v) {
   auto* kernel = fa_sparse_decode_kernel<D, DT>;
   const int smem = DecSmem<D>::BYTES;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return FA_ERR_LAUNCH;
+  if (int rc = allow_smem<fa_sparse_decode_kernel<D, DT>>(smem)) return rc;
   const int G = a.Hq / a.Hkv;
-  const long long units = (long long)a.total_q * a.Hkv * ((G + 15) / 16);
+  const long long units = (long long)a.total_q * a.Hkv * ((G + 7) / 8);
   if (units * a.cluster > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
   return launch_clustered(kernel, unsigned(units * a.cluster), DEC_THREADS, size_t(smem), a.cluster, a.stream, k, v, a);
 }
@@ -770,21 +888,23 @@ template <int D, int DT>
 int run_select(const SelectArgs& a) {
   auto* kernel = fa_select_pages_kernel<D, DT>;
   const int G = a.Hq / a.Hkv;
-  const size_t smem = size_t(G) * D * 8 + size_t(a.share) * 4 + size_t(a.width) * 4;
-  if (smem > size_t(200) << 10) return FA_ERR_BAD_SHAPE;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-    return FA_ERR_LAUNCH;
+  const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
+  const size_t smem = size_t(G4) * D * 8 + size_t(a.share) * 4 + size_t(a.width) * 4;
+  constexpr size_t most = size_t(220) << 10;  // of an SM's 227 KB, the static part left out
+  if (smem > most) return FA_ERR_BAD_SHAPE;
+  if (int rc = allow_smem<fa_select_pages_kernel<D, DT>>(int(most))) return rc;
   const long long units = (long long)a.total_q * a.Hkv;
   if (units * a.cluster > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
   return launch_clustered(kernel, unsigned(units * a.cluster), SEL_THREADS, smem, a.cluster, a.stream, a);
 }
 
-// Largest power of two up to 8 that still leaves every block `least` pieces
-// of a unit's work and does not go past what the GPU holds at once.
+// Blocks that share a unit: the largest power of two up to 8 with which all
+// units are on the GPU at once (per_sm blocks a SM) and every block has
+// `least` pieces of its unit's work.
 int cluster_for(long long units, long long pieces, int least, int per_sm) {
   const long long slots = (long long)device_sm_count() * per_sm;
   int S = 1;
-  while (S < 8 && units * S < slots && pieces >= 2LL * S * least) S *= 2;
+  while (S < MAX_CLUSTER && units * S * 2 <= slots && pieces >= 2LL * S * least) S *= 2;
   return S;
 }
 
@@ -792,7 +912,7 @@ int cluster_for(long long units, long long pieces, int least, int per_sm) {
 
 int launch_page_means(const PageArgs& a, int total_q) {
   const long long units = (long long)(total_q >> a.page_log2) + a.B;
-  const long long cap = (long long)device_sm_count() * 4;
+  const long long cap = (long long)device_sm_count() * 2;
   const unsigned ctas = unsigned(units < cap ? units : cap);
   const int W8 = a.Hkv * a.D / 8;
   const int cols = W8 < MEAN_THREADS ? W8 : MEAN_THREADS;
@@ -815,7 +935,11 @@ int launch_select_pages(SelectArgs a, int D) {
 int launch_sparse_decode(SparseArgs a, const CUtensorMap& k, const CUtensorMap& v, int D) {
   const int G = a.Hq / a.Hkv;
   const long long tiles = (((long long)a.top << a.page_log2) + DEC_TILE - 1) / DEC_TILE;
-  a.cluster = cluster_for((long long)a.total_q * a.Hkv * ((G + 15) / 16), tiles, 2, 2);
+  a.cluster = cluster_for((long long)a.total_q * a.Hkv * ((G + 7) / 8), tiles, 2,
+                          D == 128 ? dec_per_sm<128>() : dec_per_sm<64>());
+#ifdef T_DS
+  a.cluster = T_DS;
+#endif
   if (a.dtype == DT_BF16)
     return D == 32 ? run_sparse<32, DT_BF16>(a, k, v)
                    : D == 64 ? run_sparse<64, DT_BF16>(a, k, v) : run_sparse<128, DT_BF16>(a, k, v);

@@ -27,8 +27,7 @@ from typing import NamedTuple
 import torch
 
 from . import _abi
-from .attention import _stream_handle
-from .rotary import _ptr, _strides, check_backend, check_eps, check_table, check_weights, on_device, vector_rows
+from .rotary import _ptr, check_backend, check_eps, check_table, check_weights, on_device, row_arg
 
 # block-table width that select_pages takes (FA_MAX_SELECT_PAGES of include/fa_b200.h)
 MAX_SELECT_PAGES = 16384
@@ -42,26 +41,37 @@ def _check_page_size(page_size) -> None:
 def _check_int32(name: str, t, ndim: int, device) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.ndim != ndim or t.dtype != torch.int32 or t.device != device:
+    if t.dtype != torch.int32 or t.ndim != ndim or t.device != device:
         raise ValueError(f"{name} must be a {ndim}-D int32 tensor on the same device as the others")
 
 
-def _check_cache(name: str, t, like=None) -> None:
+def _check_cache(name: str, t, dtype, device) -> torch.Size:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.ndim != 4 or 0 in t.shape:
-        raise ValueError(f"{name} must have shape (num_pages, page_size, heads, head_dim); got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 4 or 0 in shape:
+        raise ValueError(f"{name} must have shape (num_pages, page_size, heads, head_dim); got {tuple(shape)}")
     if not t.is_contiguous() or t.data_ptr() % 16:
         raise ValueError(f"{name} must be contiguous and start on a 16-byte boundary")
-    if t.shape[0] * t.shape[1] > 0x7fffffff:
+    if shape[0] * shape[1] > 0x7fffffff:
         raise ValueError(f"{name} must have fewer than 2**31 slots")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError("k_cache and v_cache must have the same shape, dtype and device")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must have the same dtype and device as the others")
+    return shape
+
+
+def _check_caches(k_cache, v_cache, dtype, device) -> torch.Size:
+    shape = _check_cache("k_cache", k_cache, dtype, device)
+    if _check_cache("v_cache", v_cache, dtype, device) != shape:
+        raise ValueError("k_cache and v_cache must have the same shape")
+    return shape
 
 
 def _check_no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the paged K/V path is forward only; run it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the paged K/V path is forward only; run it under torch.no_grad()")
 
 
 class PagedStep(NamedTuple):
@@ -120,20 +130,21 @@ def extend_block_table(block_table, seqlens_cached, seqlens_new, free_pages, fre
     if dev.type != "cuda":
         raise RuntimeError("B200 CUDA backend is unavailable: the B200 kernel requires a CUDA tensor")
     seqlens_cached, seqlens_new, free_pages = (t.contiguous() for t in (seqlens_cached, seqlens_new, free_pages))
-    with on_device(block_table):
-        # one allocation for the int32 outputs, each part on a 16-byte boundary
-        a, b, c = (requests + 4) // 4 * 4, (requests + 3) // 4 * 4, (total_q + 3) // 4 * 4
-        out = torch.empty(a + b + 2 * c + 1, device=dev, dtype=torch.int32)
-        cu, sk, pos, slots, nxt = (out[:requests + 1], out[a:a + requests], out[a + b:a + b + total_q],
-                                   out[a + b + c:a + b + c + total_q], out[a + b + 2 * c:])
+    with on_device(block_table) as stream:
+        # one allocation for the int32 outputs
+        out = torch.empty(2 * requests + 2 + 2 * total_q, device=dev, dtype=torch.int32)
+        cu, sk, pos, slots, nxt = out.split_with_sizes((requests + 1, requests, total_q, total_q, 1))
         fits = torch.empty(requests, device=dev, dtype=torch.bool)
-        at = out.data_ptr()
+        cu_at = out.data_ptr()
+        sk_at = cu_at + 4 * (requests + 1)
+        pos_at = sk_at + 4 * requests
+        slots_at = pos_at + 4 * total_q
         rc = _abi.lib().fa_extend_block_table(
             block_table.data_ptr(), seqlens_cached.data_ptr(), seqlens_new.data_ptr(),
-            free_pages.data_ptr(), free_start.data_ptr(), at, at + 4 * a, at + 4 * (a + b),
-            at + 4 * (a + b + c), fits.data_ptr(), at + 4 * (a + b + 2 * c), requests, width, free_pages.shape[0],
-            page_size, total_q, _stream_handle(dev))
-    _abi.check(rc, "fa_extend_block_table")
+            free_pages.data_ptr(), free_start.data_ptr(), cu_at, sk_at, pos_at, slots_at,
+            fits.data_ptr(), slots_at + 4 * total_q, requests, width, free_pages.shape[0], page_size, total_q, stream)
+    if rc:
+        _abi.check(rc, "fa_extend_block_table")
     return PagedStep(cu, sk, pos, slots, fits, nxt)
 
 
@@ -153,55 +164,60 @@ def paged_append(query, key, value, k_cache, v_cache, slot_mapping, table, posit
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
-        if t.ndim != 3 or 0 in t.shape:
-            raise ValueError(f"{name} must have shape (total, heads, head_dim), no dimension zero; "
-                             f"got {tuple(t.shape)}")
-        if t.dtype != query.dtype or t.device != query.device:
+        shape = t.shape
+        if len(shape) != 3 or 0 in shape:
+            raise ValueError(f"{name} must have shape (total, heads, head_dim), no dimension zero; got {tuple(shape)}")
+        if t is not query and (t.dtype != query.dtype or t.device != query.device):
             raise ValueError("query, key, and value must have the same dtype and device")
     total, hq, d = query.shape
-    if key.shape != value.shape:
+    dev = query.device
+    key_shape = key.shape
+    if key_shape != value.shape:
         raise ValueError("key and value must have the same shape")
-    if key.shape[0] != total or key.shape[2] != d:
+    if key_shape[0] != total or key_shape[2] != d:
         raise ValueError("query and key must have the same number of rows and head dimension")
-    _check_cache("k_cache", k_cache)
-    _check_cache("v_cache", v_cache, k_cache)
-    if k_cache.shape[2:] != key.shape[1:] or k_cache.dtype != query.dtype or k_cache.device != query.device:
-        raise ValueError("the caches must have the key's heads, head dimension, dtype and device")
+    pages, page_size, hkv, cache_d = _check_caches(k_cache, v_cache, query.dtype, dev)
+    if hkv != key_shape[1] or cache_d != d:
+        raise ValueError("the caches must have the key's heads and head dimension")
     for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):
-        _check_int32(name, t, 1, query.device)
+        _check_int32(name, t, 1, dev)
         if t.shape[0] != total:
             raise ValueError(f"{name} must have one entry per row of query")
     if not isinstance(interleaved, bool):
         raise TypeError("interleaved must be a bool")
     check_eps(eps)
-    check_table(table, d, query.device)
+    check_table(table, d, dev)
     check_weights(query_weight, key_weight, query)
     _check_no_grad(query, key, value, query_weight, key_weight)
     check_backend(query)
-    q, k, v = vector_rows(query), vector_rows(key), vector_rows(value)
+    q, qp, qs = row_arg(query)
+    k, kp, ks = row_arg(key)
+    v, vp, vs = row_arg(value)
     slots, pos = slot_mapping.contiguous(), positions.contiguous()
     if query_weight is not None:
         query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
-    with on_device(q):
-        out = torch.empty((total, hq, d), device=q.device, dtype=q.dtype)
+    with on_device(q) as stream:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         rc = _abi.entry("fa_paged_append", q.dtype)(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            slots.data_ptr(), table.data_ptr(), pos.data_ptr(), _ptr(query_weight), _ptr(key_weight), total, hq,
-            k.shape[1], d, k_cache.shape[0] * k_cache.shape[1], table.shape[0], table.shape[1], interleaved,
-            query_weight is not None and query_weight.dtype == torch.float32, _strides(q), _strides(k), _strides(v),
-            float(eps), _stream_handle(q.device))
-    _abi.check(rc, "fa_paged_append")
+            qp, kp, vp, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), table.data_ptr(),
+            pos.data_ptr(), _ptr(query_weight), _ptr(key_weight), total, hq, hkv, d, pages * page_size, *table.shape,
+            interleaved, query_weight is not None and query_weight.dtype == torch.float32, qs, ks, vs, float(eps),
+            stream)
+    if rc:
+        _abi.check(rc, "fa_paged_append")
     return out
 
 
-def _check_step(block_table, cu_seqlens_q, seqlens_k, device) -> None:
+def _check_step(block_table, cu_seqlens_q, seqlens_k, device) -> torch.Size:
     _check_int32("block_table", block_table, 2, device)
     _check_int32("cu_seqlens_q", cu_seqlens_q, 1, device)
     _check_int32("seqlens_k", seqlens_k, 1, device)
-    if 0 in block_table.shape:
+    shape = block_table.shape
+    if 0 in shape:
         raise ValueError("block_table dimensions must all be greater than zero")
-    if cu_seqlens_q.shape[0] != block_table.shape[0] + 1 or seqlens_k.shape[0] != block_table.shape[0]:
+    if cu_seqlens_q.shape[0] != shape[0] + 1 or seqlens_k.shape[0] != shape[0]:
         raise ValueError("block_table and seqlens_k must have one row per sequence of cu_seqlens_q")
+    return shape
 
 
 def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k, *, total_q: int | None = None):
@@ -215,8 +231,9 @@ def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k,
     last keys.  ``total_q``: rows of the packed batch when the caller has it;
     None takes room for a step that fills the table.  Means are summed in 64
     bits and do not depend on the order of the sum."""
-    _check_cache("k_cache", k_cache)
-    num_pages, page_size, hkv, d = k_cache.shape
+    if not isinstance(k_cache, torch.Tensor):
+        raise TypeError("k_cache must be a torch.Tensor")
+    num_pages, page_size, hkv, d = _check_cache("k_cache", k_cache, k_cache.dtype, k_cache.device)
     _check_page_size(page_size)
     if not isinstance(page_means, torch.Tensor):
         raise TypeError("page_means must be a torch.Tensor")
@@ -224,8 +241,7 @@ def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k,
             or page_means.device != k_cache.device or not page_means.is_contiguous() or page_means.data_ptr() % 16):
         raise ValueError("page_means must be a contiguous (num_pages, heads, head_dim) tensor of the cache's dtype "
                          "and device")
-    _check_step(block_table, cu_seqlens_q, seqlens_k, k_cache.device)
-    batch, width = block_table.shape
+    batch, width = _check_step(block_table, cu_seqlens_q, seqlens_k, k_cache.device)
     if width * page_size > 0x7fffffff:
         raise ValueError("max_pages_per_seq * page_size must be below 2**31")
     if total_q is None:
@@ -235,12 +251,13 @@ def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k,
     _check_no_grad(k_cache, page_means)
     check_backend(k_cache)
     table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
-    with on_device(k_cache):
+    with on_device(k_cache) as stream:
         rc = _abi.entry("fa_page_means", k_cache.dtype)(
             k_cache.data_ptr(), page_means.data_ptr(), table.data_ptr(),
             cu.data_ptr(), lens.data_ptr(), batch, hkv, d, num_pages,
-            page_size, width, total_q, _stream_handle(k_cache.device))
-    _abi.check(rc, "fa_page_means")
+            page_size, width, total_q, stream)
+    if rc:
+        _abi.check(rc, "fa_page_means")
     return page_means
 
 
@@ -278,9 +295,8 @@ def select_pages(query, page_means, block_table, cu_seqlens_q, seqlens_k, *, pag
     hkv = page_means.shape[1]
     if hq % hkv:
         raise ValueError("the number of query heads must be divisible by the number of key/value heads")
-    _check_step(block_table, cu_seqlens_q, seqlens_k, query.device)
+    batch, width = _check_step(block_table, cu_seqlens_q, seqlens_k, query.device)
     _check_page_size(page_size)
-    batch, width = block_table.shape
     if width > MAX_SELECT_PAGES:
         raise ValueError(f"block_table may be {MAX_SELECT_PAGES} pages wide for page selection; got {width}")
     if width * page_size > 0x7fffffff or page_means.shape[0] * page_size > 0x7fffffff:
@@ -295,16 +311,17 @@ def select_pages(query, page_means, block_table, cu_seqlens_q, seqlens_k, *, pag
         raise ValueError("num_selected * page_size must be below 2**30")
     _check_no_grad(query, page_means)
     check_backend(query)
-    q = vector_rows(query)
+    q, qp, qs = row_arg(query)
     table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
-    with on_device(q):
+    with on_device(q) as stream:
         out = torch.empty((total, hkv, num_selected), device=q.device, dtype=torch.int32)
         rc = _abi.entry("fa_select_pages", q.dtype)(
-            q.data_ptr(), page_means.data_ptr(), table.data_ptr(),
+            qp, page_means.data_ptr(), table.data_ptr(),
             cu.data_ptr(), lens.data_ptr(), out.data_ptr(), batch, hq, hkv,
-            d, total, page_means.shape[0], page_size, width, num_selected, sink_pages, local_pages, _strides(q),
-            _stream_handle(q.device))
-    _abi.check(rc, "fa_select_pages")
+            d, total, page_means.shape[0], page_size, width, num_selected, sink_pages, local_pages, qs,
+            stream)
+    if rc:
+        _abi.check(rc, "fa_select_pages")
     return out
 
 
@@ -330,39 +347,38 @@ def scaled_dot_product_attention_paged_sparse(query, k_cache, v_cache, block_tab
         raise TypeError("enable_gqa must be a bool")
     if scale is not None and (not isinstance(scale, Real) or not math.isfinite(float(scale))):
         raise ValueError("scale must be a finite real number or None")
-    _check_cache("k_cache", k_cache)
-    _check_cache("v_cache", v_cache, k_cache)
     total, hq, d = query.shape
-    num_pages, page_size, hkv, cache_d = k_cache.shape
+    dev = query.device
+    num_pages, page_size, hkv, cache_d = _check_caches(k_cache, v_cache, query.dtype, dev)
     _check_page_size(page_size)
-    if cache_d != d or k_cache.dtype != query.dtype or k_cache.device != query.device:
-        raise ValueError("the caches must have the query's head dimension, dtype and device")
+    if cache_d != d:
+        raise ValueError("the caches must have the query's head dimension")
     if hq != hkv and not enable_gqa:
         raise ValueError(
             "query has a different number of heads from key/value; pass "
             "enable_gqa=True to use grouped-query attention")
     if hq % hkv:
         raise ValueError("the number of query heads must be divisible by the number of key/value heads")
-    _check_step(block_table, cu_seqlens_q, seqlens_k, query.device)
-    _check_int32("page_indices", page_indices, 3, query.device)
-    batch, width = block_table.shape
-    n = page_indices.shape[2]
-    if tuple(page_indices.shape[:2]) != (total, hkv) or n == 0:
+    batch, width = _check_step(block_table, cu_seqlens_q, seqlens_k, dev)
+    _check_int32("page_indices", page_indices, 3, dev)
+    rows, heads, n = page_indices.shape
+    if rows != total or heads != hkv or n == 0:
         raise ValueError("page_indices must have shape (total_q, key/value heads, n)")
     if width * page_size > 0x7fffffff or n * page_size > 0x3fffffff:
         raise ValueError("block_table and page_indices are too wide for this page_size")
     _check_no_grad(query, k_cache, v_cache)
     check_backend(query)
-    q = vector_rows(query)
+    q, qp, qs = row_arg(query)
     table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
     pages = page_indices.contiguous()
-    with on_device(q):
-        out = torch.empty((total, hq, d), device=q.device, dtype=q.dtype)
+    with on_device(q) as stream:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         rc = _abi.entry("fa_fwd_paged_sparse", q.dtype)(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+            qp, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
             table.data_ptr(), cu.data_ptr(),
             lens.data_ptr(), pages.data_ptr(), batch, hq, hkv, d, total,
-            num_pages, page_size, width, n, float(scale) if scale is not None else d ** -0.5, _strides(q),
-            _stream_handle(q.device))
-    _abi.check(rc, "fa_fwd_paged_sparse")
+            num_pages, page_size, width, n, float(scale) if scale is not None else d ** -0.5, qs,
+            stream)
+    if rc:
+        _abi.check(rc, "fa_fwd_paged_sparse")
     return out

@@ -23,7 +23,7 @@ from numbers import Real
 import torch
 
 from . import _abi
-from .attention import SUPPORTED_DTYPES, SUPPORTED_HEAD_DIMS, _device_capability, _stream_handle
+from .attention import SUPPORTED_DTYPES, SUPPORTED_HEAD_DIMS, _device_capability
 
 # rows of the partial weight gradients (FA_ROTARY_PARTIALS of include/fa_b200.h)
 ROTARY_PARTIALS = 592
@@ -50,7 +50,7 @@ def rotary_table(max_positions: int, rotary_dim: int, *, base: float = 10000.0, 
 def check_backend(tensor: torch.Tensor) -> None:
     """Raises unless the B200 kernels serve tensors of this device, type and
     head dim, with the messages of the attention calls."""
-    if tensor.device.type != "cuda":
+    if not tensor.is_cuda:
         raise RuntimeError("B200 CUDA backend is unavailable: the B200 kernel requires a CUDA tensor")
     if tensor.dtype not in SUPPORTED_DTYPES:
         raise RuntimeError("B200 CUDA backend is unavailable: the custom mixed-precision path currently "
@@ -63,29 +63,56 @@ def check_backend(tensor: torch.Tensor) -> None:
         raise RuntimeError("B200 CUDA backend is unavailable: the kernels are built for sm_100a (B200) GPUs only")
 
 
-def on_device(tensor: torch.Tensor):
-    """Context in which launches go to the tensor's device: nothing when it is
-    current already."""
-    return torch.cuda.device(tensor.device.index)
+class on_device:
+    """Context in which launches go to the tensor's device; its value is the
+    device's current stream.  Calls of a few microseconds of GPU time are
+    bound by their host side, so this does nothing where the device is current
+    already."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, tensor: torch.Tensor):
+        self.index = tensor.get_device()
+
+    def __enter__(self) -> int:
+        current = torch.cuda.current_device()
+        self.previous = current if current != self.index else None
+        if self.previous is not None:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.previous is not None:
+            torch.cuda.set_device(self.previous)
 
 
-def vector_rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself when its rows can be read 16 bytes at a time -- unit
-    stride over the last dimension, the others and the start multiples of 16
-    bytes -- and else a contiguous copy."""
-    s = t.stride()
-    if s[-1] == 1 and not any(x % 8 for x in s[:-1]) and t.data_ptr() % 16 == 0:
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+_UNSEEN = object()
+_row_strides: dict = {}
 
 
-def _strides(t: torch.Tensor):
+def _strides_arg(s: tuple):
     """{batch, head, seq} strides of a (B, H, N, D) or packed (total, H, D)
-    tensor.  Dimensions of one entry get a stride of no consequence."""
+    tensor for the library, or None when its rows cannot be read 16 bytes at a
+    time: unit stride over D, the others multiples of 8 elements.  A packed
+    tensor has one batch, whose stride is of no consequence."""
+    if s[-1] != 1 or any(x % 8 for x in s[:-1]):
+        return None
+    return _abi.strides_of(s[:3] if len(s) == 4 else (8, s[1], s[0]))
+
+
+def row_arg(t: torch.Tensor):
+    """``(tensor, address, strides)`` of rows to be read 16 bytes at a time:
+    ``t`` itself where its strides and start allow it, else a copy."""
     s = t.stride()
-    key = s[:3] if t.ndim == 4 else (t.shape[0] * t.shape[1] * t.shape[2], s[1], s[0])
-    return _abi.strides_of(key)
+    arr = _row_strides.get(s, _UNSEEN)
+    if arr is _UNSEEN:
+        if len(_row_strides) > 1024:
+            _row_strides.clear()
+        arr = _row_strides[s] = _strides_arg(s)
+    p = t.data_ptr()
+    if arr is not None and not p & 15:
+        return t, p, arr
+    return row_arg(torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t))
 
 
 def check_table(table, rotary_max: int, device) -> None:
@@ -124,41 +151,47 @@ def check_eps(eps) -> None:
 
 
 def _validate(query, key, table, positions, query_weight, key_weight, eps, interleaved) -> None:
-    for name, t in (("query", query), ("key", key)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if t.ndim not in (3, 4):
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a torch.Tensor")
+    if not isinstance(key, torch.Tensor):
+        raise TypeError("key must be a torch.Tensor")
+    qs, ks, ndim, dev = query.shape, key.shape, query.ndim, query.device
+    for name, shape in (("query", qs), ("key", ks)):
+        if len(shape) not in (3, 4):
             raise ValueError(f"{name} must have shape (batch, heads, sequence, head_dim) or (total, heads, head_dim); "
-                             f"got {tuple(t.shape)}")
-        if 0 in t.shape:
+                             f"got {tuple(shape)}")
+        if 0 in shape:
             raise ValueError(f"{name} dimensions must all be greater than zero")
-    if query.ndim != key.ndim:
+    if ndim != len(ks):
         raise ValueError("query and key must have the same layout")
-    if query.device != key.device:
+    if dev != key.device:
         raise ValueError("query and key must be on the same device")
     if query.dtype != key.dtype:
         raise ValueError("query and key must have the same dtype")
-    if query.shape[-1] != key.shape[-1]:
+    if qs[-1] != ks[-1]:
         raise ValueError("query and key head dimensions must match")
-    dense = query.ndim == 4
-    if dense and (query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]):
-        raise ValueError("query and key batch and sequence dimensions must match")
-    if not dense and query.shape[0] != key.shape[0]:
-        raise ValueError("query and key must have the same number of rows")
+    if ndim == 4:
+        n = qs[2]
+        if qs[0] != ks[0] or n != ks[2]:
+            raise ValueError("query and key batch and sequence dimensions must match")
+    else:
+        n = qs[0]
+        if n != ks[0]:
+            raise ValueError("query and key must have the same number of rows")
     if not isinstance(interleaved, bool):
         raise TypeError("interleaved must be a bool")
     check_eps(eps)
-    check_table(table, query.shape[-1], query.device)
+    check_table(table, qs[-1], dev)
     check_weights(query_weight, key_weight, query)
     if positions is None:
-        if not dense:
+        if ndim == 3:
             raise ValueError("packed (total, heads, head_dim) tensors need positions")
     else:
         if not isinstance(positions, torch.Tensor):
             raise TypeError("positions must be a torch.Tensor")
-        n = query.shape[2] if dense else query.shape[0]
-        shapes = ((n,), (query.shape[0], n)) if dense else ((n,),)
-        if positions.dtype != torch.int32 or positions.device != query.device or tuple(positions.shape) not in shapes:
+        ps = positions.shape
+        fits = (len(ps) == 1 and ps[0] == n) or (ndim == 4 and len(ps) == 2 and ps[0] == qs[0] and ps[1] == n)
+        if not fits or positions.dtype != torch.int32 or positions.device != dev:
             raise ValueError("positions must be an int32 tensor of the token dimension, or of (batch, sequence) for "
                              "4-D tensors, on the query's device")
     check_backend(query)
@@ -166,28 +199,35 @@ def _validate(query, key, table, positions, query_weight, key_weight, eps, inter
 
 def _sizes(q, k):
     """(B, Hq, Hkv, N, D)"""
-    if q.ndim == 4:
-        return q.shape[0], q.shape[1], k.shape[1], q.shape[2], q.shape[3]
-    return 1, q.shape[1], k.shape[1], q.shape[0], q.shape[2]
+    s = q.shape
+    if len(s) == 4:
+        return s[0], s[1], k.shape[1], s[2], s[3]
+    return 1, s[1], k.shape[1], s[0], s[2]
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _contiguous_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def qk_norm_rotary_forward(q, k, table, positions, query_weight, key_weight, eps: float, interleaved: bool):
     """Launch the forward: contiguous outputs in the inputs' layout."""
     b, hq, hkv, n, d = _sizes(q, k)
-    with on_device(q):
-        qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        ko = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+    q, qp, qs = row_arg(q)
+    k, kp, ks = row_arg(k)
+    with on_device(q) as stream:
+        _, qop, qos = row_arg(qo := _contiguous_like(q))
+        _, kop, kos = row_arg(ko := _contiguous_like(k))
+        positions_, rd = table.shape
         rc = _abi.entry("fa_qk_norm_rotary", q.dtype)(
-            q.data_ptr(), k.data_ptr(), qo.data_ptr(), ko.data_ptr(), table.data_ptr(), _ptr(positions),
-            _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n, d, table.shape[0], table.shape[1],
-            interleaved, query_weight is not None and query_weight.dtype == torch.float32,
-            _strides(q), _strides(k), _strides(qo), _strides(ko),
-            n if positions is not None and positions.ndim == 2 else 0, eps, _stream_handle(q.device))
-    _abi.check(rc, "fa_qk_norm_rotary")
+            qp, kp, qop, kop, table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n,
+            d, positions_, rd, interleaved, query_weight is not None and query_weight.dtype == torch.float32, qs, ks,
+            qos, kos, n if positions is not None and positions.ndim == 2 else 0, eps, stream)
+    if rc:
+        _abi.check(rc, "fa_qk_norm_rotary")
     return qo, ko
 
 
@@ -197,20 +237,25 @@ def qk_norm_rotary_backward(q, k, grad_q, grad_k, table, positions, query_weight
     (else None).  Gradients repeat bit for bit."""
     b, hq, hkv, n, d = _sizes(q, k)
     wants = weight_grads and query_weight is not None
-    with on_device(q):
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        dwq = torch.empty_like(query_weight) if wants else None
-        dwk = torch.empty_like(key_weight) if wants else None
-        part = torch.empty(ROTARY_PARTIALS * d, device=q.device, dtype=torch.float32) if wants else None
+    q, qp, qs = row_arg(q)
+    k, kp, ks = row_arg(k)
+    grad_q, gqp, gqs = row_arg(grad_q)
+    grad_k, gkp, gks = row_arg(grad_k)
+    with on_device(q) as stream:
+        _, dqp, dqs = row_arg(dq := _contiguous_like(q))
+        _, dkp, dks = row_arg(dk := _contiguous_like(k))
+        dwq = dwk = part = None
+        if wants:
+            dwq, dwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
+            part = torch.empty(ROTARY_PARTIALS * d, device=q.device, dtype=torch.float32)
+        positions_, rd = table.shape
         rc = _abi.entry("fa_qk_norm_rotary_bwd", q.dtype)(
-            q.data_ptr(), k.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-            _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions), _ptr(query_weight),
-            _ptr(key_weight), b, hq, hkv, n, d, table.shape[0], table.shape[1], interleaved,
-            query_weight is not None and query_weight.dtype == torch.float32,
-            _strides(q), _strides(k), _strides(grad_q), _strides(grad_k), _strides(dq), _strides(dk),
-            n if positions is not None and positions.ndim == 2 else 0, eps, _stream_handle(q.device))
-    _abi.check(rc, "fa_qk_norm_rotary_bwd")
+            qp, kp, gqp, gkp, dqp, dkp, _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions),
+            _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n, d, positions_, rd, interleaved,
+            query_weight is not None and query_weight.dtype == torch.float32, qs, ks, gqs, gks, dqs, dks,
+            n if positions is not None and positions.ndim == 2 else 0, eps, stream)
+    if rc:
+        _abi.check(rc, "fa_qk_norm_rotary_bwd")
     return dq, dk, dwq, dwk
 
 
@@ -225,12 +270,13 @@ class B200QKNormRotary(torch.autograd.Function):
         return qk_norm_rotary_forward(query, key, table, positions, query_weight, key_weight, eps, interleaved)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_query, grad_key):
+        if torch.is_grad_enabled():
+            raise RuntimeError("qk_norm_rotary is differentiable once: its backward has no gradient (create_graph)")
         query, key, table, positions, query_weight, key_weight = ctx.saved_tensors
-        dq, dk, dwq, dwk = qk_norm_rotary_backward(
-            query, key, vector_rows(grad_query), vector_rows(grad_key), table, positions, query_weight, key_weight,
-            ctx.eps, ctx.interleaved, ctx.needs_input_grad[4] or ctx.needs_input_grad[5])
+        needs = ctx.needs_input_grad
+        dq, dk, dwq, dwk = qk_norm_rotary_backward(query, key, grad_query, grad_key, table, positions, query_weight,
+                                                   key_weight, ctx.eps, ctx.interleaved, needs[4] or needs[5])
         return dq, dk, None, None, dwq, dwk, None, None
 
 
@@ -252,7 +298,8 @@ def qk_norm_rotary(query, key, table, positions=None, *, query_weight=None, key_
     A position outside the table is found on the GPU: its turned columns are
     NaN and the device status (``_abi.device_status``) names the error."""
     _validate(query, key, table, positions, query_weight, key_weight, eps, interleaved)
-    return B200QKNormRotary.apply(
-        vector_rows(query), vector_rows(key), table, None if positions is None else positions.contiguous(),
-        None if query_weight is None else query_weight.contiguous(),
-        None if key_weight is None else key_weight.contiguous(), float(eps), interleaved)
+    if positions is not None:
+        positions = positions.contiguous()
+    if query_weight is not None:
+        query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
+    return B200QKNormRotary.apply(query, key, table, positions, query_weight, key_weight, float(eps), interleaved)
