@@ -120,12 +120,13 @@ struct RotaryArgs {
   float eps;
   int max_pos, rd, interleaved, w_fp32, n_slots;
   int B, N, Hq, Hkv, dtype;
-  int q_ctas;
+  // set by the launches: ranges of tokens and their length (backward: the query
+  // rows' and the key rows'), blocks of the query rows
+  int parts, per_part, k_parts, k_per_part, q_ctas;
   int* status;
   cudaStream_t stream;
 };
 constexpr int ROTARY_BWD_CTAS = FA_ROTARY_PARTIALS;
-void rotary_bwd_ctas(int Hq, int Hkv, long long rows, int D, int* q_ctas, int* k_ctas);
 int launch_rotary_fwd(const RotaryArgs& a, int D);
 int launch_rotary_bwd(const RotaryArgs& a, int D);
 int launch_paged_append(const RotaryArgs& a, int D);

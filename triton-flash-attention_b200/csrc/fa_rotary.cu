@@ -14,40 +14,59 @@
 // All arithmetic is fp32 on registers and each result is rounded once.  The
 // table holds fp32 cosines and sines made from 64-bit angles.
 //
-// Bound: HBM.  A forward moves 4 bytes an element, a backward 6.  D / 8
-// lanes own a row, each lane 4 + 4 of its columns placed so that a lane
-// holds both halves of its pairs: the rotation needs no exchange and the
-// mean of squares log2(D / 8) shuffles.  A group of lanes takes several
-// heads of one token, so that its cosines and sines are read once for all of
-// them and that many 8-byte load pairs are in flight.  (8 + 8 columns a lane
-// halve the loads but double what a lane keeps -- angles, weights, weight
-// gradients --, and with fewer warps a SM ran slower.)
+// Bound: HBM.  A forward moves 4 bytes an element, a backward 6.  D / 2 C
+// lanes own a row, each lane C + C of its columns placed so that a lane holds
+// both halves of its pairs: the rotation needs no exchange and the mean of
+// squares log2(D / 2 C) shuffles.  A warp takes GW = 64 C / D neighbouring
+// heads of all tokens of a range, one token a step, so that its weights and
+// strides stay in registers and a step adds to its pointers and no more: these
+// kernels run out of issued instructions before they run out of bytes, and
+// what is worked out for a token or a kind of row costs as much as its
+// arithmetic.  Asynchronous copies bring the next steps' rows and angles into
+// a ring of the warp's own in shared memory, so that no register waits for
+// them.
 #include "fa_kernels.h"
 
 namespace fa {
 namespace {
 
-// A lane's run of C columns as fp32 pairs: packed instructions take two of
-// them at once (the forward issued 70 % of its slots without them).
+// A lane's run of C columns in fp32.  (Packed pairs, f32x2, were slower: the
+// kernel is bound by issued instructions before it is by bytes, and pairs cost
+// more moves than they save.)
 template <int C>
 struct Run {
-  uint64_t p[C / 2];
+  float v[C];
 };
 template <int C>
 struct Raw {  // the same run in the operand type
   uint32_t u[C / 2];
 };
 
-// C elements, read once.
+// C elements of a row into shared memory, asynchronously; nothing where !valid.
 template <int C>
-__device__ __forceinline__ Raw<C> ld_stream(const void* p) {
+__device__ __forceinline__ void copy_run(uint32_t saddr, const void* p, bool valid) {
+  if (valid) {
+    if constexpr (C == 8)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr), "l"(p) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(saddr), "l"(p) : "memory");
+  }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int C>
+__device__ __forceinline__ Raw<C> ld_run(uint32_t saddr) {
   Raw<C> r;
   if constexpr (C == 8)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3])
-                 : "l"(p));
+                 : "r"(saddr)
+                 : "memory");
   else
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.u[0]), "=r"(r.u[1]) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.u[0]), "=r"(r.u[1]) : "r"(saddr) : "memory");
   return r;
 }
 template <int C>
@@ -61,7 +80,8 @@ __device__ __forceinline__ Run<C> widen(const Raw<C>& r) {
 #pragma unroll
   for (int i = 0; i < C / 2; ++i) {
     const float2 t = unpack2<DT>(r.u[i]);
-    f.p[i] = f2pack(t.x, t.y);
+    f.v[2 * i] = t.x;
+    f.v[2 * i + 1] = t.y;
   }
   return f;
 }
@@ -69,27 +89,15 @@ template <int DT, int C>
 __device__ __forceinline__ Raw<C> narrow(const Run<C>& f) {
   Raw<C> r;
 #pragma unroll
-  for (int i = 0; i < C / 2; ++i) r.u[i] = pack2_f2<DT>(f.p[i]);
+  for (int i = 0; i < C / 2; ++i) r.u[i] = pack2<DT>(f.v[2 * i], f.v[2 * i + 1]);
   return r;
 }
 template <int C>
-__device__ __forceinline__ Run<C> zero_run() {
+__device__ __forceinline__ Run<C> fill_run(float v) {
   Run<C> f;
 #pragma unroll
-  for (int i = 0; i < C / 2; ++i) f.p[i] = 0;
+  for (int i = 0; i < C; ++i) f.v[i] = v;
   return f;
-}
-__device__ __forceinline__ uint64_t both(float v) { return f2pack(v, v); }
-__device__ __forceinline__ uint64_t neg2(uint64_t v) { return v ^ 0x8000000080000000ull; }
-__device__ __forceinline__ uint64_t swap2(uint64_t v) {
-  float lo, hi;
-  f2unpack(v, lo, hi);
-  return f2pack(hi, lo);
-}
-__device__ __forceinline__ float add_halves(uint64_t v) {
-  float lo, hi;
-  f2unpack(v, lo, hi);
-  return lo + hi;
 }
 
 // Columns [a, a + C) and [b, b + C) of a row belong to lane l of its group.
@@ -113,67 +121,23 @@ __device__ __forceinline__ LaneCols lane_cols(int l, int rd) {
   return c;
 }
 
-// C consecutive floats.
+// Cosines and sines of the C pairs of a lane's runs a, b: pair i is (a i, b i),
+// or interleaved (a 2 i, a 2 i + 1) and from C / 2 on those of b.
 template <int C>
-__device__ __forceinline__ Run<C> ld_floats(const float* p) {
-  Run<C> f;
-#pragma unroll
-  for (int i = 0; i < C / 4; ++i) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
-    f.p[2 * i] = f2pack(v.x, v.y);
-    f.p[2 * i + 1] = f2pack(v.z, v.w);
-  }
-  return f;
-}
-
-// A lane's angles, laid out for turn(): cosines and sines of its C pairs.
-// Halves: cs and sn of pair i at place i.  Interleaved: pair i is one packed
-// value, so cs and sn hold (c, c) and (-s, s) of the pairs of run a, then b
-// (C / 2 each, in ca, sa and cb, sb).
-template <bool INTER, int C>
 struct Angles {
-  Run<C> ca, sa;
-  Run<INTER ? C : 2> cb, sb;
+  Run<C> c, s;
 };
-template <bool INTER, int C>
-__device__ __forceinline__ Angles<INTER, C> arrange(const Run<C>& cs, const Run<C>& sn) {
-  Angles<INTER, C> g;
-  if constexpr (INTER) {
-#pragma unroll
-    for (int i = 0; i < C / 2; ++i) {  // pairs 2 i and 2 i + 1 of the lane's C
-      float c0, c1, s0, s1;
-      f2unpack(cs.p[i], c0, c1);
-      f2unpack(sn.p[i], s0, s1);
-      Run<C>& c = 2 * i < C / 2 ? g.ca : g.cb;
-      Run<C>& s = 2 * i < C / 2 ? g.sa : g.sb;
-      const int at = (2 * i) % (C / 2);
-      c.p[at] = both(c0);
-      c.p[at + 1] = both(c1);
-      s.p[at] = f2pack(-s0, s0);
-      s.p[at + 1] = f2pack(-s1, s1);
-    }
-  } else {
-    g.ca = cs;
-    g.sa = sn;
-    g.cb.p[0] = g.sb.p[0] = 0;
-  }
-  return g;
-}
 // Turns the runs; BACK: the other way.
 template <bool INTER, bool BACK, int C>
-__device__ __forceinline__ void turn(Run<C>& a, Run<C>& b, const Angles<INTER, C>& g) {
+__device__ __forceinline__ void turn(Run<C>& a, Run<C>& b, const Angles<C>& g) {
 #pragma unroll
-  for (int i = 0; i < C / 2; ++i) {
-    const uint64_t x = a.p[i], y = b.p[i];
-    if constexpr (INTER) {
-      const uint64_t sx = BACK ? neg2(g.sa.p[i]) : g.sa.p[i], sy = BACK ? neg2(g.sb.p[i]) : g.sb.p[i];
-      a.p[i] = ffma2(x, g.ca.p[i], fmul2(swap2(x), sx));
-      b.p[i] = ffma2(y, g.cb.p[i], fmul2(swap2(y), sy));
-    } else {
-      const uint64_t s = BACK ? neg2(g.sa.p[i]) : g.sa.p[i];
-      a.p[i] = ffma2(x, g.ca.p[i], fmul2(neg2(y), s));
-      b.p[i] = ffma2(y, g.ca.p[i], fmul2(x, s));
-    }
+  for (int i = 0; i < C; ++i) {
+    float& x = INTER ? (2 * i < C ? a.v[(2 * i) % C] : b.v[(2 * i) % C]) : a.v[i];
+    float& y = INTER ? (2 * i < C ? a.v[(2 * i + 1) % C] : b.v[(2 * i + 1) % C]) : b.v[i];
+    const float c = g.c.v[i], s = BACK ? -g.s.v[i] : g.s.v[i];
+    const float t = x * c - y * s;
+    y = y * c + x * s;
+    x = t;
   }
 }
 
@@ -182,14 +146,9 @@ template <int DT, int C>
 __device__ __forceinline__ Run<C> load_w(const void* w, int w_fp32, int c) {
   Run<C> f;
 #pragma unroll
-  for (int i = 0; i < C / 2; ++i) {
-    if (w_fp32) {
-      const float* p = static_cast<const float*>(w) + c + 2 * i;
-      f.p[i] = f2pack(__ldg(p), __ldg(p + 1));
-    } else {
-      const uint16_t* p = static_cast<const uint16_t*>(w) + c + 2 * i;
-      f.p[i] = f2pack(unpack2<DT>(uint32_t(__ldg(p))).x, unpack2<DT>(uint32_t(__ldg(p + 1))).x);
-    }
+  for (int i = 0; i < C; ++i) {
+    f.v[i] = w_fp32 ? __ldg(static_cast<const float*>(w) + c + i)
+                    : unpack2<DT>(uint32_t(__ldg(static_cast<const uint16_t*>(w) + c + i))).x;
   }
   return f;
 }
@@ -200,281 +159,311 @@ __device__ __forceinline__ float group_sum(float v) {
   for (int m = L / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
 }
-template <int L>
-__device__ __forceinline__ uint64_t group_sum2(uint64_t v) {
-#pragma unroll
-  for (int m = L / 2; m > 0; m >>= 1) v = fadd2(v, __shfl_xor_sync(0xffffffffu, v, m));
-  return v;
+__device__ __forceinline__ int raw_pos(const RotaryArgs& a, int b, int n) {
+  return a.pos ? __ldg(a.pos + (long long)b * a.pos_sb + n) : n;
 }
-
-// Position of token (b, n), or -1 (with the device status word set) when it
-// has no row in the table.
-__device__ __forceinline__ int checked_pos(const RotaryArgs& a, int b, int n) {
-  const int p = a.pos ? __ldg(a.pos + (long long)b * a.pos_sb + n) : n;
+// The position, or -1 (with the device status word set) when it has no row in
+// the table.
+__device__ __forceinline__ int checked_pos(const RotaryArgs& a, int p) {
   if (p >= 0 && p < a.max_pos) return p;
   if (a.status) atomicCAS(a.status, 0, (FA_SITE_POSITION << 8) | FA_ERR_BAD_INDEX);
   return -1;
 }
-template <bool INTER, int C>
-__device__ __forceinline__ Angles<INTER, C> load_angles(const RotaryArgs& a, int p, int l) {
-  Run<C> cs, sn;
-  if (p >= 0) {
-    const float* t = a.table + (long long)p * a.rd + C * l;
-    cs = ld_floats<C>(t);
-    sn = ld_floats<C>(t + a.rd / 2);
-  } else {  // no such position: the turned columns come out NaN
-#pragma unroll
-    for (int i = 0; i < C / 2; ++i) cs.p[i] = sn.p[i] = both(__int_as_float(0x7fc00000));
-  }
-  return arrange<INTER, C>(cs, sn);
+constexpr int THREADS = 128;
+constexpr int WARPS = THREADS / 32;
+// Steps of a ring and blocks a SM.  Measured at B2 H32/8 N8191 D128 bf16 (HBM
+// alone takes 51 and 77 us): forward 4 steps x 5 blocks 58 us, 6 x 4 60, 5 x 6
+// 59; backward 3 x 4 85 us, 4 x 4 87, 4 x 3 87 (and 113 with C = 4).
+constexpr int FWD_STEPS = 4, FWD_BLOCKS = 5;
+constexpr int BWD_STEPS = 3, BWD_BLOCKS = 4;
+template <int D>
+constexpr int run_cols() {  // C: of narrow rows fewer, so that a step is 8 rows at most
+  return D == 32 ? 4 : 8;
 }
 
-#ifndef T_FC
-#define T_FC 8
-#endif
-#ifndef T_BC
-#define T_BC 4
-#endif
-#ifndef T_HB
-#define T_HB 4
-#endif
-#ifndef T_BHB
-#define T_BHB 4
-#endif
-#ifndef T_FMIN
-#define T_FMIN 2
-#endif
-#ifndef T_BMIN
-#define T_BMIN 2
-#endif
-#ifndef T_BCTAS
-#define T_BCTAS 296
-#endif
-#ifndef T_FT
-#define T_FT 256
-#endif
-#ifndef T_BT
-#define T_BT 256
-#endif
-constexpr int FWD_THREADS = T_FT;
-constexpr int FC = T_FC;  // columns of a lane's run
-constexpr int HB = T_HB;  // heads a group of lanes takes of one token
+// A warp's ring of ST steps in shared memory: a step's rows (STREAMS runs a and
+// b of 32 lanes) and its token's angles (cosines, sines of a row's lanes).
+template <int D, int C, int ST, int STREAMS>
+struct Ring {
+  static constexpr uint32_t RUN = 2 * C;                    // bytes
+  static constexpr uint32_t LANES = D / (2 * C);            // of a row
+  static constexpr uint32_t ANGLES = 32 * 2 * RUN * STREAMS;  // where they begin
+  static constexpr uint32_t STEP = ANGLES + LANES * 8 * C;
+  static constexpr uint32_t BYTES = ST * STEP;
+  static_assert(STEP % 16 == 0, "16-byte copies");
+};
 
-// One group of D / 2 C lanes per (token, HB heads of q, of k or -- APPEND --
-// of v); groups of one token are neighbours, so that they share its table
-// row in L1.  APPEND: k and v rows go to row slots[n] of the caches.
-template <int D, int DT, bool INTER, bool APPEND>
-__global__ void __launch_bounds__(FWD_THREADS, T_FMIN) fa_rotary_fwd_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int C = FC;
+// Fetches a token's angles, 16 bytes a copy, by the lanes of the first group.
+// A position without a row in the table gives NaN.
+template <int D, int C>
+__device__ __forceinline__ void fetch_angles(const RotaryArgs& a, uint32_t to, int p, int lane) {
+  constexpr uint32_t LANES = D / (2 * C);
+  if (lane < int(LANES) && lane < a.rd / (2 * C)) {
+    const float* t = a.table + (long long)max(p, 0) * a.rd + C * lane;
+#pragma unroll
+    for (int i = 0; i < C / 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // cosines, sines
+        const uint32_t at = to + uint32_t(j * (C / 4) + i) * (LANES * 16) + lane * 16;
+        if (p >= 0)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(at), "l"(t + j * (a.rd / 2) + 4 * i)
+                       : "memory");
+        else
+          st_shared_v4(at, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u, 0x7fc00000u);
+      }
+  }
+}
+template <int D, int C>
+__device__ __forceinline__ Angles<C> read_angles(uint32_t from, int l) {
+  constexpr uint32_t LANES = D / (2 * C);
+  Angles<C> g;
+#pragma unroll
+  for (int i = 0; i < C / 4; ++i) {
+    const float4 c = ld_shared_f4(from + uint32_t(i) * (LANES * 16) + l * 16);
+    const float4 s = ld_shared_f4(from + uint32_t(C / 4 + i) * (LANES * 16) + l * 16);
+    g.c.v[4 * i] = c.x, g.c.v[4 * i + 1] = c.y, g.c.v[4 * i + 2] = c.z, g.c.v[4 * i + 3] = c.w;
+    g.s.v[4 * i] = s.x, g.s.v[4 * i + 1] = s.y, g.s.v[4 * i + 2] = s.z, g.s.v[4 * i + 3] = s.w;
+  }
+  return g;
+}
+
+// The tokens of a warp's range, one after the other: where a token's row of
+// head h lies in a tensor, and its position.
+struct Rows {
+  const uint16_t* p;
+  long long sn, sb;  // to the next token; from a batch's last token to the next batch's first
+  __device__ __forceinline__ Rows(const void* base, const RowStrides& s, int N, int b, int n, int h, int col)
+      : p(static_cast<const uint16_t*>(base) + (b * s.b + n * s.n + h * s.h + col)),
+        sn(s.n),
+        sb(s.b - (N - 1) * s.n) {}
+  __device__ __forceinline__ void next(bool batch_ends) { p += batch_ends ? sb : sn; }
+};
+
+// Range of a warp: `parts` warps share all tokens for the same heads.
+struct Range {
+  int count, b, n;
+  __device__ __forceinline__ Range(const RotaryArgs& a, int part, int per_part) {
+    const long long tokens = (long long)a.B * a.N, first = (long long)part * per_part;
+    count = int(min((long long)per_part, tokens - first));
+    b = int(first / a.N);
+    n = int(first - (long long)b * a.N);
+  }
+};
+
+// Forward.  Chunks of GW heads: the query's, the key's and -- APPEND -- the
+// value's, which are copied as they are; k and v rows go to row slots[n] of
+// the caches.  Warps of a block take neighbouring chunks of the same tokens.
+template <int D, int DT, bool INTER, bool NORM, bool APPEND>
+__global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int C = run_cols<D>();
   constexpr int L = D / (2 * C);
-  const uint32_t item = (blockIdx.x * uint32_t(FWD_THREADS) + threadIdx.x) / L;
-  const int l = threadIdx.x % L;
-  const int q_blocks = (a.Hq + HB - 1) / HB, k_blocks = (a.Hkv + HB - 1) / HB;
-  const uint32_t per_token = q_blocks + k_blocks * (APPEND ? 2 : 1);
-  const uint32_t token = item / per_token;
-  int blk = int(item - token * per_token);
-  // groups past the end stay for the shuffles and touch nothing
-  const bool live = token < uint32_t(a.B) * uint32_t(a.N);
-  const int b = live ? int(token / uint32_t(a.N)) : 0;
-  const int n = live ? int(token - uint32_t(b) * uint32_t(a.N)) : 0;
-  const int which = blk < q_blocks ? 0 : blk < q_blocks + k_blocks ? 1 : 2;
-  blk -= which == 0 ? 0 : which == 1 ? q_blocks : q_blocks + k_blocks;
-  const int h0 = blk * HB;
-  const int heads = live ? min(HB, (which == 0 ? a.Hq : a.Hkv) - h0) : 0;
-  const uint16_t* src = static_cast<const uint16_t*>(which == 0 ? a.q : which == 1 ? a.k : a.v);
-  const RowStrides si = which == 0 ? a.qs : which == 1 ? a.ks : a.vs;
+  constexpr int GW = 32 / L;
+  constexpr int ST = FWD_STEPS;
+  using R = Ring<D, C, ST, 1>;
+  extern __shared__ __align__(16) unsigned char ring[];
+  const int lane = threadIdx.x & 31, l = lane % L;
+  const uint32_t mem = smem_u32(ring) + (threadIdx.x / 32) * R::BYTES;
   const LaneCols c = lane_cols<INTER, C>(l, a.rd);
-  src += (long long)b * si.b + (long long)n * si.n + (long long)h0 * si.h;
-  Raw<C> va[HB], vb[HB];
-#pragma unroll
-  for (int i = 0; i < HB; ++i)
-    if (i < heads) {
-      va[i] = ld_stream<C>(src + (long long)i * si.h + c.a);
-      vb[i] = ld_stream<C>(src + (long long)i * si.h + c.b);
-    }
-  uint16_t* dst;
-  RowStrides so;
-  int stored = heads;
-  if (which == 0 || !APPEND) {
-    dst = static_cast<uint16_t*>(which == 0 ? a.qo : a.ko);
-    so = which == 0 ? a.qos : a.kos;
-    dst += (long long)b * so.b + (long long)n * so.n + (long long)h0 * so.h;
-  } else {
-    so.h = D;
-    long long slot = live ? __ldg(a.slots + n) : -1;
-    if (slot >= a.n_slots) {
-      if (a.status) atomicCAS(a.status, 0, (FA_SITE_SLOT << 8) | FA_ERR_BAD_INDEX);
-      slot = -1;
-    }
-    if (slot < 0) stored = 0, slot = 0;
-    dst = static_cast<uint16_t*>(which == 1 ? a.ko : a.vo) + (slot * a.Hkv + h0) * D;
-  }
-  if (APPEND && which == 2) {
-#pragma unroll
-    for (int i = 0; i < HB; ++i)
-      if (i < stored) {
-        st_run<C>(dst + (long long)i * so.h + c.a, va[i]);
-        st_run<C>(dst + (long long)i * so.h + c.b, vb[i]);
-      }
-    stored = 0;
-  }
-  if (APPEND && __all_sync(0xffffffffu, which == 2)) return;
-  Angles<INTER, C> g;
-  const bool turned = c.turned && which != 2 && heads > 0;
-  if (turned) g = load_angles<INTER, C>(a, checked_pos(a, b, n), l);
-  const bool norm = a.wq != nullptr;  // of every row of the launch
-  Run<C> wa, wb;
-  if (norm) {
-    const void* w = which == 0 ? a.wq : a.wk;
-    wa = load_w<DT, C>(w, a.w_fp32, c.a);
-    wb = load_w<DT, C>(w, a.w_fp32, c.b);
-  }
-#pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    Run<C> x, y;
-    if (i < heads) {
-      x = widen<DT, C>(va[i]);
-      y = widen<DT, C>(vb[i]);
-    } else {
-      x = y = zero_run<C>();
-    }
-    if (norm) {
-      uint64_t ss = 0;
-#pragma unroll
-      for (int j = 0; j < C / 2; ++j) ss = ffma2(x.p[j], x.p[j], ffma2(y.p[j], y.p[j], ss));
-      const float s = group_sum<L>(add_halves(ss));  // all lanes of the warp come here
-      const uint64_t r = both(rsqrtf(s * (1.f / D) + a.eps));
-#pragma unroll
-      for (int j = 0; j < C / 2; ++j) {
-        x.p[j] = fmul2(x.p[j], fmul2(r, wa.p[j]));
-        y.p[j] = fmul2(y.p[j], fmul2(r, wb.p[j]));
-      }
-    }
-    if (turned) turn<INTER, false, C>(x, y, g);
-    if (i < stored) {
-      st_run<C>(dst + (long long)i * so.h + c.a, narrow<DT, C>(x));
-      st_run<C>(dst + (long long)i * so.h + c.b, narrow<DT, C>(y));
-    }
-  }
-}
+  const int ab = c.b - c.a;
+  const int q_chunks = (a.Hq + GW - 1) / GW, k_chunks = (a.Hkv + GW - 1) / GW;
+  const int chunks = q_chunks + k_chunks * (APPEND ? 2 : 1);
+  const int wid = blockIdx.x * WARPS + threadIdx.x / 32;
+  const int part = wid / chunks, chunk = wid - part * chunks;
+  if (part >= a.parts) return;
+  const int kind = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;
+  const int h = (chunk - (kind == 0 ? 0 : kind == 1 ? q_chunks : q_chunks + k_chunks)) * GW + lane / L;
+  const bool valid = h < (kind == 0 ? a.Hq : a.Hkv);
+  const Range range(a, part, a.per_part);
 
-constexpr int BWD_THREADS = T_BT;
-constexpr int BC = T_BC;
-constexpr int BWD_HB = T_BHB;
+  // rows and angles to come: one group of copies a step, empty behind the end
+  Rows src(kind == 0 ? a.q : kind == 1 ? a.k : a.v, kind == 0 ? a.qs : kind == 1 ? a.ks : a.vs, a.N, range.b, range.n,
+           h, c.a);
+  int to_come = range.count, src_b = range.b, src_n = range.n;
+  int pos = raw_pos(a, src_b, src_n);
+  auto fetch = [&](uint32_t to) {
+    if (to_come > 0) {
+      copy_run<C>(to + lane * R::RUN, src.p, valid);
+      copy_run<C>(to + (32 + lane) * R::RUN, src.p + ab, valid);
+      if (!APPEND || kind != 2) fetch_angles<D, C>(a, to + R::ANGLES, checked_pos(a, pos), lane);
+      const bool ends = src_n + 1 == a.N;
+      src.next(ends);
+      src_n = ends ? 0 : src_n + 1;
+      src_b += ends;
+      if (--to_come > 0) pos = raw_pos(a, src_b, src_n);
+    }
+    copies_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < ST - 1; ++i) fetch(mem + i * R::STEP);
+
+  const bool cached = APPEND && kind != 0;
+  Rows dst(kind == 0 ? a.qo : kind == 1 ? a.ko : a.vo, kind == 0 ? a.qos : a.kos, a.N, cached ? 0 : range.b,
+           cached ? 0 : range.n, h, c.a);
+  Run<C> wa, wb;
+  if (NORM && kind != 2) {
+    wa = load_w<DT, C>(kind == 0 ? a.wq : a.wk, a.w_fp32, c.a);
+    wb = load_w<DT, C>(kind == 0 ? a.wq : a.wk, a.w_fp32, c.b);
+  }
+  int slot = cached ? __ldg(a.slots + range.n) : 0;
+  int n = range.n;
+  uint32_t here = mem;
+  for (int left = range.count; left > 0; --left) {
+    copies_wait<ST - 2>();
+    __syncwarp();  // the angles were copied by some lanes for all, and those of the step before are read
+    Raw<C> ra = ld_run<C>(here + lane * R::RUN), rb = ld_run<C>(here + (32 + lane) * R::RUN);
+    if (!APPEND || kind != 2) {
+      Run<C> x = widen<DT, C>(ra), y = widen<DT, C>(rb);
+      if (NORM) {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) s0 = fmaf(x.v[j], x.v[j], s0), s1 = fmaf(y.v[j], y.v[j], s1);
+        const float r = rsqrtf(group_sum<L>(s0 + s1) * (1.f / D) + a.eps);
+#pragma unroll
+        for (int j = 0; j < C; ++j) x.v[j] *= r * wa.v[j], y.v[j] *= r * wb.v[j];
+      }
+      if (c.turned) turn<INTER, false, C>(x, y, read_angles<D, C>(here + R::ANGLES, l));
+      ra = narrow<DT, C>(x);
+      rb = narrow<DT, C>(y);
+    }
+    if (cached) {
+      const bool in = slot >= 0 && slot < a.n_slots;
+      if (slot >= a.n_slots && a.status) atomicCAS(a.status, 0, (FA_SITE_SLOT << 8) | FA_ERR_BAD_INDEX);
+      uint16_t* p = const_cast<uint16_t*>(dst.p) + (in ? (long long)slot * (a.Hkv * D) : 0);
+      if (valid && in) {
+        st_run<C>(p, ra);
+        st_run<C>(p + ab, rb);
+      }
+      if (left > 1) slot = __ldg(a.slots + ++n);
+    } else {
+      if (valid) {
+        st_run<C>(const_cast<uint16_t*>(dst.p), ra);
+        st_run<C>(const_cast<uint16_t*>(dst.p) + ab, rb);
+      }
+      const bool ends = n + 1 == a.N;
+      dst.next(ends);
+      n = ends ? 0 : n + 1;
+    }
+    // into the place of the step before, which every lane has read
+    fetch(here == mem ? mem + (ST - 1) * R::STEP : here - R::STEP);
+    here = here == mem + (ST - 1) * R::STEP ? mem : here + R::STEP;
+  }
+  copies_wait<0>();
+}
 
 // Backward.  The first q_ctas blocks take the query rows, the others the key
-// rows, so that a lane's weight-gradient sums (2 C fp32 registers) are of one
-// weight; each block loops over its (token, BWD_HB heads) items and leaves
-// its sums in w_part[block][D] for the reduction that follows.  The sums run
-// in an order that the launch alone decides, so gradients repeat bit for bit.
-template <int D, int DT, bool INTER>
-__global__ void __launch_bounds__(BWD_THREADS, T_BMIN) fa_rotary_bwd_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int C = BC;
+// rows, so that a block's weight-gradient sums (2 C fp32 registers a lane) are
+// of one weight; it leaves them in w_part[block][D] for the reduction that
+// follows.  The sums run in an order that the launch alone decides, so
+// gradients repeat bit for bit.
+template <int D, int DT, bool INTER, bool NORM>
+__global__ void __launch_bounds__(THREADS, BWD_BLOCKS) fa_rotary_bwd_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int C = run_cols<D>();
   constexpr int L = D / (2 * C);
-  constexpr int GROUPS = BWD_THREADS / L;
+  constexpr int GW = 32 / L;
+  constexpr int ST = BWD_STEPS;
+  using R = Ring<D, C, ST, 2>;  // gradients, then rows
+  extern __shared__ __align__(16) unsigned char ring[];
   const bool is_q = int(blockIdx.x) < a.q_ctas;
-  const uint32_t cta = is_q ? blockIdx.x : blockIdx.x - a.q_ctas;
-  const uint32_t ctas = is_q ? a.q_ctas : gridDim.x - a.q_ctas;
-  const int l = threadIdx.x % L;
-  const int H = is_q ? a.Hq : a.Hkv;
-  const uint32_t blocks = (H + BWD_HB - 1) / BWD_HB;
-  const uint32_t items = uint32_t(a.B) * uint32_t(a.N) * blocks;
-  const uint16_t* xb = static_cast<const uint16_t*>(is_q ? a.q : a.k);
-  const uint16_t* gb = static_cast<const uint16_t*>(is_q ? a.gq : a.gk);
-  uint16_t* ob = static_cast<uint16_t*>(is_q ? a.qo : a.ko);
-  const RowStrides sx = is_q ? a.qs : a.ks, sg = is_q ? a.gqs : a.gks, so = is_q ? a.qos : a.kos;
-  const void* w = is_q ? a.wq : a.wk;
-  const bool norm = w != nullptr;
+  const int lane = threadIdx.x & 31, l = lane % L;
+  const uint32_t mem = smem_u32(ring) + (threadIdx.x / 32) * R::BYTES;
   const LaneCols c = lane_cols<INTER, C>(l, a.rd);
-  Run<C> wa, wb, dwa = zero_run<C>(), dwb = zero_run<C>();
-  if (norm) {
-    wa = load_w<DT, C>(w, a.w_fp32, c.a);
-    wb = load_w<DT, C>(w, a.w_fp32, c.b);
-  }
-  // the trip count is the block's, so that its warps stay whole for the shuffles
-  for (uint32_t base = cta * GROUPS; base < items; base += ctas * GROUPS) {
-    const uint32_t item = base + threadIdx.x / L;
-    const bool live = item < items;
-    const uint32_t token = live ? item / blocks : 0;
-    const int h0 = live ? int(item - token * blocks) * BWD_HB : 0;
-    const int heads = live ? min(BWD_HB, H - h0) : 0;
-    const int b = int(token / uint32_t(a.N));
-    const int n = int(token - uint32_t(b) * uint32_t(a.N));
-    const uint16_t* xp = xb + (long long)b * sx.b + (long long)n * sx.n + (long long)h0 * sx.h;
-    const uint16_t* gp = gb + (long long)b * sg.b + (long long)n * sg.n + (long long)h0 * sg.h;
-    uint16_t* op = ob + (long long)b * so.b + (long long)n * so.n + (long long)h0 * so.h;
-    Raw<C> xa[BWD_HB], xv[BWD_HB], ga[BWD_HB], gv[BWD_HB];
-#pragma unroll
-    for (int i = 0; i < BWD_HB; ++i)
-      if (i < heads) {
-        ga[i] = ld_stream<C>(gp + (long long)i * sg.h + c.a);
-        gv[i] = ld_stream<C>(gp + (long long)i * sg.h + c.b);
-        if (norm) {
-          xa[i] = ld_stream<C>(xp + (long long)i * sx.h + c.a);
-          xv[i] = ld_stream<C>(xp + (long long)i * sx.h + c.b);
-        }
+  const int ab = c.b - c.a;
+  const int H = is_q ? a.Hq : a.Hkv;
+  const int chunks = (H + GW - 1) / GW;
+  const int wid = (is_q ? blockIdx.x : blockIdx.x - a.q_ctas) * WARPS + threadIdx.x / 32;
+  const int part = wid / chunks, h = (wid - part * chunks) * GW + lane / L;
+  const bool valid = h < H;
+  const int per_part = is_q ? a.per_part : a.k_per_part;
+  Run<C> dwa = fill_run<C>(0.f), dwb = dwa;
+  if (part < (is_q ? a.parts : a.k_parts)) {
+    const Range range(a, part, per_part);
+    Rows gp(is_q ? a.gq : a.gk, is_q ? a.gqs : a.gks, a.N, range.b, range.n, h, c.a);
+    Rows xp(is_q ? a.q : a.k, is_q ? a.qs : a.ks, a.N, range.b, range.n, h, c.a);
+    Rows dst(is_q ? a.qo : a.ko, is_q ? a.qos : a.kos, a.N, range.b, range.n, h, c.a);
+    int to_come = range.count, src_b = range.b, src_n = range.n;
+    int pos = raw_pos(a, src_b, src_n);
+    auto fetch = [&](uint32_t to) {
+      if (to_come > 0) {
+        copy_run<C>(to + lane * R::RUN, gp.p, valid);
+        copy_run<C>(to + (32 + lane) * R::RUN, gp.p + ab, valid);
+        copy_run<C>(to + (64 + lane) * R::RUN, xp.p, NORM && valid);
+        copy_run<C>(to + (96 + lane) * R::RUN, xp.p + ab, NORM && valid);
+        fetch_angles<D, C>(a, to + R::ANGLES, checked_pos(a, pos), lane);
+        const bool ends = src_n + 1 == a.N;
+        gp.next(ends);
+        xp.next(ends);
+        src_n = ends ? 0 : src_n + 1;
+        src_b += ends;
+        if (--to_come > 0) pos = raw_pos(a, src_b, src_n);
       }
-    Angles<INTER, C> g;
-    const bool turned = c.turned && heads > 0;
-    if (turned) g = load_angles<INTER, C>(a, checked_pos(a, b, n), l);
-#pragma unroll
-    for (int i = 0; i < BWD_HB; ++i) {
-      Run<C> ya, yb;
-      if (i < heads) {
-        ya = widen<DT, C>(ga[i]);
-        yb = widen<DT, C>(gv[i]);
-      } else {
-        ya = yb = zero_run<C>();
-      }
-      if (turned && i < heads) turn<INTER, true, C>(ya, yb, g);
-      if (norm) {
-        Run<C> x, y;
-        if (i < heads) {
-          x = widen<DT, C>(xa[i]);
-          y = widen<DT, C>(xv[i]);
-        } else {
-          x = y = zero_run<C>();
-        }
-        uint64_t ss = 0, gx = 0;
+      copies_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < ST - 1; ++i) fetch(mem + i * R::STEP);
+    Run<C> wa, wb;
+    if (NORM) {
+      wa = load_w<DT, C>(is_q ? a.wq : a.wk, a.w_fp32, c.a);
+      wb = load_w<DT, C>(is_q ? a.wq : a.wk, a.w_fp32, c.b);
+    }
+    int n = range.n;
+    uint32_t here = mem;
+    for (int left = range.count; left > 0; --left) {
+      copies_wait<ST - 2>();
+      __syncwarp();
+      Run<C> ya = widen<DT, C>(ld_run<C>(here + lane * R::RUN));
+      Run<C> yb = widen<DT, C>(ld_run<C>(here + (32 + lane) * R::RUN));
+      if (c.turned) turn<INTER, true, C>(ya, yb, read_angles<D, C>(here + R::ANGLES, l));
+      if (NORM) {
+        const Run<C> x = widen<DT, C>(ld_run<C>(here + (64 + lane) * R::RUN));
+        const Run<C> y = widen<DT, C>(ld_run<C>(here + (96 + lane) * R::RUN));
+        float ss = 0.f, gx = 0.f;
         Run<C> ta, tb;  // dy w
 #pragma unroll
-        for (int j = 0; j < C / 2; ++j) {
-          ta.p[j] = fmul2(ya.p[j], wa.p[j]);
-          tb.p[j] = fmul2(yb.p[j], wb.p[j]);
-          ss = ffma2(x.p[j], x.p[j], ffma2(y.p[j], y.p[j], ss));
-          gx = ffma2(ta.p[j], x.p[j], ffma2(tb.p[j], y.p[j], gx));
+        for (int j = 0; j < C; ++j) {
+          ta.v[j] = ya.v[j] * wa.v[j];
+          tb.v[j] = yb.v[j] * wb.v[j];
+          ss = fmaf(x.v[j], x.v[j], fmaf(y.v[j], y.v[j], ss));
+          gx = fmaf(ta.v[j], x.v[j], fmaf(tb.v[j], y.v[j], gx));
         }
-        float s, t;
-        f2unpack(group_sum2<L>(f2pack(add_halves(ss), add_halves(gx))), s, t);
-        const float r = rsqrtf(s * (1.f / D) + a.eps);
-        const uint64_t rr = both(r), m = both(-t * (1.f / D) * r * r);
+        ss = group_sum<L>(ss);
+        gx = group_sum<L>(gx);
+        const float r = rsqrtf(ss * (1.f / D) + a.eps);
+        const float m = -gx * (1.f / D) * r * r;
 #pragma unroll
-        for (int j = 0; j < C / 2; ++j) {
-          const uint64_t xr = fmul2(x.p[j], rr), yr = fmul2(y.p[j], rr);
-          dwa.p[j] = ffma2(ya.p[j], xr, dwa.p[j]);
-          dwb.p[j] = ffma2(yb.p[j], yr, dwb.p[j]);
-          ya.p[j] = ffma2(xr, m, fmul2(ta.p[j], rr));
-          yb.p[j] = ffma2(yr, m, fmul2(tb.p[j], rr));
+        for (int j = 0; j < C; ++j) {
+          const float xr = x.v[j] * r, yr = y.v[j] * r;
+          dwa.v[j] = fmaf(ya.v[j], xr, dwa.v[j]);
+          dwb.v[j] = fmaf(yb.v[j], yr, dwb.v[j]);
+          ya.v[j] = fmaf(xr, m, ta.v[j] * r);
+          yb.v[j] = fmaf(yr, m, tb.v[j] * r);
         }
       }
-      if (i < heads) {
-        st_run<C>(op + (long long)i * so.h + c.a, narrow<DT, C>(ya));
-        st_run<C>(op + (long long)i * so.h + c.b, narrow<DT, C>(yb));
+      if (valid) {
+        st_run<C>(const_cast<uint16_t*>(dst.p), narrow<DT, C>(ya));
+        st_run<C>(const_cast<uint16_t*>(dst.p) + ab, narrow<DT, C>(yb));
       }
+      const bool ends = n + 1 == a.N;
+      dst.next(ends);
+      n = ends ? 0 : n + 1;
+      fetch(here == mem ? mem + (ST - 1) * R::STEP : here - R::STEP);
+      here = here == mem + (ST - 1) * R::STEP ? mem : here + R::STEP;
     }
+    copies_wait<0>();
   }
-  if (!norm || a.w_part == nullptr) return;
-  __shared__ float sums[GROUPS][D + 4];
+  if (!NORM || a.w_part == nullptr) return;
+  static_assert(WARPS * GW * (D + 4) * 4 <= WARPS * R::BYTES, "the sums reuse the ring");
+  float(*sums)[D + 4] = reinterpret_cast<float(*)[D + 4]>(ring);
+  __syncthreads();  // every warp is done with its part of the ring
   float* mine = sums[threadIdx.x / L];
 #pragma unroll
-  for (int j = 0; j < C / 2; ++j) {
-    f2unpack(dwa.p[j], mine[c.a + 2 * j], mine[c.a + 2 * j + 1]);
-    f2unpack(dwb.p[j], mine[c.b + 2 * j], mine[c.b + 2 * j + 1]);
+  for (int j = 0; j < C; ++j) {
+    mine[c.a + j] = valid ? dwa.v[j] : 0.f;  // what lanes without a head worked on is nothing
+    mine[c.b + j] = valid ? dwb.v[j] : 0.f;
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < D; d += BWD_THREADS) {
+  for (int d = threadIdx.x; d < D; d += THREADS) {
     float s = 0.f;
-    for (int g = 0; g < GROUPS; ++g) s += sums[g][d];
+    for (int r = 0; r < WARPS * GW; ++r) s += sums[r][d];
     a.w_part[(long long)blockIdx.x * D + d] = s;
   }
 }
@@ -507,72 +496,84 @@ __global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const float* __restr
     static_cast<uint16_t*>(out)[c] = uint16_t(pack2<DT>(v, 0.f) & 0xffffu);
 }
 
-template <int D, int DT, bool INTER, bool APPEND>
-int run_fwd(const RotaryArgs& a) {
-  const long long per = (a.Hq + HB - 1) / HB + (long long)((a.Hkv + HB - 1) / HB) * (APPEND ? 2 : 1);
-  const long long items = per * a.B * a.N;
-  constexpr int GROUPS = FWD_THREADS / (D / (2 * FC));
-  if (items > 0x7fffffffLL * GROUPS || items + GROUPS > 0xffffffffLL) return FA_ERR_BAD_SHAPE;
-  fa_rotary_fwd_kernel<D, DT, INTER, APPEND>
-      <<<unsigned((items + GROUPS - 1) / GROUPS), FWD_THREADS, 0, a.stream>>>(a);
+// Ranges of tokens for `warps` warps that share `chunks` chunks of heads:
+// returns how many, each per_part long.
+int cut_tokens(long long tokens, int chunks, long long warps, int* per_part) {
+  long long parts = warps / chunks;
+  if (parts < 1) parts = 1;
+  if (parts > tokens) parts = tokens;
+  *per_part = int((tokens + parts - 1) / parts);
+  return int((tokens + *per_part - 1) / *per_part);
+}
+
+template <int D, int DT, bool INTER, bool NORM, bool APPEND>
+int run_fwd(RotaryArgs a) {
+  constexpr int GW = 64 * run_cols<D>() / D;
+  constexpr int smem = WARPS * Ring<D, run_cols<D>(), FWD_STEPS, 1>::BYTES;
+  static_assert(smem <= 48 * 1024, "no larger than any kernel may have");
+  const long long tokens = (long long)a.B * a.N, most = (long long)device_sm_count() * FWD_BLOCKS;
+  const int chunks = (a.Hq + GW - 1) / GW + (a.Hkv + GW - 1) / GW * (APPEND ? 2 : 1);
+  a.parts = cut_tokens(tokens, chunks, most * WARPS, &a.per_part);
+  const long long ctas = ((long long)a.parts * chunks + WARPS - 1) / WARPS;
+  if (ctas * WARPS > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
+  fa_rotary_fwd_kernel<D, DT, INTER, NORM, APPEND><<<unsigned(ctas), THREADS, smem, a.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-template <int D, int DT, bool INTER>
+template <int D, int DT, bool INTER, bool NORM>
 int run_bwd(RotaryArgs a) {
-  constexpr int GROUPS = BWD_THREADS / (D / (2 * BC));
-  const long long rows = (long long)a.B * a.N;
-  const long long q_items = rows * ((a.Hq + BWD_HB - 1) / BWD_HB), k_items = rows * ((a.Hkv + BWD_HB - 1) / BWD_HB);
-  if (q_items + 4096LL * GROUPS > 0xffffffffLL || k_items + 4096LL * GROUPS > 0xffffffffLL) return FA_ERR_BAD_SHAPE;
-  int q_ctas, k_ctas;
-  rotary_bwd_ctas(a.Hq, a.Hkv, rows, D, &q_ctas, &k_ctas);
-  a.q_ctas = q_ctas;
-  fa_rotary_bwd_kernel<D, DT, INTER><<<q_ctas + k_ctas, BWD_THREADS, 0, a.stream>>>(a);
+  constexpr int GW = 64 * run_cols<D>() / D;
+  constexpr int smem = WARPS * Ring<D, run_cols<D>(), BWD_STEPS, 2>::BYTES;
+  static_assert(smem <= 48 * 1024, "no larger than any kernel may have");
+  // blocks shared between queries and keys by their chunks of heads
+  const long long tokens = (long long)a.B * a.N;
+  long long most = (long long)device_sm_count() * BWD_BLOCKS;
+  if (most > ROTARY_BWD_CTAS) most = ROTARY_BWD_CTAS;
+  const int q_chunks = (a.Hq + GW - 1) / GW, k_chunks = (a.Hkv + GW - 1) / GW;
+  long long k_most = most * k_chunks / (q_chunks + k_chunks);
+  if (k_most < 1) k_most = 1;
+  a.parts = cut_tokens(tokens, q_chunks, (most - k_most) * WARPS, &a.per_part);
+  a.k_parts = cut_tokens(tokens, k_chunks, k_most * WARPS, &a.k_per_part);
+  const long long q_ctas = ((long long)a.parts * q_chunks + WARPS - 1) / WARPS;
+  const long long k_ctas = ((long long)a.k_parts * k_chunks + WARPS - 1) / WARPS;
+  // thousands of heads: more chunks than warps, which would take more rows of
+  // w_part than there are
+  if (q_ctas + k_ctas > ROTARY_BWD_CTAS) return FA_ERR_BAD_SHAPE;
+  a.q_ctas = int(q_ctas);
+  fa_rotary_bwd_kernel<D, DT, INTER, NORM><<<unsigned(q_ctas + k_ctas), THREADS, smem, a.stream>>>(a);
   if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
   if (a.w_part) {
-    fa_rotary_dw_kernel<DT><<<dim3(D / 32, 2), 1024, 0, a.stream>>>(a.w_part, D, q_ctas, q_ctas + k_ctas, a.dwq, a.dwk, a.w_fp32);
+    fa_rotary_dw_kernel<DT><<<dim3(D / 32, 2), 1024, 0, a.stream>>>(a.w_part, D, int(q_ctas), int(q_ctas + k_ctas),
+                                                                    a.dwq, a.dwk, a.w_fp32);
     if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
   }
   return FA_OK;
 }
 
-template <int DT, bool INTER, bool APPEND>
-int by_d(const RotaryArgs& a, int D, bool bwd) {
-  if constexpr (!APPEND)
-    if (bwd) {
-      if (D == 32) return run_bwd<32, DT, INTER>(a);
-      if (D == 64) return run_bwd<64, DT, INTER>(a);
-      return run_bwd<128, DT, INTER>(a);
-    }
-  if (D == 32) return run_fwd<32, DT, INTER, APPEND>(a);
-  if (D == 64) return run_fwd<64, DT, INTER, APPEND>(a);
-  return run_fwd<128, DT, INTER, APPEND>(a);
+// Instantiated for the head dims, operand types, pairings and with and
+// without a norm.
+enum class Op { kForward, kBackward, kAppend };
+template <Op OP, int D, int DT, bool INTER, bool NORM>
+int run(const RotaryArgs& a) {
+  if constexpr (OP == Op::kBackward) return run_bwd<D, DT, INTER, NORM>(a);
+  else return run_fwd<D, DT, INTER, NORM, OP == Op::kAppend>(a);
 }
-template <bool APPEND>
-int by_type(const RotaryArgs& a, int D, bool bwd) {
+template <Op OP, int D, int DT>
+int by_form(const RotaryArgs& a) {
+  if (a.wq) return a.interleaved ? run<OP, D, DT, true, true>(a) : run<OP, D, DT, false, true>(a);
+  return a.interleaved ? run<OP, D, DT, true, false>(a) : run<OP, D, DT, false, false>(a);
+}
+template <Op OP>
+int by_type(const RotaryArgs& a, int D) {
   if (a.dtype == DT_BF16)
-    return a.interleaved ? by_d<DT_BF16, true, APPEND>(a, D, bwd) : by_d<DT_BF16, false, APPEND>(a, D, bwd);
-  return a.interleaved ? by_d<DT_F16, true, APPEND>(a, D, bwd) : by_d<DT_F16, false, APPEND>(a, D, bwd);
+    return D == 32 ? by_form<OP, 32, DT_BF16>(a) : D == 64 ? by_form<OP, 64, DT_BF16>(a) : by_form<OP, 128, DT_BF16>(a);
+  return D == 32 ? by_form<OP, 32, DT_F16>(a) : D == 64 ? by_form<OP, 64, DT_F16>(a) : by_form<OP, 128, DT_F16>(a);
 }
 
 }  // namespace
 
-// Blocks of the backward: four a SM at most, shared between queries and keys
-// by their heads, none without a full turn of work.
-void rotary_bwd_ctas(int Hq, int Hkv, long long rows, int D, int* q_ctas, int* k_ctas) {
-  const long long groups = BWD_THREADS / (D / (2 * BC));
-  const long long most = T_BCTAS;
-  const long long q_need = (rows * ((Hq + BWD_HB - 1) / BWD_HB) + groups - 1) / groups;
-  const long long k_need = (rows * ((Hkv + BWD_HB - 1) / BWD_HB) + groups - 1) / groups;
-  long long k = most * Hkv / (Hq + Hkv);
-  if (k < 1) k = 1;
-  const long long q = most - k;
-  *q_ctas = int(q < q_need ? q : q_need);
-  *k_ctas = int(k < k_need ? k : k_need);
-}
-
-int launch_rotary_fwd(const RotaryArgs& a, int D) { return by_type<false>(a, D, false); }
-int launch_rotary_bwd(const RotaryArgs& a, int D) { return by_type<false>(a, D, true); }
-int launch_paged_append(const RotaryArgs& a, int D) { return by_type<true>(a, D, false); }
+int launch_rotary_fwd(const RotaryArgs& a, int D) { return by_type<Op::kForward>(a, D); }
+int launch_rotary_bwd(const RotaryArgs& a, int D) { return by_type<Op::kBackward>(a, D); }
+int launch_paged_append(const RotaryArgs& a, int D) { return by_type<Op::kAppend>(a, D); }
 
 }  // namespace fa

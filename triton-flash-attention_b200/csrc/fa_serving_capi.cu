@@ -134,6 +134,7 @@ int append_impl(const void* q, const void* k, const void* v, void* q_out, void* 
   a.vs = strides(vs);
   a.qo = q_out;
   a.qos = RowStrides{0, D, (long long)Hq * D};
+  a.kos = RowStrides{0, D, (long long)Hkv * D};  // of a cache's rows
   a.ko = k_cache;
   a.vo = v_cache;
   a.slots = slots;

@@ -213,50 +213,67 @@ def _contiguous_like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def qk_norm_rotary_forward(q, k, table, positions, query_weight, key_weight, eps: float, interleaved: bool):
-    """Launch the forward: contiguous outputs in the inputs' layout."""
-    b, hq, hkv, n, d = _sizes(q, k)
+def _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved):
+    """The forward's launch; besides the outputs what the backward's takes of
+    it: the rows as they were read and the arguments both have."""
     q, qp, qs = row_arg(q)
     k, kp, ks = row_arg(k)
+    b, hq, hkv, n, d = _sizes(q, k)
+    max_positions, rd = table.shape
+    fp32 = query_weight is not None and query_weight.dtype == torch.float32
+    per_batch = n if positions is not None and positions.ndim == 2 else 0
     with on_device(q) as stream:
-        _, qop, qos = row_arg(qo := _contiguous_like(q))
-        _, kop, kos = row_arg(ko := _contiguous_like(k))
-        positions_, rd = table.shape
+        qo, ko = _contiguous_like(q), _contiguous_like(k)
+        _, qop, qos = row_arg(qo)
+        _, kop, kos = row_arg(ko)
         rc = _abi.entry("fa_qk_norm_rotary", q.dtype)(
             qp, kp, qop, kop, table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n,
-            d, positions_, rd, interleaved, query_weight is not None and query_weight.dtype == torch.float32, qs, ks,
-            qos, kos, n if positions is not None and positions.ndim == 2 else 0, eps, stream)
+            d, max_positions, rd, interleaved, fp32, qs, ks, qos, kos, per_batch, eps, stream)
     if rc:
         _abi.check(rc, "fa_qk_norm_rotary")
-    return qo, ko
+    return qo, ko, q, k, (b, hq, hkv, n, d, max_positions, rd, interleaved, fp32), (qs, ks, qos, kos, per_batch, eps)
+
+
+def _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, sizes, rest, weight_grads):
+    """The backward's launch, for q and k as ``_forward`` gave them back.  (It
+    runs on autograd's own thread, where host work costs more: what the
+    forward worked out is not worked out again.)"""
+    grad_q, gqp, gqs = row_arg(grad_q)
+    grad_k, gkp, gks = row_arg(grad_k)
+    qs, ks, qos, kos, per_batch, eps = rest
+    with on_device(q) as stream:
+        dq, dk = _contiguous_like(q), _contiguous_like(k)
+        dwq = dwk = part = None
+        if weight_grads:
+            dwq, dwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
+            part = torch.empty(ROTARY_PARTIALS * sizes[4], device=q.device, dtype=torch.float32)
+        rc = _abi.entry("fa_qk_norm_rotary_bwd", q.dtype)(
+            q.data_ptr(), k.data_ptr(), gqp, gkp, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk), _ptr(part),
+            table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight), *sizes, qs, ks, gqs, gks, qos,
+            kos, per_batch, eps, stream)
+    if rc:
+        _abi.check(rc, "fa_qk_norm_rotary_bwd")
+    return dq, dk, dwq, dwk
+
+
+def qk_norm_rotary_forward(q, k, table, positions, query_weight, key_weight, eps: float, interleaved: bool):
+    """Launch the forward: contiguous outputs in the inputs' layout."""
+    return _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved)[:2]
 
 
 def qk_norm_rotary_backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, eps: float,
                             interleaved: bool, weight_grads: bool = True):
     """dQ, dK and, with weights and ``weight_grads``, the weights' gradients
     (else None).  Gradients repeat bit for bit."""
-    b, hq, hkv, n, d = _sizes(q, k)
-    wants = weight_grads and query_weight is not None
-    q, qp, qs = row_arg(q)
-    k, kp, ks = row_arg(k)
-    grad_q, gqp, gqs = row_arg(grad_q)
-    grad_k, gkp, gks = row_arg(grad_k)
-    with on_device(q) as stream:
-        _, dqp, dqs = row_arg(dq := _contiguous_like(q))
-        _, dkp, dks = row_arg(dk := _contiguous_like(k))
-        dwq = dwk = part = None
-        if wants:
-            dwq, dwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
-            part = torch.empty(ROTARY_PARTIALS * d, device=q.device, dtype=torch.float32)
-        positions_, rd = table.shape
-        rc = _abi.entry("fa_qk_norm_rotary_bwd", q.dtype)(
-            qp, kp, gqp, gkp, dqp, dkp, _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions),
-            _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n, d, positions_, rd, interleaved,
-            query_weight is not None and query_weight.dtype == torch.float32, qs, ks, gqs, gks, dqs, dks,
-            n if positions is not None and positions.ndim == 2 else 0, eps, stream)
-    if rc:
-        _abi.check(rc, "fa_qk_norm_rotary_bwd")
-    return dq, dk, dwq, dwk
+    q, _, qs = row_arg(q)
+    k, _, ks = row_arg(k)
+    # the gradients of q and k are contiguous, in the layout of the outputs
+    qos, kos = (_strides_arg(torch.empty(t.shape, device="meta").stride()) for t in (q, k))
+    sizes = (*_sizes(q, k), *table.shape, interleaved,
+             query_weight is not None and query_weight.dtype == torch.float32)
+    per_batch = sizes[3] if positions is not None and positions.ndim == 2 else 0
+    return _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, sizes,
+                     (qs, ks, qos, kos, per_batch, eps), weight_grads and query_weight is not None)
 
 
 class B200QKNormRotary(torch.autograd.Function):
@@ -265,9 +282,10 @@ class B200QKNormRotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, query, key, table, positions, query_weight, key_weight, eps, interleaved):
+        qo, ko, query, key, ctx.sizes, ctx.rest = _forward(query, key, table, positions, query_weight, key_weight, eps,
+                                                           interleaved)
         ctx.save_for_backward(query, key, table, positions, query_weight, key_weight)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return qk_norm_rotary_forward(query, key, table, positions, query_weight, key_weight, eps, interleaved)
+        return qo, ko
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):
@@ -275,8 +293,8 @@ class B200QKNormRotary(torch.autograd.Function):
             raise RuntimeError("qk_norm_rotary is differentiable once: its backward has no gradient (create_graph)")
         query, key, table, positions, query_weight, key_weight = ctx.saved_tensors
         needs = ctx.needs_input_grad
-        dq, dk, dwq, dwk = qk_norm_rotary_backward(query, key, grad_query, grad_key, table, positions, query_weight,
-                                                   key_weight, ctx.eps, ctx.interleaved, needs[4] or needs[5])
+        dq, dk, dwq, dwk = _backward(query, key, grad_query, grad_key, table, positions, query_weight, key_weight,
+                                     ctx.sizes, ctx.rest, needs[4] or needs[5])
         return dq, dk, None, None, dwq, dwk, None, None
 
 
