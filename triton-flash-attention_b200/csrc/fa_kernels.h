@@ -159,7 +159,7 @@ struct SelectArgs {
   const int *table, *cu, *seqlens;
   int* out;  // (total_q, Hkv, top)
   int B, Hq, Hkv, total_q, num_pages, page_log2, width, top, sink, local, dtype;
-  int cluster, share;  // set by the launch
+  int cluster;  // set by the launch
   int* status;
   cudaStream_t stream;
 };

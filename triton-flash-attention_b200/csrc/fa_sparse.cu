@@ -195,22 +195,34 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
 // block scores its share of the pages into the first block's shared memory,
 // which then finds the top ones.
 //
-// Scoring: D / 8 lanes own a page, 8 columns a lane, SEL_PAGES pages at once,
-// the next ones' loads in flight.  The group's queries lie in shared memory in
+// Scoring: a few lanes own a page, 16 columns a lane (8 of D = 32), SEL_PAGES
+// pages at once; asynchronous copies to the lane's own places in shared memory
+// bring the next batch meanwhile.  The group's queries lie in shared memory in
 // 64 bits and are taken SEL_HEADS heads at a time.  Lanes swap halves of
-// their page sums until each holds whole ones.  Bound: for a group of 4 heads
-// the 64-bit products (64 a clock and SM) take about as long as the means'
-// bytes, for larger ones longer.
+// their page sums until each holds whole ones; more columns a lane leave fewer
+// of these exchanges.
+// Bound: for a group of 4 heads the 64-bit products (64 a clock and SM) and
+// the conversions of the means (16) take about as long as the means' bytes;
+// for larger groups the products take longer.
 //
-// Selection: keys are the scores' bits in an order that whole numbers have,
-// neighbouring ones a thread.  The kk-th largest key is found two bits a
-// round, by block-wide counts of the keys at and above three candidates; the
-// pages above it, and of the pages at it the first ones, are written in order
-// of their index.
+// Selection: keys are the scores' bits in an order that whole numbers have.
+// Up to a key a thread, every thread counts the keys that go before its own.
+// For more, neighbouring keys a thread, the kk-th largest key is found two
+// bits a round, by block-wide counts of the keys at and above three
+// candidates; the pages above it, and of the pages at it the first ones, are
+// written in order of their index.
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
 constexpr int SEL_PAGES = 4;
 constexpr int SEL_HEADS = 4;
+template <int D>
+constexpr int sel_cols() {  // of a lane
+  return D == 32 ? 8 : 16;
+}
+template <int D>
+constexpr int sel_ring() {  // bytes of the two batches
+  return 2 * SEL_PAGES * SEL_THREADS * sel_cols<D>() * 2;
+}
 
 __device__ __forceinline__ uint32_t order_key(float f) {
   if (f != f) return 0u;  // NaN: behind everything
@@ -218,30 +230,45 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Scores of the block's pn pages (ids in shared memory), as keys to keys_at.
+// Scores of the block's pn pages, as keys to keys_at.  ids holds their pages
+// and may be where the keys go: a page's key replaces its id, which is read by
+// then.
 template <int D, int DT>
-__device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* qd, const int* ids, int h, int G,
-                                            int pn, uint32_t keys_at) {
-  constexpr int LP = D / 8;  // lanes of a page
+__device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* qd, const int* ids, uint32_t ring,
+                                            int h, int G, int pn, uint32_t keys_at) {
+  constexpr int CH = sel_cols<D>() / 8;  // 16-byte chunks of a lane
+  constexpr int LP = D / (8 * CH);       // lanes of a page
   constexpr int SUBS = SEL_THREADS / LP;
+  constexpr int BATCH = SUBS * SEL_PAGES;  // pages of the block's step
+  constexpr uint32_t PIECE = SEL_THREADS * 16, STAGE = SEL_PAGES * CH * PIECE;
   const int lane = threadIdx.x & 31;
   const int l = threadIdx.x % LP;
+  // chunk c of lane l: columns 8 (c LP + l) .. + 7
   const uint16_t* means = static_cast<const uint16_t*>(a.means) + (long long)h * D + 8 * l;
   const long long page_stride = (long long)a.Hkv * D;
-  auto load = [&](int first, uint4 (&v)[SEL_PAGES]) {
+  const uint32_t mine_at = ring + threadIdx.x * 16;
+  auto fetch = [&](int first, uint32_t to) {
 #pragma unroll
     for (int i = 0; i < SEL_PAGES; ++i) {
       const int id = first + i < pn ? ids[first + i] : -1;
-      v[i] = id >= 0 ? __ldg(reinterpret_cast<const uint4*>(means + id * page_stride)) : make_uint4(0, 0, 0, 0);
+      if (id >= 0)
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (i * CH + c) * PIECE),
+                       "l"(means + id * page_stride + c * (8 * LP))
+                       : "memory");
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // the trip count is the warp's, for the shuffles
   int first = (threadIdx.x / LP) * SEL_PAGES;
-  uint4 v[SEL_PAGES];
-  load(first, v);
-  for (int base = (threadIdx.x - lane) / LP * SEL_PAGES; base < pn; base += SUBS * SEL_PAGES, first += SUBS * SEL_PAGES) {
-    uint4 next[SEL_PAGES];
-    load(first + SUBS * SEL_PAGES, next);
+  fetch(first, mine_at);
+  uint32_t stage = 0;
+  // the trip count is the warp's, for the shuffles
+  for (int base = (threadIdx.x - lane) / LP * SEL_PAGES; base < pn; base += BATCH, first += BATCH) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const uint32_t from = mine_at + stage;
+    stage = STAGE - stage;
+    fetch(first + BATCH, mine_at + stage);  // where the batch before was, which this lane has read
     float best = -INFINITY;
     bool nan = false;
     for (int g0 = 0; g0 < G; g0 += SEL_HEADS) {
@@ -251,20 +278,29 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* 
 #pragma unroll
         for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = 0.0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        double lo[SEL_PAGES], hi[SEL_PAGES];
+      for (int c = 0; c < CH; ++c) {
+        uint32_t w[SEL_PAGES][4];  // what no page was copied to gives a sum that nobody looks at
 #pragma unroll
-        for (int i = 0; i < SEL_PAGES; ++i) {
-          const uint32_t w = j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w;
-          const float2 f = unpack2<DT>(w);
-          lo[i] = double(f.x);
-          hi[i] = double(f.y);
-        }
+        for (int i = 0; i < SEL_PAGES; ++i)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                       : "r"(from + (i * CH + c) * PIECE)
+                       : "memory");
 #pragma unroll
-        for (int g = 0; g < SEL_HEADS; ++g) {
-          const double2 x = qd[((g0 + g) * 4 + j) * LP + l];
+        for (int j = 0; j < 4; ++j) {
+          double lo[SEL_PAGES], hi[SEL_PAGES];
 #pragma unroll
-          for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = fma(x.y, hi[i], fma(x.x, lo[i], s[g][i]));
+          for (int i = 0; i < SEL_PAGES; ++i) {
+            const float2 f = unpack2<DT>(w[i][j]);
+            lo[i] = double(f.x);
+            hi[i] = double(f.y);
+          }
+#pragma unroll
+          for (int g = 0; g < SEL_HEADS; ++g) {
+            const double2 x = qd[((g0 + g) * (4 * CH) + c * 4 + j) * LP + l];
+#pragma unroll
+            for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = fma(x.y, hi[i], fma(x.x, lo[i], s[g][i]));
+          }
         }
       }
 #pragma unroll
@@ -289,9 +325,44 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* 
     const int mine = first + ((l & (LP / 2)) ? 2 : 0) + ((l & (LP / 4)) ? 1 : 0);
     if ((l & (LP / 4 - 1)) == 0 && mine < pn)
       st_cluster_u32(keys_at + 4u * uint32_t(mine), ids[mine] < 0 || nan ? 0u : order_key(best));
-#pragma unroll
-    for (int i = 0; i < SEL_PAGES; ++i) v[i] = next[i];
   }
+}
+
+// Writes the kk largest of M <= SEL_THREADS keys, a key a thread.
+__device__ __forceinline__ void write_top_small(uint32_t* keys, int M, int kk, int off, int* out) {
+  __shared__ int counts[SEL_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x;
+  const uint32_t mine = me < M ? keys[me] : 0u;
+  if (me >= M && me < (M + 3) / 4 * 4) keys[me] = 0u;
+  __syncthreads();
+  const int w0 = warp * 32, padded = (M + 3) / 4 * 4;  // the keys behind M are 0: behind all that count
+  int before = 0;                                      // keys that go before this one
+  if (w0 < M) {
+    // of equal keys those of lower index go before: all of the warps before, none of those behind
+#pragma unroll 4
+    for (int i = 0; i < w0; i += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+      before += (k.x >= mine) + (k.y >= mine) + (k.z >= mine) + (k.w >= mine);
+    }
+#pragma unroll 4
+    for (int i = w0 + 32; i < padded; i += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+      before += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const uint32_t k = __shfl_sync(0xffffffffu, mine, j);
+      before += k > mine || (k == mine && j < lane);
+    }
+  }
+  const bool kept = me < M && before < kk;
+  const uint32_t votes = __ballot_sync(0xffffffffu, kept);
+  if (lane == 0) counts[warp] = __popc(votes);
+  __syncthreads();
+  int at = __popc(votes & ((1u << lane) - 1u));
+#pragma unroll
+  for (int w = 0; w < SEL_WARPS; ++w) at += w < warp ? counts[w] : 0;
+  if (kept) out[at] = off + me;
 }
 
 // The kk largest of the M keys, to out in order of their index, plus off.
@@ -377,25 +448,26 @@ __device__ __forceinline__ void write_top(const uint32_t* keys, int M, int kk, i
 template <int D, int DT>
 __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const __grid_constant__ SelectArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int LP = D / 8;
+  constexpr int CH = sel_cols<D>() / 8, LP = D / (8 * CH);
   const int S = a.cluster;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / S;
   const int t = unit / a.Hkv, h = unit - t * a.Hkv;
   const int G = a.Hq / a.Hkv;
-  // the group's queries in 64 bits, [head][4][LP] pairs of columns, zeros up
-  // to a whole SEL_HEADS; then page ids; then keys
+  // the group's queries in 64 bits, [head][4 CH][LP] pairs of columns, zeros up
+  // to a whole SEL_HEADS; then the ring; then page ids and keys
   const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
   double2* qd = reinterpret_cast<double2*>(smem);
-  int* ids = reinterpret_cast<int*>(smem + size_t(G4) * D * 8);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(ids + a.share);
+  const uint32_t ring = smem_u32(smem + size_t(G4) * D * 8);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem + size_t(G4) * D * 8 + sel_ring<D>());
+  int* ids = reinterpret_cast<int*>(keys);  // until their scores are known
 
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
   for (int i = threadIdx.x; i < G4 * D / 2; i += SEL_THREADS) {
-    const int g = i / (D / 2), d = i % (D / 2) * 2;  // columns d, d + 1: lane d / 8, pair (d % 8) / 2
+    const int g = i / (D / 2), d = i % (D / 2) * 2;  // columns d, d + 1: chunk, lane and pair
     float2 f = make_float2(0.f, 0.f);
     if (g < G) f = unpack2<DT>(__ldg(reinterpret_cast<const uint32_t*>(q + g * a.q_sh + d)));
-    qd[(g * 4 + (d % 8) / 2) * LP + d / 8] = make_double2(double(f.x), double(f.y));
+    qd[(g * (4 * CH) + d / (8 * LP) * 4 + d % 8 / 2) * LP + d / 8 % LP] = make_double2(double(f.x), double(f.y));
   }
   const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
   int* out = a.out + (long long)unit * a.top;
@@ -426,15 +498,16 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   if (S > 1) cluster_sync();  // and the first block has begun, so that its shared memory may be written
   else __syncthreads();
   const uint32_t keys0 = smem_u32(keys) + 4u * uint32_t(p0);
-  score_pages<D, DT>(a, qd, ids, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
+  score_pages<D, DT>(a, qd, ids, ring, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
   if (S > 1) {
     cluster_sync();
     if (rank != 0) return;
   } else {
     __syncthreads();
   }
-  if (M <= SEL_THREADS) write_top<1>(keys, M, kk, a.sink, out + a.sink);
+  if (M <= SEL_THREADS) write_top_small(keys, M, kk, a.sink, out + a.sink);
   else if (M <= 4 * SEL_THREADS) write_top<4>(keys, M, kk, a.sink, out + a.sink);
+  else if (M <= 8 * SEL_THREADS) write_top<8>(keys, M, kk, a.sink, out + a.sink);
   else if (M <= 16 * SEL_THREADS) write_top<16>(keys, M, kk, a.sink, out + a.sink);
   else write_top<0>(keys, M, kk, a.sink, out + a.sink);
 }
@@ -889,7 +962,7 @@ int run_select(const SelectArgs& a) {
   auto* kernel = fa_select_pages_kernel<D, DT>;
   const int G = a.Hq / a.Hkv;
   const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
-  const size_t smem = size_t(G4) * D * 8 + size_t(a.share) * 4 + size_t(a.width) * 4;
+  const size_t smem = size_t(G4) * D * 8 + sel_ring<D>() + (size_t(a.width) * 4 + 15) / 16 * 16;
   constexpr size_t most = size_t(220) << 10;  // of an SM's 227 KB, the static part left out
   if (smem > most) return FA_ERR_BAD_SHAPE;
   if (int rc = allow_smem<fa_select_pages_kernel<D, DT>>(int(most))) return rc;
@@ -926,7 +999,6 @@ int launch_page_means(const PageArgs& a, int total_q) {
 
 int launch_select_pages(SelectArgs a, int D) {
   a.cluster = cluster_for((long long)a.total_q * a.Hkv, a.width, 64, 2);
-  a.share = (a.width + a.cluster - 1) / a.cluster;
   if (a.dtype == DT_BF16)
     return D == 32 ? run_select<32, DT_BF16>(a) : D == 64 ? run_select<64, DT_BF16>(a) : run_select<128, DT_BF16>(a);
   return D == 32 ? run_select<32, DT_F16>(a) : D == 64 ? run_select<64, DT_F16>(a) : run_select<128, DT_F16>(a);
