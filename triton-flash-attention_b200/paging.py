@@ -26,8 +26,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _abi
-from .rotary import _ptr, check_backend, check_eps, check_table, check_weights, on_device, row_arg
+from .rotary import _ptr, check_backend, check_eps, check_table, check_weights, launch, row_arg
 
 # block-table width that select_pages takes (FA_MAX_SELECT_PAGES of include/fa_b200.h)
 MAX_SELECT_PAGES = 16384
@@ -130,21 +129,17 @@ def extend_block_table(block_table, seqlens_cached, seqlens_new, free_pages, fre
     if dev.type != "cuda":
         raise RuntimeError("B200 CUDA backend is unavailable: the B200 kernel requires a CUDA tensor")
     seqlens_cached, seqlens_new, free_pages = (t.contiguous() for t in (seqlens_cached, seqlens_new, free_pages))
-    with on_device(block_table) as stream:
-        # one allocation for the int32 outputs
-        out = torch.empty(2 * requests + 2 + 2 * total_q, device=dev, dtype=torch.int32)
-        cu, sk, pos, slots, nxt = out.split_with_sizes((requests + 1, requests, total_q, total_q, 1))
-        fits = torch.empty(requests, device=dev, dtype=torch.bool)
-        cu_at = out.data_ptr()
-        sk_at = cu_at + 4 * (requests + 1)
-        pos_at = sk_at + 4 * requests
-        slots_at = pos_at + 4 * total_q
-        rc = _abi.lib().fa_extend_block_table(
-            block_table.data_ptr(), seqlens_cached.data_ptr(), seqlens_new.data_ptr(),
-            free_pages.data_ptr(), free_start.data_ptr(), cu_at, sk_at, pos_at, slots_at,
-            fits.data_ptr(), slots_at + 4 * total_q, requests, width, free_pages.shape[0], page_size, total_q, stream)
-    if rc:
-        _abi.check(rc, "fa_extend_block_table")
+    # one allocation for the int32 outputs
+    out = block_table.new_empty(2 * requests + 2 + 2 * total_q)
+    cu, sk, pos, slots, nxt = out.split_with_sizes((requests + 1, requests, total_q, total_q, 1))
+    fits = torch.empty(requests, device=dev, dtype=torch.bool)
+    cu_at = out.data_ptr()
+    sk_at = cu_at + 4 * (requests + 1)
+    pos_at = sk_at + 4 * requests
+    slots_at = pos_at + 4 * total_q
+    launch(block_table, "fa_extend_block_table", None, block_table.data_ptr(), seqlens_cached.data_ptr(),
+           seqlens_new.data_ptr(), free_pages.data_ptr(), free_start.data_ptr(), cu_at, sk_at, pos_at, slots_at,
+           fits.data_ptr(), slots_at + 4 * total_q, requests, width, free_pages.shape[0], page_size, total_q)
     return PagedStep(cu, sk, pos, slots, fits, nxt)
 
 
@@ -196,15 +191,11 @@ def paged_append(query, key, value, k_cache, v_cache, slot_mapping, table, posit
     slots, pos = slot_mapping.contiguous(), positions.contiguous()
     if query_weight is not None:
         query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
-    with on_device(q) as stream:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        rc = _abi.entry("fa_paged_append", q.dtype)(
-            qp, kp, vp, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), table.data_ptr(),
-            pos.data_ptr(), _ptr(query_weight), _ptr(key_weight), total, hq, hkv, d, pages * page_size, *table.shape,
-            interleaved, query_weight is not None and query_weight.dtype == torch.float32, qs, ks, vs, float(eps),
-            stream)
-    if rc:
-        _abi.check(rc, "fa_paged_append")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    launch(q, "fa_paged_append", q.dtype, qp, kp, vp, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+           slots.data_ptr(), table.data_ptr(), pos.data_ptr(), _ptr(query_weight), _ptr(key_weight), total, hq, hkv, d,
+           pages * page_size, *table.shape, interleaved,
+           query_weight is not None and query_weight.dtype == torch.float32, qs, ks, vs, float(eps))
     return out
 
 
@@ -251,13 +242,8 @@ def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k,
     _check_no_grad(k_cache, page_means)
     check_backend(k_cache)
     table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
-    with on_device(k_cache) as stream:
-        rc = _abi.entry("fa_page_means", k_cache.dtype)(
-            k_cache.data_ptr(), page_means.data_ptr(), table.data_ptr(),
-            cu.data_ptr(), lens.data_ptr(), batch, hkv, d, num_pages,
-            page_size, width, total_q, stream)
-    if rc:
-        _abi.check(rc, "fa_page_means")
+    launch(k_cache, "fa_page_means", k_cache.dtype, k_cache.data_ptr(), page_means.data_ptr(), table.data_ptr(),
+           cu.data_ptr(), lens.data_ptr(), batch, hkv, d, num_pages, page_size, width, total_q)
     return page_means
 
 
@@ -313,15 +299,10 @@ def select_pages(query, page_means, block_table, cu_seqlens_q, seqlens_k, *, pag
     check_backend(query)
     q, qp, qs = row_arg(query)
     table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
-    with on_device(q) as stream:
-        out = torch.empty((total, hkv, num_selected), device=q.device, dtype=torch.int32)
-        rc = _abi.entry("fa_select_pages", q.dtype)(
-            qp, page_means.data_ptr(), table.data_ptr(),
-            cu.data_ptr(), lens.data_ptr(), out.data_ptr(), batch, hq, hkv,
-            d, total, page_means.shape[0], page_size, width, num_selected, sink_pages, local_pages, qs,
-            stream)
-    if rc:
-        _abi.check(rc, "fa_select_pages")
+    out = block_table.new_empty((total, hkv, num_selected))
+    launch(q, "fa_select_pages", q.dtype, qp, page_means.data_ptr(), table.data_ptr(), cu.data_ptr(), lens.data_ptr(),
+           out.data_ptr(), batch, hq, hkv, d, total, page_means.shape[0], page_size, width, num_selected, sink_pages,
+           local_pages, qs)
     return out
 
 
@@ -371,14 +352,8 @@ def scaled_dot_product_attention_paged_sparse(query, k_cache, v_cache, block_tab
     q, qp, qs = row_arg(query)
     table, cu, lens = block_table.contiguous(), cu_seqlens_q.contiguous(), seqlens_k.contiguous()
     pages = page_indices.contiguous()
-    with on_device(q) as stream:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        rc = _abi.entry("fa_fwd_paged_sparse", q.dtype)(
-            qp, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-            table.data_ptr(), cu.data_ptr(),
-            lens.data_ptr(), pages.data_ptr(), batch, hq, hkv, d, total,
-            num_pages, page_size, width, n, float(scale) if scale is not None else d ** -0.5, qs,
-            stream)
-    if rc:
-        _abi.check(rc, "fa_fwd_paged_sparse")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    launch(q, "fa_fwd_paged_sparse", q.dtype, qp, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+           table.data_ptr(), cu.data_ptr(), lens.data_ptr(), pages.data_ptr(), batch, hq, hkv, d, total, num_pages,
+           page_size, width, n, float(scale) if scale is not None else d ** -0.5, qs)
     return out

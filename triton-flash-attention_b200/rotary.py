@@ -63,27 +63,20 @@ def check_backend(tensor: torch.Tensor) -> None:
         raise RuntimeError("B200 CUDA backend is unavailable: the kernels are built for sm_100a (B200) GPUs only")
 
 
-class on_device:
-    """Context in which launches go to the tensor's device; its value is the
-    device's current stream.  Calls of a few microseconds of GPU time are
-    bound by their host side, so this does nothing where the device is current
-    already."""
-
-    __slots__ = ("index", "previous")
-
-    def __init__(self, tensor: torch.Tensor):
-        self.index = tensor.get_device()
-
-    def __enter__(self) -> int:
-        current = torch.cuda.current_device()
-        self.previous = current if current != self.index else None
-        if self.previous is not None:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.previous is not None:
-            torch.cuda.set_device(self.previous)
+def launch(tensor: torch.Tensor, what: str, dtype, *args) -> None:
+    """Calls the entry ``what`` for operands of ``dtype`` (None: the entry has
+    no type) with ``args`` and the tensor's device's current stream, on that
+    device.  (Calls of a few microseconds of GPU time are bound by their host
+    side: this asks for no more than it has to.)"""
+    fn = _abi.entry(what, dtype)
+    index = tensor.get_device()
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _abi.check(rc, what)
 
 
 _UNSEEN = object()
@@ -118,11 +111,12 @@ def row_arg(t: torch.Tensor):
 def check_table(table, rotary_max: int, device) -> None:
     if not isinstance(table, torch.Tensor):
         raise TypeError("table must be a torch.Tensor")
-    if table.ndim != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.shape[0] == 0:
+    shape = table.shape
+    if len(shape) != 2 or table.dtype != torch.float32 or not table.is_contiguous() or shape[0] == 0:
         raise ValueError("table must be a contiguous (max_positions, rotary_dim) float32 tensor")
-    if table.shape[1] == 0 or table.shape[1] % 16 or table.shape[1] > rotary_max:
-        raise ValueError(f"the table's rotary_dim must be a multiple of 16 up to the head dim {rotary_max}; "
-                         f"got {table.shape[1]}")
+    rd = shape[1]
+    if rd == 0 or rd % 16 or rd > rotary_max:
+        raise ValueError(f"the table's rotary_dim must be a multiple of 16 up to the head dim {rotary_max}; got {rd}")
     if table.device != device:
         raise ValueError("table must be on the same device as query")
     if table.data_ptr() % 16:
@@ -134,18 +128,22 @@ def check_weights(query_weight, key_weight, query) -> None:
         raise ValueError("pass both query_weight and key_weight, or neither for the rotation alone")
     if query_weight is None:
         return
+    d, device = query.shape[-1], query.device
     for name, w in (("query_weight", query_weight), ("key_weight", key_weight)):
         if not isinstance(w, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor")
-        if w.ndim != 1 or w.shape[0] != query.shape[-1] or w.device != query.device:
+        if w.shape != (d,) or w.device != device:
             raise ValueError(f"{name} must be a 1-D tensor of head_dim weights on the query's device")
-        if w.dtype not in (query.dtype, torch.float32):
-            raise ValueError(f"{name} must have the query's dtype or float32")
-    if query_weight.dtype != key_weight.dtype:
+    dtype = query_weight.dtype
+    if dtype != torch.float32 and dtype != query.dtype:
+        raise ValueError("query_weight and key_weight must have the query's dtype or float32")
+    if dtype != key_weight.dtype:
         raise ValueError("query_weight and key_weight must have the same dtype")
 
 
 def check_eps(eps) -> None:
+    if type(eps) is float and 0.0 <= eps < math.inf:
+        return
     if isinstance(eps, bool) or not isinstance(eps, Real) or not 0.0 <= eps < math.inf:
         raise ValueError("eps must be a finite non-negative number")
 
@@ -205,6 +203,12 @@ def _sizes(q, k):
     return 1, s[1], k.shape[1], s[0], s[2]
 
 
+def _contiguous_strides(shape):
+    """Strides of an output of that shape: contiguous."""
+    *_, h, n, d = shape
+    return _strides_arg((h * n * d, n * d, d, 1) if len(shape) == 4 else (n * d, d, 1))
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -222,15 +226,11 @@ def _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved)
     max_positions, rd = table.shape
     fp32 = query_weight is not None and query_weight.dtype == torch.float32
     per_batch = n if positions is not None and positions.ndim == 2 else 0
-    with on_device(q) as stream:
-        qo, ko = _contiguous_like(q), _contiguous_like(k)
-        _, qop, qos = row_arg(qo)
-        _, kop, kos = row_arg(ko)
-        rc = _abi.entry("fa_qk_norm_rotary", q.dtype)(
-            qp, kp, qop, kop, table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight), b, hq, hkv, n,
-            d, max_positions, rd, interleaved, fp32, qs, ks, qos, kos, per_batch, eps, stream)
-    if rc:
-        _abi.check(rc, "fa_qk_norm_rotary")
+    qo, ko = _contiguous_like(q), _contiguous_like(k)
+    _, qop, qos = row_arg(qo)
+    _, kop, kos = row_arg(ko)
+    launch(q, "fa_qk_norm_rotary", q.dtype, qp, kp, qop, kop, table.data_ptr(), _ptr(positions), _ptr(query_weight),
+           _ptr(key_weight), b, hq, hkv, n, d, max_positions, rd, interleaved, fp32, qs, ks, qos, kos, per_batch, eps)
     return qo, ko, q, k, (b, hq, hkv, n, d, max_positions, rd, interleaved, fp32), (qs, ks, qos, kos, per_batch, eps)
 
 
@@ -241,18 +241,14 @@ def _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, 
     grad_q, gqp, gqs = row_arg(grad_q)
     grad_k, gkp, gks = row_arg(grad_k)
     qs, ks, qos, kos, per_batch, eps = rest
-    with on_device(q) as stream:
-        dq, dk = _contiguous_like(q), _contiguous_like(k)
-        dwq = dwk = part = None
-        if weight_grads:
-            dwq, dwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
-            part = torch.empty(ROTARY_PARTIALS * sizes[4], device=q.device, dtype=torch.float32)
-        rc = _abi.entry("fa_qk_norm_rotary_bwd", q.dtype)(
-            q.data_ptr(), k.data_ptr(), gqp, gkp, dq.data_ptr(), dk.data_ptr(), _ptr(dwq), _ptr(dwk), _ptr(part),
-            table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight), *sizes, qs, ks, gqs, gks, qos,
-            kos, per_batch, eps, stream)
-    if rc:
-        _abi.check(rc, "fa_qk_norm_rotary_bwd")
+    dq, dk = _contiguous_like(q), _contiguous_like(k)
+    dwq = dwk = part = None
+    if weight_grads:
+        dwq, dwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
+        part = table.new_empty(ROTARY_PARTIALS * sizes[4])
+    launch(q, "fa_qk_norm_rotary_bwd", q.dtype, q.data_ptr(), k.data_ptr(), gqp, gkp, dq.data_ptr(), dk.data_ptr(),
+           _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight),
+           *sizes, qs, ks, gqs, gks, qos, kos, per_batch, eps)
     return dq, dk, dwq, dwk
 
 
@@ -267,8 +263,7 @@ def qk_norm_rotary_backward(q, k, grad_q, grad_k, table, positions, query_weight
     (else None).  Gradients repeat bit for bit."""
     q, _, qs = row_arg(q)
     k, _, ks = row_arg(k)
-    # the gradients of q and k are contiguous, in the layout of the outputs
-    qos, kos = (_strides_arg(torch.empty(t.shape, device="meta").stride()) for t in (q, k))
+    qos, kos = _contiguous_strides(q.shape), _contiguous_strides(k.shape)
     sizes = (*_sizes(q, k), *table.shape, interleaved,
              query_weight is not None and query_weight.dtype == torch.float32)
     per_batch = sizes[3] if positions is not None and positions.ndim == 2 else 0
