@@ -614,10 +614,10 @@ def select_pages_reference(q, means, block_table, cu, seqlens_k, page_size: int,
             else:
                 g = q[t, h * (hq // hkv):(h + 1) * (hq // hkv)]
                 s = (means[block_table[b, :n], h] @ g.T).max(1).astype(np.float32)
-                s = np.where(np.isnan(s), -np.inf, s)
-                s[:sink] = np.inf
-                s[n - local:] = np.inf
-                keep = np.sort(np.argsort(-s, kind="stable")[:top])
+                rank = np.where(np.isnan(s), 0, 1)  # NaN is lowest, then -inf
+                rank[:sink] = rank[n - local:] = 2  # kept whatever their score
+                best = np.where(np.isnan(s), 0.0, s)
+                keep = np.sort(np.lexsort((np.arange(n), -best, -rank))[:top])
             out[t, h, :len(keep)] = keep
     return out
 

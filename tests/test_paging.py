@@ -387,6 +387,56 @@ def test_selection_ties_nan_and_infinite_scores():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,d,dt,group", [(120, 128, BF16, 2), (700, 64, F16, 1), (2500, 128, F16, 3), (5000, 32, BF16, 6)])
+def test_selection_where_fp32_sums_do_not_decide(n, d, dt, group):
+    """Large terms that cancel: the scores differ by far less than the
+    roundings of an fp32 sum, and the pages are those of the 64-bit ones."""
+    page = 16
+    c = Case([1], [page * n - 3], page, group, 1, d, dt, n, junk=0.0)
+    q, kc, _, table, cu, lens = c.cuda()
+    g = torch.Generator().manual_seed(n)
+    half = d // 2
+    q[:, :, :half] = 900.0 + torch.randint(0, 8, (1, group, half), generator=g).to(q)
+    q[:, :, half:] = -q[:, :, :half]
+    k = _randn(g, n, half)
+    k = torch.cat([k, k + 2.0 ** -7 * torch.randint(-1, 2, (n, half), generator=g)], 1).to(dt)
+    means = torch.zeros(kc.shape[0], 1, d, dtype=dt, device="cuda")
+    means[torch.from_numpy(c.table[0].astype(np.int64)).cuda(), 0] = k.cuda()
+    for top in (3, n // 4, n // 2, n - 1):
+        got = fa.select_pages(q, means, table, cu, lens, page_size=page, num_selected=top)
+        want = orc.select_pages_reference(_f64(q), _f64(means), c.table, c.cu, c.lens, page, top, 1, 1)
+        assert np.array_equal(got.cpu().numpy(), want), top
+    # all scores equal: the first pages
+    means[:] = means[0]
+    got = fa.select_pages(q, means, table, cu, lens, page_size=page, num_selected=n // 2)
+    assert got[0, 0].tolist() == [*range(n // 2 - 1), n - 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["huge", "tiny", "zero", "nan", "inf"])
+def test_selection_with_queries_and_means_at_the_edges(what):
+    page, n = 16, 900
+    c = Case([1], [page * n - 3], page, 2, 1, 64, BF16, 5, junk=0.0)
+    q, kc, _, table, cu, lens = c.cuda()
+    g = torch.Generator().manual_seed(6)
+    means = _randn(g, kc.shape[0], 1, 64, dtype=BF16).cuda()
+    if what == "huge":  # squares and products past the fp32 range, with both signs
+        q, means = q * 2.0 ** 90, means * 2.0 ** 60
+    elif what == "tiny":  # products below it
+        q, means = q * 2.0 ** -90, means * 2.0 ** -60
+    elif what == "zero":
+        means[:] = 0
+    elif what == "nan":
+        q[0, 1, 3] = float("nan")
+    else:
+        q[0, 0, 3] = float("inf")
+    got = fa.select_pages(q, means, table, cu, lens, page_size=page, num_selected=100)
+    with np.errstate(all="ignore"):
+        want = orc.select_pages_reference(_f64(q), _f64(means), c.table, c.cu, c.lens, page, 100, 1, 1)
+    assert np.array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
 def test_selection_over_the_widest_table():
     n = 16384
     c = Case([1], [16 * n], 16, 2, 1, 32, F16, 4, junk=0.0)

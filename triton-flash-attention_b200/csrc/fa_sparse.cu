@@ -9,10 +9,11 @@
 //    pages that the token may see.
 //
 // Means and scores decide which pages are kept, and two pages' scores may be
-// as near as their roundings, so both are summed in 64 bits and rounded once
+// as near as their roundings, so both are defined by 64-bit sums, rounded once
 // to what they are kept in (means: to fp32 and then the cache's type; scores:
 // to fp32).  The kept pages then depend on the inputs alone, not on the order
-// of a sum.
+// of a sum.  (Scores are summed in fp32 first, and in 64 bits where that could
+// change which pages are kept.)
 #include <atomic>
 
 #include "fa_kernels.h"
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
 
 // ---------------------------------------------------------------------------
 // Cluster helpers: `S` blocks of one launch cluster share a unit's work.
+constexpr int MAX_CLUSTER = 8;
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -197,20 +199,24 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
 //
 // Scoring: a few lanes own a page, 16 columns a lane (8 of D = 32), SEL_PAGES
 // pages at once; asynchronous copies to the lane's own places in shared memory
-// bring the next batch meanwhile.  The group's queries lie in shared memory in
-// 64 bits and are taken SEL_HEADS heads at a time.  Lanes swap halves of
-// their page sums until each holds whole ones; more columns a lane leave fewer
-// of these exchanges.
-// Bound: for a group of 4 heads the 64-bit products (64 a clock and SM) and
-// the conversions of the means (16) take about as long as the means' bytes;
-// for larger groups the products take longer.
+// bring the next batch meanwhile.  The group's queries lie in shared memory
+// and are taken SEL_HEADS heads at a time.  Lanes swap halves of their page
+// sums until each holds whole ones.  The sums are fp32, of exact products: 16
+// roundings in a lane and up to 3 between lanes, each at most 2^-24 of the
+// sum of sizes |q| . |k| <= ||q||_1 max |k|.
 //
-// Selection: keys are the scores' bits in an order that whole numbers have.
-// Up to a key a thread, every thread counts the keys that go before its own.
-// For more, neighbouring keys a thread, the kk-th largest key is found two
-// bits a round, by block-wide counts of the keys at and above three
-// candidates; the pages above it, and of the pages at it the first ones, are
+// Selection: keys are the scores' bits in an order that whole numbers have,
+// neighbouring keys a thread.  T, the kk-th largest, is found two bits a
+// round by block-wide counts of the keys at and above three candidates, and
+// once few keys can still be it, by counting those that go before each of
+// them.  If more than one key lies so near T that its score's roundings may
+// decide, the pages of all such keys are scored again in 64 bits, and T is
+// found again.  The pages above T, and of those at T the first ones, are
 // written in order of their index.
+//
+// Bound: the means' bytes and the start; 64-bit sums throughout (64 products a
+// clock and SM, 16 conversions) took 23 us for 64 units of 2,048 pages where
+// this takes SELECT_US.
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
 constexpr int SEL_PAGES = 4;
@@ -229,13 +235,16 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float key_score(uint32_t k) {  // of a key that is not 0
+  return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
 
-// Scores of the block's pn pages, as keys to keys_at.  ids holds their pages
-// and may be where the keys go: a page's key replaces its id, which is read by
-// then.
+// fp32 scores of the block's pn pages, as keys to keys_at.  ids holds their
+// pages and may be where the keys go: a page's key replaces its id, which is
+// read by then.  Returns the largest |k| of the pages this thread has seen.
 template <int D, int DT>
-__device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* qd, const int* ids, uint32_t ring,
-                                            int h, int G, int pn, uint32_t keys_at) {
+__device__ __forceinline__ float score_pages(const SelectArgs& a, const float4* qf, const int* ids, uint32_t ring,
+                                             int h, int G, int pn, uint32_t keys_at) {
   constexpr int CH = sel_cols<D>() / 8;  // 16-byte chunks of a lane
   constexpr int LP = D / (8 * CH);       // lanes of a page
   constexpr int SUBS = SEL_THREADS / LP;
@@ -263,6 +272,7 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* 
   int first = (threadIdx.x / LP) * SEL_PAGES;
   fetch(first, mine_at);
   uint32_t stage = 0;
+  float top = 0.f;
   // the trip count is the warp's, for the shuffles
   for (int base = (threadIdx.x - lane) / LP * SEL_PAGES; base < pn; base += BATCH, first += BATCH) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -272,174 +282,288 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, const double2* 
     float best = -INFINITY;
     bool nan = false;
     for (int g0 = 0; g0 < G; g0 += SEL_HEADS) {
-      double s[SEL_HEADS][SEL_PAGES];
+      float s[SEL_HEADS][SEL_PAGES], size[SEL_PAGES];
 #pragma unroll
-      for (int g = 0; g < SEL_HEADS; ++g)
+      for (int i = 0; i < SEL_PAGES; ++i) {
+        size[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = 0.0;
+        for (int g = 0; g < SEL_HEADS; ++g) s[g][i] = 0.f;
+      }
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        uint32_t w[SEL_PAGES][4];  // what no page was copied to gives a sum that nobody looks at
+        float k[SEL_PAGES][8];  // what no page was copied to gives a sum that nobody looks at
 #pragma unroll
-        for (int i = 0; i < SEL_PAGES; ++i)
+        for (int i = 0; i < SEL_PAGES; ++i) {
+          uint32_t w[4];
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                        : "r"(from + (i * CH + c) * PIECE)
                        : "memory");
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          double lo[SEL_PAGES], hi[SEL_PAGES];
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack2<DT>(w[j]);
+            k[i][2 * j] = f.x;
+            k[i][2 * j + 1] = f.y;
+            size[i] = fmax3(size[i], fabsf(f.x), fabsf(f.y));
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < SEL_HEADS; ++g) {
+          const float4 lo = qf[((g0 + g) * (2 * CH) + c * 2) * LP + l];
+          const float4 hi = qf[((g0 + g) * (2 * CH) + c * 2 + 1) * LP + l];
 #pragma unroll
           for (int i = 0; i < SEL_PAGES; ++i) {
-            const float2 f = unpack2<DT>(w[i][j]);
-            lo[i] = double(f.x);
-            hi[i] = double(f.y);
-          }
-#pragma unroll
-          for (int g = 0; g < SEL_HEADS; ++g) {
-            const double2 x = qd[((g0 + g) * (4 * CH) + c * 4 + j) * LP + l];
-#pragma unroll
-            for (int i = 0; i < SEL_PAGES; ++i) s[g][i] = fma(x.y, hi[i], fma(x.x, lo[i], s[g][i]));
+            float t = s[g][i];
+            t = fmaf(lo.x, k[i][0], t), t = fmaf(lo.y, k[i][1], t);
+            t = fmaf(lo.z, k[i][2], t), t = fmaf(lo.w, k[i][3], t);
+            t = fmaf(hi.x, k[i][4], t), t = fmaf(hi.y, k[i][5], t);
+            t = fmaf(hi.z, k[i][6], t), t = fmaf(hi.w, k[i][7], t);
+            s[g][i] = t;
           }
         }
       }
+      // 4 page sums over LP lanes: keep 2, then 1, then add it up
+      const bool up0 = (l & (LP / 2)) != 0, up1 = (l & (LP / 4)) != 0;
 #pragma unroll
       for (int g = 0; g < SEL_HEADS; ++g) {
         if (g0 + g >= G) break;  // uniform
-        // 4 page sums over LP lanes: keep 2, then 1, then add it up
-        const bool up0 = (l & (LP / 2)) != 0;
-        double e0 = up0 ? s[g][2] : s[g][0], e1 = up0 ? s[g][3] : s[g][1];
+        float e0 = up0 ? s[g][2] : s[g][0], e1 = up0 ? s[g][3] : s[g][1];
         e0 += __shfl_xor_sync(0xffffffffu, up0 ? s[g][0] : s[g][2], LP / 2);
         e1 += __shfl_xor_sync(0xffffffffu, up0 ? s[g][1] : s[g][3], LP / 2);
-        const bool up1 = (l & (LP / 4)) != 0;
-        double e = up1 ? e1 : e0;
+        float e = up1 ? e1 : e0;
         e += __shfl_xor_sync(0xffffffffu, up1 ? e0 : e1, LP / 4);
 #pragma unroll
         for (int m = LP / 8; m > 0; m >>= 1) e += __shfl_xor_sync(0xffffffffu, e, m);
-        const float f = __double2float_rn(e);
-        nan |= f != f;
-        best = fmaxf(best, f);
+        nan |= e != e;
+        best = fmaxf(best, e);
       }
+      if (g0 == 0)
+#pragma unroll
+        for (int i = 0; i < SEL_PAGES; ++i)
+          if (first + i < pn && ids[first + i] >= 0) top = fmaxf(top, size[i]);
     }
+    __syncwarp();  // the batch's ids are read
     // this lane's page of the four
     const int mine = first + ((l & (LP / 2)) ? 2 : 0) + ((l & (LP / 4)) ? 1 : 0);
     if ((l & (LP / 4 - 1)) == 0 && mine < pn)
       st_cluster_u32(keys_at + 4u * uint32_t(mine), ids[mine] < 0 || nan ? 0u : order_key(best));
   }
+  return top;
 }
 
-// Writes the kk largest of M <= SEL_THREADS keys, a key a thread.
-__device__ __forceinline__ void write_top_small(uint32_t* keys, int M, int kk, int off, int* out) {
-  __shared__ int counts[SEL_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x;
-  const uint32_t mine = me < M ? keys[me] : 0u;
-  if (me >= M && me < (M + 3) / 4 * 4) keys[me] = 0u;
-  __syncthreads();
-  const int w0 = warp * 32, padded = (M + 3) / 4 * 4;  // the keys behind M are 0: behind all that count
-  int before = 0;                                      // keys that go before this one
-  if (w0 < M) {
-    // of equal keys those of lower index go before: all of the warps before, none of those behind
-#pragma unroll 4
-    for (int i = 0; i < w0; i += 4) {
-      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
-      before += (k.x >= mine) + (k.y >= mine) + (k.z >= mine) + (k.w >= mine);
-    }
-#pragma unroll 4
-    for (int i = w0 + 32; i < padded; i += 4) {
-      const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
-      before += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
-    }
+// The score of page `id` by its definition: 64-bit sums, rounded to fp32.  One
+// warp; a lane's D / 32 neighbouring columns against the queries in shared
+// memory, which hold the operands exactly.
+template <int D, int DT>
+__device__ __forceinline__ uint32_t exact_key(const SelectArgs& a, const float4* qf, int h, int G, int id) {
+  constexpr int CH = sel_cols<D>() / 8, LP = D / (8 * CH);
+  constexpr int N = D / 32;
+  const int d0 = (threadIdx.x & 31) * N;
+  const uint16_t* k = static_cast<const uint16_t*>(a.means) + ((long long)id * a.Hkv + h) * D + d0;
+  double kd[N];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const uint32_t k = __shfl_sync(0xffffffffu, mine, j);
-      before += k > mine || (k == mine && j < lane);
-    }
+  for (int i = 0; i < N; ++i) kd[i] = double(to_f32<DT>(__ldg(k + i)));
+  // where columns d0 .. d0 + N - 1 of head 0 lie in qf (N divides 4)
+  const float* q = reinterpret_cast<const float*>(qf + (d0 / (8 * LP) * 2 + d0 / 4 % 2) * LP + d0 / 8 % LP) + d0 % 4;
+  float best = -INFINITY;
+  bool nan = false;
+#pragma unroll 4
+  for (int g = 0; g < G; ++g) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s = fma(double(q[g * D + i]), kd[i], s);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+    const float f = __double2float_rn(s);
+    nan |= f != f;
+    best = fmaxf(best, f);
   }
-  const bool kept = me < M && before < kk;
-  const uint32_t votes = __ballot_sync(0xffffffffu, kept);
-  if (lane == 0) counts[warp] = __popc(votes);
-  __syncthreads();
-  int at = __popc(votes & ((1u << lane) - 1u));
-#pragma unroll
-  for (int w = 0; w < SEL_WARPS; ++w) at += w < warp ? counts[w] : 0;
-  if (kept) out[at] = off + me;
+  return nan ? 0u : order_key(best);
 }
 
-// The kk largest of the M keys, to out in order of their index, plus off.
-// E: keys a thread, held in registers; 0: read again from shared memory.
+// Shared memory of the selection.
+struct SelectShared {
+  uint2 counts[2][SEL_WARPS];
+  uint32_t list[SEL_THREADS];
+  int pages[SEL_THREADS];
+  uint32_t found;
+  int listed;
+};
+
+// The rank-th largest (from 1) of n <= SEL_THREADS values; v has zeros up to a
+// multiple of 4.  All threads; ends with a barrier.
+__device__ __forceinline__ uint32_t ranked(SelectShared& sh, const uint32_t* v, int n, int rank) {
+  const int me = threadIdx.x;
+  if ((me & ~31) < n) {
+    const uint32_t mine = me < n ? v[me] : 0u;
+    int above = 0, from = 0;  // values > mine, >= mine
+#pragma unroll 4
+    for (int i = 0; i < n; i += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(v + i);
+      above += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+      from += (k.x >= mine) + (k.y >= mine) + (k.z >= mine) + (k.w >= mine);
+    }
+    if (me < n && above < rank && rank <= from) sh.found = mine;
+  }
+  __syncthreads();
+  return sh.found;
+}
+
+// A thread's neighbouring keys: E of them in registers, or (E = 0) read again
+// from shared memory.
 template <int E>
-__device__ __forceinline__ void write_top(const uint32_t* keys, int M, int kk, int off, int* out) {
-  __shared__ uint2 counts[2][SEL_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = E > 0 ? E : (M + SEL_THREADS - 1) / SEL_THREADS;
-  const int k0 = min(M, int(threadIdx.x) * each), k1 = min(M, k0 + each);
-  uint32_t mine[E > 0 ? E : 1];
-  if constexpr (E > 0) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) mine[i] = k0 + i < k1 ? keys[k0 + i] : 0u;
-  }
-  uint32_t T = 0;  // the kk-th largest key
-#pragma unroll 1
-  for (int bit = 30; bit >= 0; bit -= 2) {
-    const uint32_t t1 = T | (1u << bit), t2 = T | (2u << bit), t3 = T | (3u << bit);
-    // counts of keys >= t1, t2 and t3; M is below 2^16
-    uint32_t c12 = 0, c3 = 0;
+struct Held {
+  const uint32_t* keys;
+  int k0, k1;
+  uint32_t v[E > 0 ? E : 1];
+  __device__ __forceinline__ Held(const uint32_t* all, int M) : keys(all) {
+    const int each = E > 0 ? E : (M + SEL_THREADS - 1) / SEL_THREADS;
+    k0 = min(M, int(threadIdx.x) * each);
+    k1 = min(M, k0 + each);
     if constexpr (E > 0) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) c12 += (mine[i] >= t1) + ((mine[i] >= t2) << 16), c3 += mine[i] >= t3;
-    } else {
-      for (int i = k0; i < k1; ++i) {
-        const uint32_t k = keys[i];
-        c12 += (k >= t1) + ((k >= t2) << 16), c3 += k >= t3;
-      }
+      for (int i = 0; i < E; ++i) v[i] = k0 + i < k1 ? keys[k0 + i] : 0u;
     }
-    c12 = __reduce_add_sync(0xffffffffu, c12);
-    c3 = __reduce_add_sync(0xffffffffu, c3);
-    uint2* slot = counts[(bit >> 1) & 1];
-    if (lane == 0) slot[warp] = make_uint2(c12, c3);
-    __syncthreads();
-    c12 = c3 = 0;
-#pragma unroll
-    for (int w = 0; w < SEL_WARPS; ++w) c12 += slot[w].x, c3 += slot[w].y;
-    const uint32_t want = uint32_t(kk);
-    T = c3 >= want ? t3 : (c12 >> 16) >= want ? t2 : (c12 & 0xffffu) >= want ? t1 : T;
   }
-  // a thread's keys above and at T (padding never counts: it lies behind k1)
-  int gt = 0, eq = 0;
-  auto key_at = [&](int i) {
-    if constexpr (E > 0) return mine[i];
-    else return keys[k0 + i];
-  };
-  auto each_key = [&](auto f) {
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {  // f(index, key)
     if constexpr (E > 0) {
 #pragma unroll
       for (int i = 0; i < E; ++i)
-        if (k0 + i < k1) f(i);
+        if (k0 + i < k1) f(k0 + i, v[i]);
     } else {
-      for (int i = 0; k0 + i < k1; ++i) f(i);
+      for (int i = k0; i < k1; ++i) f(i, keys[i]);
     }
-  };
-  each_key([&](int i) { gt += key_at(i) > T, eq += key_at(i) == T; });
-  uint32_t both = uint32_t(gt) | (uint32_t(eq) << 16), sum = both;
+  }
+};
+// Block-wide sums of two counts below 2^16 each a thread; one barrier.
+__device__ __forceinline__ uint2 block_counts(SelectShared& sh, int turn, uint32_t x, uint32_t y) {
+  x = __reduce_add_sync(0xffffffffu, x);
+  y = __reduce_add_sync(0xffffffffu, y);
+  uint2* slot = sh.counts[turn & 1];
+  if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = make_uint2(x, y);
+  __syncthreads();
+  x = y = 0;
+#pragma unroll
+  for (int w = 0; w < SEL_WARPS; ++w) x += slot[w].x, y += slot[w].y;
+  return make_uint2(x, y);
+}
+
+// The kk-th largest of the M keys (below 2^16 of them).
+template <int E>
+__device__ __forceinline__ uint32_t kth_largest(SelectShared& sh, const Held<E>& held, int M, int kk) {
+  uint32_t T = 0;
+  int above = 0, active = M;  // keys above T's range, keys in it
+#pragma unroll 1
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    if (bit <= 20 && active <= SEL_THREADS) {  // few keys agree with T so far
+      const uint32_t low = bit + 1 >= 31 ? 0xffffffffu : (4u << bit) - 1u;
+      if (threadIdx.x == 0) sh.listed = 0;
+      sh.list[threadIdx.x] = 0u;
+      __syncthreads();
+      held.each([&](int, uint32_t k) {
+        if ((k & ~low) == T) sh.list[atomicAdd(&sh.listed, 1)] = k;
+      });
+      __syncthreads();
+      return ranked(sh, sh.list, active, kk - above);
+    }
+    const uint32_t t1 = T | (1u << bit), t2 = T | (2u << bit), t3 = T | (3u << bit);
+    uint32_t c12 = 0, c3 = 0;
+    held.each([&](int, uint32_t k) { c12 += (k >= t1) + ((k >= t2) << 16), c3 += k >= t3; });
+    const uint2 c = block_counts(sh, bit >> 1, c12, c3);
+    const int c1 = int(c.x & 0xffffu), c2 = int(c.x >> 16), n3 = int(c.y);
+    // the range that T is in, the keys above it and from it on
+    if (n3 >= kk) T = t3, active = n3 - above;
+    else if (c2 >= kk) T = t2, active = c2 - n3, above = n3;
+    else if (c1 >= kk) T = t1, active = c1 - c2, above = c2;
+    else active -= c1 - above, above = c1;
+  }
+  return T;
+}
+
+// Writes the kk largest of the M keys, to out in order of their index, plus
+// off.  slack: how far an fp32 score may be from the one by definition; where
+// that leaves a choice, rescore(page, key) gives the key by definition.
+template <int E, class Rescore>
+__device__ __forceinline__ void write_top(SelectShared& sh, uint32_t* keys, int M, int kk, int off, int* out,
+                                          float slack, Rescore rescore) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Held<E> held(keys, M);
+  uint32_t T = E == 1 ? ranked(sh, keys, M, kk) : kth_largest(sh, held, M, kk);
+  // keys whose scores by definition may lie on either side of the kk-th
+  uint32_t lo = 0u, hi = 0xffffffffu;
+  bool all_open = !(slack < INFINITY);  // infinities or NaN: any key
+  if (!all_open && slack > 0.f && T != 0u) {
+    lo = order_key(__fsub_rd(key_score(T), 2.f * slack));
+    hi = order_key(__fadd_ru(key_score(T), 2.f * slack));
+    uint32_t near = 0, over = 0;
+    held.each([&](int, uint32_t k) { near += k >= lo && k <= hi, over += k > hi; });
+    const uint2 c = block_counts(sh, 1, near, over);
+    const int n = int(c.x), want = kk - int(c.y);  // pages near T, and how many of them are kept
+    all_open = n > SEL_THREADS;
+    if (n > 1 && !all_open) {
+      if (threadIdx.x == 0) sh.listed = 0;
+      __syncthreads();
+      held.each([&](int i, uint32_t k) {
+        if (k >= lo && k <= hi) sh.pages[atomicAdd(&sh.listed, 1)] = i;
+      });
+      __syncthreads();
+      for (int i = warp; i < n; i += SEL_WARPS) {
+        const uint32_t key = rescore(sh.pages[i]);
+        if (lane == 0) sh.list[i] = key;
+      }
+      __syncthreads();
+      if (int(threadIdx.x) < n) {
+        const uint32_t mine = sh.list[threadIdx.x];
+        const int page = sh.pages[threadIdx.x];
+        int before = 0;
+        for (int i = 0; i < n; ++i) before += sh.list[i] > mine || (sh.list[i] == mine && sh.pages[i] < page);
+        keys[page] = before < want ? 0xffffffffu : 0u;  // kept: above every other, or not: below
+      }
+      __syncthreads();
+      held = Held<E>(keys, M);
+      T = hi;
+    }
+  }
+  if (all_open) {  // uniform
+    __syncthreads();
+    for (int p0 = warp * 32; p0 < M; p0 += SEL_THREADS) {
+      const uint32_t k = p0 + lane < M ? keys[p0 + lane] : 0u;
+      uint32_t todo = __ballot_sync(0xffffffffu, p0 + lane < M && k >= lo && k <= hi);
+      while (todo) {
+        const int j = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const uint32_t key = rescore(p0 + j);
+        if (lane == 0) keys[p0 + j] = key;
+      }
+    }
+    __syncthreads();
+    held = Held<E>(keys, M);
+    T = E == 1 ? ranked(sh, keys, M, kk) : kth_largest(sh, held, M, kk);
+  }
+  int gt = 0, eq = 0;
+  held.each([&](int, uint32_t k) { gt += k > T, eq += k == T; });
+  const uint32_t both = uint32_t(gt) | (uint32_t(eq) << 16);
+  uint32_t sum = both;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
     const uint32_t x = __shfl_up_sync(0xffffffffu, sum, m);
     if (lane >= m) sum += x;
   }
   __syncthreads();
-  if (lane == 31) counts[0][warp].x = sum;
+  if (lane == 31) sh.counts[0][warp].x = sum;
   __syncthreads();
   uint32_t before = sum - both, all = 0;
 #pragma unroll
   for (int w = 0; w < SEL_WARPS; ++w) {
-    if (w < warp) before += counts[0][w].x;
-    all += counts[0][w].x;
+    const uint32_t x = sh.counts[0][w].x;
+    before += w < warp ? x : 0u;
+    all += x;
   }
   int gs = int(before & 0xffffu), es = int(before >> 16);
   const int want_eq = kk - int(all & 0xffffu);
-  each_key([&](int i) {
-    const uint32_t key = key_at(i);
-    if (key > T || (key == T && es < want_eq)) out[gs + min(es, want_eq)] = off + k0 + i;
+  held.each([&](int i, uint32_t key) {
+    if (key > T || (key == T && es < want_eq)) out[gs + min(es, want_eq)] = off + i;
     gs += key > T;
     es += key == T;
   });
@@ -448,26 +572,34 @@ __device__ __forceinline__ void write_top(const uint32_t* keys, int M, int kk, i
 template <int D, int DT>
 __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const __grid_constant__ SelectArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ SelectShared sh;
+  __shared__ uint32_t q_size, k_size, k_sizes[MAX_CLUSTER];  // ||q||_1; max |k| of the block; of all blocks
   constexpr int CH = sel_cols<D>() / 8, LP = D / (8 * CH);
   const int S = a.cluster;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / S;
   const int t = unit / a.Hkv, h = unit - t * a.Hkv;
   const int G = a.Hq / a.Hkv;
-  // the group's queries in 64 bits, [head][4 CH][LP] pairs of columns, zeros up
-  // to a whole SEL_HEADS; then the ring; then page ids and keys
+  const int lane = threadIdx.x & 31;
+  // the group's queries in fp32, [head][2 CH][LP] fours of columns, zeros up to
+  // a whole SEL_HEADS; then the ring; then page ids and keys
   const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
-  double2* qd = reinterpret_cast<double2*>(smem);
-  const uint32_t ring = smem_u32(smem + size_t(G4) * D * 8);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(smem + size_t(G4) * D * 8 + sel_ring<D>());
+  float4* qf = reinterpret_cast<float4*>(smem);
+  const uint32_t ring = smem_u32(smem + size_t(G4) * D * 4);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem + size_t(G4) * D * 4 + sel_ring<D>());
   int* ids = reinterpret_cast<int*>(keys);  // until their scores are known
+  if (threadIdx.x == 0) q_size = k_size = 0u;
 
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
-  for (int i = threadIdx.x; i < G4 * D / 2; i += SEL_THREADS) {
-    const int g = i / (D / 2), d = i % (D / 2) * 2;  // columns d, d + 1: chunk, lane and pair
-    float2 f = make_float2(0.f, 0.f);
-    if (g < G) f = unpack2<DT>(__ldg(reinterpret_cast<const uint32_t*>(q + g * a.q_sh + d)));
-    qd[(g * (4 * CH) + d / (8 * LP) * 4 + d % 8 / 2) * LP + d / 8 % LP] = make_double2(double(f.x), double(f.y));
+  for (int i = threadIdx.x; i < G4 * D / 4; i += SEL_THREADS) {
+    const int g = i / (D / 4), d = i % (D / 4) * 4;  // columns d .. d + 3: chunk, half and lane
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (g < G) {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(q + g * a.q_sh + d));
+      const float2 x = unpack2<DT>(w.x), y = unpack2<DT>(w.y);
+      f = make_float4(x.x, x.y, y.x, y.y);
+    }
+    qf[(g * (2 * CH) + d / (8 * LP) * 2 + d / 4 % 2) * LP + d / 8 % LP] = f;
   }
   const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
   int* out = a.out + (long long)unit * a.top;
@@ -489,27 +621,57 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   // this block's pages: a contiguous share
   const int share = (M + S - 1) / S;
   const int p0 = rank * share, pn = max(0, min(share, M - p0));
+  const int* pages = a.table + (long long)row.b * a.width + a.sink;
   for (int i = threadIdx.x; i < pn; i += SEL_THREADS) {
-    const int id = __ldg(a.table + (long long)row.b * a.width + a.sink + p0 + i);
+    const int id = __ldg(pages + p0 + i);
     const bool ok = id >= 0 && id < a.num_pages;
     if (!ok && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
     ids[i] = ok ? id : -1;
   }
   if (S > 1) cluster_sync();  // and the first block has begun, so that its shared memory may be written
   else __syncthreads();
+  if (rank == 0)  // as bits: of sizes, these have the floats' order, and NaN is the largest
+    for (int g = threadIdx.x >> 5; g < G; g += SEL_WARPS) {
+      const float* row_of = reinterpret_cast<const float*>(qf + g * (D / 4));
+      float s = 0.f;
+#pragma unroll
+      for (int d = 0; d < D; d += 32) s += fabsf(row_of[d + lane]);
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+      if (lane == 0) atomicMax(&q_size, __float_as_uint(s) & 0x7fffffffu);
+    }
   const uint32_t keys0 = smem_u32(keys) + 4u * uint32_t(p0);
-  score_pages<D, DT>(a, qd, ids, ring, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
+  const float top = score_pages<D, DT>(a, qf, ids, ring, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
+  const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if (lane == 0) atomicMax(&k_size, top_bits);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t to = smem_u32(k_sizes + rank);
+    st_cluster_u32(S > 1 ? cluster_map(to, 0) : to, k_size);
+  }
+  if (threadIdx.x < 4 && rank == 0 && M + int(threadIdx.x) < (M + 3) / 4 * 4) keys[M + threadIdx.x] = 0u;
   if (S > 1) {
     cluster_sync();
     if (rank != 0) return;
   } else {
     __syncthreads();
   }
-  if (M <= SEL_THREADS) write_top_small(keys, M, kk, a.sink, out + a.sink);
-  else if (M <= 4 * SEL_THREADS) write_top<4>(keys, M, kk, a.sink, out + a.sink);
-  else if (M <= 8 * SEL_THREADS) write_top<8>(keys, M, kk, a.sink, out + a.sink);
-  else if (M <= 16 * SEL_THREADS) write_top<16>(keys, M, kk, a.sink, out + a.sink);
-  else write_top<0>(keys, M, kk, a.sink, out + a.sink);
+  uint32_t size = 0u;
+  for (int i = 0; i < S; ++i) size = max(size, k_sizes[i]);
+  // 19 roundings of a score's sum and the one of its definition, 2^-24 of the
+  // sum of sizes each (and 2^-150 below the normal numbers), rounded up
+  const float sizes = __uint_as_float(q_size) * __uint_as_float(size);
+  const float slack = q_size == 0u || size == 0u ? 0.f : sizes * (24.f / 16777216.f) + 1e-43f;
+  auto rescore = [&](int p) {
+    const int id = __ldg(pages + p);
+    return id >= 0 && id < a.num_pages ? exact_key<D, DT>(a, qf, h, G, id) : 0u;
+  };
+  out += a.sink;
+  if (M <= SEL_THREADS) write_top<1>(sh, keys, M, kk, a.sink, out, slack, rescore);
+  else if (M <= 4 * SEL_THREADS) write_top<4>(sh, keys, M, kk, a.sink, out, slack, rescore);
+  else if (M <= 8 * SEL_THREADS) write_top<8>(sh, keys, M, kk, a.sink, out, slack, rescore);
+  else if (M <= 16 * SEL_THREADS) write_top<16>(sh, keys, M, kk, a.sink, out, slack, rescore);
+  else write_top<0>(sh, keys, M, kk, a.sink, out, slack, rescore);
 }
 
 // ---------------------------------------------------------------------------
@@ -537,7 +699,6 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = (DEC_WARPS + 2) * 32;
 constexpr int DEC_TILE = 64;
 constexpr int NO_KEY = 0x7fffffff;
-constexpr int MAX_CLUSTER = 8;
 
 template <int D>
 constexpr int dec_stages() {
@@ -962,7 +1123,7 @@ int run_select(const SelectArgs& a) {
   auto* kernel = fa_select_pages_kernel<D, DT>;
   const int G = a.Hq / a.Hkv;
   const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
-  const size_t smem = size_t(G4) * D * 8 + sel_ring<D>() + (size_t(a.width) * 4 + 15) / 16 * 16;
+  const size_t smem = size_t(G4) * D * 4 + sel_ring<D>() + (size_t(a.width) * 4 + 15) / 16 * 16;
   constexpr size_t most = size_t(220) << 10;  // of an SM's 227 KB, the static part left out
   if (smem > most) return FA_ERR_BAD_SHAPE;
   if (int rc = allow_smem<fa_select_pages_kernel<D, DT>>(int(most))) return rc;
