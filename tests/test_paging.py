@@ -685,3 +685,56 @@ def test_serving_step_captured_and_replayed():
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
     assert torch.equal(a.lens, eager.lens) and torch.equal(a.means, eager.means) and torch.equal(a.bt, eager.bt)
     assert _abi.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once_with_strided_queries_and_tables():
+    """The same calls from two streams that overlap, with queries that are
+    views of a projection (and one off the 16-byte boundary) and a table that
+    is a view, give what they give alone."""
+    cases = [Case([1, 2, 1], [900, 333, 64], 16, 8, 2, 64, BF16, s, pad=1) for s in (21, 22)]
+    want, work = [], []
+    for c in cases:
+        q, kc, vc, table, cu, lens = c.cuda()
+        proj = torch.zeros(q.shape[0], 12, 64, dtype=BF16, device="cuda")
+        proj[:, 2:10] = q
+        odd = torch.zeros(q.numel() + 1, dtype=BF16, device="cuda")
+        odd[1:] = q.flatten()
+        wide = torch.full((table.shape[0], table.shape[1] + 3), -1, dtype=torch.int32, device="cuda")
+        wide[:, :-3] = table
+        work.append((proj[:, 2:10], odd[1:].view(q.shape), kc, vc, wide[:, :-3], cu, lens))
+        want.append(_select_and_attend(q, kc, vc, table, cu, lens))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for st, (view, odd, *rest) in zip(streams, work):
+            with torch.cuda.stream(st):
+                got.append([_select_and_attend(q, *rest) for q in (view, odd)])
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for one in g:
+                assert all(torch.equal(a, b) for a, b in zip(one, w))
+    assert _abi.device_status() == 0
+
+
+def _select_and_attend(q, kc, vc, table, cu, lens):
+    means = torch.zeros(kc.shape[0], *kc.shape[2:], dtype=kc.dtype, device=kc.device)
+    full = torch.cat([cu[:1], lens.cumsum(0)]).int()
+    fa.update_page_means(kc, means, table, full, lens)
+    pages = fa.select_pages(q, means, table, cu, lens, page_size=kc.shape[1], num_selected=7)
+    return pages, fa.scaled_dot_product_attention_paged_sparse(q, kc, vc, table, cu, lens, pages, enable_gqa=True)
+
+
+@pytest.mark.gpu
+def test_many_rows_a_sequence():
+    """A prefill chunk through the decode calls: more rows than the GPU holds
+    blocks, with lists of all their pages, against the paged call."""
+    c = Case([700, 1, 300], [700, 1000, 333], 32, 8, 2, 64, F16, 31, junk=0.0)
+    q, kc, vc, table, cu, lens = c.cuda()
+    means = torch.zeros(kc.shape[0], 2, 64, dtype=F16, device="cuda")
+    pages = fa.select_pages(q, means, table, cu, lens, page_size=32, num_selected=table.shape[1])
+    got = fa.scaled_dot_product_attention_paged_sparse(q, kc, vc, table, cu, lens, pages, enable_gqa=True)
+    want = fa.scaled_dot_product_attention_paged(q, kc, vc, table.clamp(min=0), cu, lens, 700, 1000, is_causal=True,
+                                                 enable_gqa=True)
+    assert float((got.float() - want.float()).abs().max()) <= 4e-3  # each within 2e-3 of float64

@@ -375,3 +375,40 @@ def test_training_step_with_the_attention():
     assert float((o.double() - o64).abs().max()) <= 4e-3  # 2e-3, and q and k rounded on the way
     for a, r in zip(got, want):
         assert float((a.double() - r).abs().max()) <= 1e-2 * max(1.0, float(r.abs().max()))
+
+
+@pytest.mark.gpu
+def test_a_gradient_of_the_gradient_is_refused():
+    q = torch.randn(4, 2, 32, device="cuda").half().requires_grad_()
+    table, pos = fa.rotary_table(4, 32).cuda(), torch.arange(4, dtype=torch.int32).cuda()
+    z, _ = fa.qk_norm_rotary(q, q, table, pos)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(z.float().sum(), q, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_rows_that_cannot_be_read_in_place_are_copied():
+    """Rows off the 16-byte boundary, odd strides and a transposed head
+    dimension give what contiguous rows give, forward and backward."""
+    g = torch.Generator().manual_seed(9)
+    table, pos = fa.rotary_table(50, 64).cuda(), torch.arange(50, dtype=torch.int32).cuda()
+    w = torch.rand(64, generator=g).cuda()
+    base = _randn(g, 50, 4, 64, dtype=F16).cuda()
+    wide = torch.zeros(50, 4, 67, dtype=F16, device="cuda")
+    wide[:, :, 3:] = base
+    shifted = torch.zeros(base.numel() + 1, dtype=F16, device="cuda")
+    shifted[1:] = base.flatten()
+    views = [wide[:, :, 3:], shifted[1:].view(50, 4, 64), base.transpose(1, 2).contiguous().transpose(1, 2)]
+    gz = _randn(g, 50, 4, 64, dtype=F16).cuda()
+
+    def step(x, gz):
+        x = x.detach().requires_grad_()
+        z = fa.qk_norm_rotary(x, x, table, pos, query_weight=w, key_weight=w)[0]
+        return z.detach(), torch.autograd.grad(z, x, gz)[0]
+
+    want = step(base, gz)
+    for v in views:
+        got = step(v, gz.transpose(1, 2).contiguous().transpose(1, 2))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    z = fa.qk_norm_rotary(base, base, table, pos)[0]
+    assert torch.equal(z.expand(1, 50, 4, 64)[0], z)

@@ -214,9 +214,12 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
 // found again.  The pages above T, and of those at T the first ones, are
 // written in order of their index.
 //
-// Bound: the means' bytes and the start; 64-bit sums throughout (64 products a
-// clock and SM, 16 conversions) took 23 us for 64 units of 2,048 pages where
-// this takes SELECT_US.
+// Bound: issued instructions of the scores, then the latency of the rounds.
+// 64 (token, K/V head) units of 2,048 pages, 4 heads each, D 128: 21 us, of
+// which the scores take 8 and finding T and writing 6 (the means' bytes alone
+// take 5); 128 units of 128 pages: 7.4 us, nearly all of it start and
+// latency.  64-bit sums throughout (64 products a clock and SM, 16
+// conversions) took 15 us for the scores, and larger groups in proportion.
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
 constexpr int SEL_PAGES = 4;
@@ -694,7 +697,10 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
 //
 // Bound: HBM, 4 D bytes a key.  For a key the products take some 3 clocks of
 // the 22 that its bytes take an SM's share of HBM; tcgen05's 128 rows would
-// be 15 of 16 parts empty for a group's heads.
+// be 15 of 16 parts empty for a group's heads.  16 sequences x 8 K/V heads x
+// 2,048 keys at D 128: 27 us (134 MB: 20.5 us of HBM), of which 4 go before the
+// first keys arrive and 2.5 behind the last; without the products it takes 24.
+// 2 sequences x 8 x 8,192 keys in pages of 16: 19 us (10.3 of HBM).
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = (DEC_WARPS + 2) * 32;
 constexpr int DEC_TILE = 64;
@@ -702,13 +708,7 @@ constexpr int NO_KEY = 0x7fffffff;
 
 template <int D>
 constexpr int dec_stages() {
-#ifndef T_ST64
-#define T_ST64 3
-#endif
-#ifndef T_ST32
-#define T_ST32 6
-#endif
-  return D == 128 ? 3 : D == 64 ? T_ST64 : T_ST32;
+  return D == 32 ? 6 : 3;
 }
 template <int D>
 constexpr int dec_tile_bytes() {
@@ -764,12 +764,14 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c, uint32_t box) {
   else return (D == 128 && (c & 8) ? box : 0u) + uint32_t(r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-#ifndef T_M64
-#define T_M64 4
-#endif
+// Blocks a SM, with what dec_stages takes of shared memory.  D 64, 4 drafted
+// tokens of 31 sequences (496 units): 4 blocks x 3 stages hold all units at
+// once, 27 us; 3 x 3 35, 2 x 6 33, in two waves.  D 128, 2 blocks: 3 stages
+// 27 us, 2 stages and 3 blocks 29 (16 sequences, 128 units in clusters of 2;
+// in clusters of 1, 4 and 8: 28, 33 and 45).
 template <int D>
 constexpr int dec_per_sm() {
-  return D == 128 ? 2 : T_M64;
+  return D == 128 ? 2 : 4;
 }
 template <int D, int DT>
 __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
@@ -1170,9 +1172,6 @@ int launch_sparse_decode(SparseArgs a, const CUtensorMap& k, const CUtensorMap& 
   const long long tiles = (((long long)a.top << a.page_log2) + DEC_TILE - 1) / DEC_TILE;
   a.cluster = cluster_for((long long)a.total_q * a.Hkv * ((G + 7) / 8), tiles, 2,
                           D == 128 ? dec_per_sm<128>() : dec_per_sm<64>());
-#ifdef T_DS
-  a.cluster = T_DS;
-#endif
   if (a.dtype == DT_BF16)
     return D == 32 ? run_sparse<32, DT_BF16>(a, k, v)
                    : D == 64 ? run_sparse<64, DT_BF16>(a, k, v) : run_sparse<128, DT_BF16>(a, k, v);
