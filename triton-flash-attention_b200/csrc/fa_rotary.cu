@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(cons
   const int chunks = q_chunks + k_chunks * (APPEND ? 2 : 1);
   const int wid = blockIdx.x * WARPS + threadIdx.x / 32;
   const int part = wid / chunks, chunk = wid - part * chunks;
+  begin_after_previous();
   if (part >= a.parts) return;
   const int kind = chunk < q_chunks ? 0 : chunk < q_chunks + k_chunks ? 1 : 2;
   const int h = (chunk - (kind == 0 ? 0 : kind == 1 ? q_chunks : q_chunks + k_chunks)) * GW + lane / L;
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) fa_rotary_bwd_kernel(cons
   const bool valid = h < H;
   const int per_part = is_q ? a.per_part : a.k_per_part;
   Run<C> dwa = fill_run<C>(0.f), dwb = dwa;
+  begin_after_previous();
   if (part < (is_q ? a.parts : a.k_parts)) {
     const Range range(a, part, per_part);
     Rows gp(is_q ? a.gq : a.gk, is_q ? a.gqs : a.gks, a.N, range.b, range.n, h, c.a);
@@ -479,6 +481,7 @@ __global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const float* __restr
   const int last = blockIdx.y == 0 ? q_ctas : ctas;
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int d = blockIdx.x * 32 + lane;
+  begin_after_previous();
   float v = 0.f;
 #pragma unroll 8
   for (int i = first + row; i < last; i += 32) v += part[(long long)i * D + d];
@@ -516,8 +519,8 @@ int run_fwd(RotaryArgs a) {
   a.parts = cut_tokens(tokens, chunks, most * WARPS, &a.per_part);
   const long long ctas = ((long long)a.parts * chunks + WARPS - 1) / WARPS;
   if (ctas * WARPS > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
-  fa_rotary_fwd_kernel<D, DT, INTER, NORM, APPEND><<<unsigned(ctas), THREADS, smem, a.stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  return launch_early(fa_rotary_fwd_kernel<D, DT, INTER, NORM, APPEND>, dim3(unsigned(ctas)), THREADS, smem, 1, a.stream,
+                      a);
 }
 
 template <int D, int DT, bool INTER, bool NORM>
@@ -540,14 +543,12 @@ int run_bwd(RotaryArgs a) {
   // w_part than there are
   if (q_ctas + k_ctas > ROTARY_BWD_CTAS) return FA_ERR_BAD_SHAPE;
   a.q_ctas = int(q_ctas);
-  fa_rotary_bwd_kernel<D, DT, INTER, NORM><<<unsigned(q_ctas + k_ctas), THREADS, smem, a.stream>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
-  if (a.w_part) {
-    fa_rotary_dw_kernel<DT><<<dim3(D / 32, 2), 1024, 0, a.stream>>>(a.w_part, D, int(q_ctas), int(q_ctas + k_ctas),
-                                                                    a.dwq, a.dwk, a.w_fp32);
-    if (cudaGetLastError() != cudaSuccess) return FA_ERR_LAUNCH;
-  }
-  return FA_OK;
+  if (int rc = launch_early(fa_rotary_bwd_kernel<D, DT, INTER, NORM>, dim3(unsigned(q_ctas + k_ctas)), THREADS, smem, 1,
+                            a.stream, a))
+    return rc;
+  if (!a.w_part) return FA_OK;
+  return launch_early(fa_rotary_dw_kernel<DT>, dim3(D / 32, 2), 1024, 0, 1, a.stream, (const float*)a.w_part, D,
+                      int(q_ctas), int(q_ctas + k_ctas), a.dwq, a.dwk, a.w_fp32);
 }
 
 // Instantiated for the head dims, operand types, pairings and with and

@@ -62,22 +62,32 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
   const int cols = min(W8, MEAN_THREADS);
   const int groups = min(MEAN_THREADS / cols, 8);
   const int P = 1 << a.page_log2;
+  let_next_begin();
+  begin_after_previous();
   units = min(units, (__ldg(a.cu + a.B) >> a.page_log2) + a.B);  // the step's own rows
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    // last b with off(b) <= u
-    const int lane = threadIdx.x & 31;
-    int lo = 0, len = a.B;
-    while (len > 1) {
-      const int step = (len + 31) / 32;
-      const int i = lane * step;
-      const bool ok = i < len && (__ldg(a.cu + lo + i) >> a.page_log2) + lo + i <= u;
-      const int c = __popc(__ballot_sync(0xffffffffu, ok));
-      const int at = c > 0 ? (c - 1) * step : 0;
-      lo += at;
-      len = min(step, len - at);
+    // last b with off(b) <= u.  A decode step's first guess is b = u, loaded at
+    // once; the search with its dependent loads is for other batches
+    int b = min(u, a.B - 1);
+    int q0 = __ldg(a.cu + b), q1 = __ldg(a.cu + b + 1), nk = __ldg(a.seqlens + b);
+    if ((q0 >> a.page_log2) + b > u || (b + 1 < a.B && (q1 >> a.page_log2) + b + 1 <= u)) {
+      const int lane = threadIdx.x & 31;
+      int lo = 0, len = a.B;
+      while (len > 1) {
+        const int step = (len + 31) / 32;
+        const int i = lane * step;
+        const bool ok = i < len && (__ldg(a.cu + lo + i) >> a.page_log2) + lo + i <= u;
+        const int c = __popc(__ballot_sync(0xffffffffu, ok));
+        const int at = c > 0 ? (c - 1) * step : 0;
+        lo += at;
+        len = min(step, len - at);
+      }
+      b = lo;
+      q0 = __ldg(a.cu + b);
+      q1 = __ldg(a.cu + b + 1);
+      nk = __ldg(a.seqlens + b);
     }
-    const int b = lo;
-    const int q0 = __ldg(a.cu + b), nq = __ldg(a.cu + b + 1) - q0, nk = __ldg(a.seqlens + b);
+    const int nq = q1 - q0;
     if (nq <= 0 || nk <= 0) continue;
     const int from = max(nk - nq, 0) >> a.page_log2;
     const long long p = (long long)from + (u - ((q0 >> a.page_log2) + b));
@@ -592,6 +602,8 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   uint32_t* keys = reinterpret_cast<uint32_t*>(smem + size_t(G4) * D * 4 + sel_ring<D>());
   int* ids = reinterpret_cast<int*>(keys);  // until their scores are known
   if (threadIdx.x == 0) q_size = k_size = 0u;
+  let_next_begin();
+  begin_after_previous();
 
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
   for (int i = threadIdx.x; i < G4 * D / 4; i += SEL_THREADS) {
@@ -809,6 +821,8 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
     }
     fence_mbar_init();
   }
+  let_next_begin();
+  begin_after_previous();
   // the producers' first list entries do not wait for the row's place
   const int PT = DEC_TILE / PR;                  // pieces of a tile
   const int sub_log2 = max(0, a.page_log2 - 6);  // pieces of a page
@@ -1091,24 +1105,6 @@ int allow_smem(int bytes) {
   return FA_OK;
 }
 
-// A launch in clusters of S blocks (1: none).
-template <class... Params, class... Args>
-int launch_clustered(void (*kernel)(Params...), unsigned blocks, unsigned threads, size_t smem, int S,
-                     cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = unsigned(S);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = S > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
-}
-
 template <int D, int DT>
 int run_sparse(const SparseArgs& a, const CUtensorMap& k, const CUtensorMap& v) {
   auto* kernel = fa_sparse_decode_kernel<D, DT>;
@@ -1117,7 +1113,7 @@ int run_sparse(const SparseArgs& a, const CUtensorMap& k, const CUtensorMap& v) 
   const int G = a.Hq / a.Hkv;
   const long long units = (long long)a.total_q * a.Hkv * ((G + 7) / 8);
   if (units * a.cluster > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
-  return launch_clustered(kernel, unsigned(units * a.cluster), DEC_THREADS, size_t(smem), a.cluster, a.stream, k, v, a);
+  return launch_early(kernel, dim3(unsigned(units * a.cluster)), DEC_THREADS, size_t(smem), a.cluster, a.stream, k, v, a);
 }
 
 template <int D, int DT>
@@ -1131,7 +1127,7 @@ int run_select(const SelectArgs& a) {
   if (int rc = allow_smem<fa_select_pages_kernel<D, DT>>(int(most))) return rc;
   const long long units = (long long)a.total_q * a.Hkv;
   if (units * a.cluster > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
-  return launch_clustered(kernel, unsigned(units * a.cluster), SEL_THREADS, smem, a.cluster, a.stream, a);
+  return launch_early(kernel, dim3(unsigned(units * a.cluster)), SEL_THREADS, smem, a.cluster, a.stream, a);
 }
 
 // Blocks that share a unit: the largest power of two up to 8 with which all
@@ -1155,9 +1151,8 @@ int launch_page_means(const PageArgs& a, int total_q) {
   const int groups = MEAN_THREADS / cols < 8 ? MEAN_THREADS / cols : 8;
   const size_t smem = size_t(groups - 1) * 8 * cols * 8;
   if (units > 0x7fffffffLL) return FA_ERR_BAD_SHAPE;
-  if (a.dtype == DT_BF16) fa_page_means_kernel<DT_BF16><<<ctas, MEAN_THREADS, smem, a.stream>>>(a, int(units));
-  else fa_page_means_kernel<DT_F16><<<ctas, MEAN_THREADS, smem, a.stream>>>(a, int(units));
-  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  return launch_early(a.dtype == DT_BF16 ? fa_page_means_kernel<DT_BF16> : fa_page_means_kernel<DT_F16>, dim3(ctas),
+                      MEAN_THREADS, smem, 1, a.stream, a, int(units));
 }
 
 int launch_select_pages(SelectArgs a, int D) {

@@ -62,6 +62,8 @@ __global__ void __launch_bounds__(THREADS) fa_extend_table_kernel(const __grid_c
   __shared__ int have[THREADS], first[THREADS], cached[THREADS];
   __shared__ unsigned char fit[THREADS];
   const int tid = threadIdx.x;
+  let_next_begin();
+  begin_after_previous();
   const long long page = 1LL << a.page_log2;
   long long start = *a.free_start;
   if (start < 0) start = 0;
@@ -153,8 +155,7 @@ int launch_extend_table(const TableArgs& a) {
   if (ctas < 1) ctas = 1;
   const int sms = device_sm_count();
   if (ctas > sms) ctas = sms;
-  fa_extend_table_kernel<<<unsigned(ctas), THREADS, 0, a.stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  return launch_early(fa_extend_table_kernel, dim3(unsigned(ctas)), THREADS, 0, 1, a.stream, a);
 }
 
 }  // namespace fa
