@@ -412,3 +412,37 @@ def test_rows_that_cannot_be_read_in_place_are_copied():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     z = fa.qk_norm_rotary(base, base, table, pos)[0]
     assert torch.equal(z.expand(1, 50, 4, 64)[0], z)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_may_come_back_laid_out_otherwise():
+    """Queries and keys are views of a fused projection; hooks on the saved
+    tensors give them back contiguous, off a 16-byte boundary, or by way of the
+    host.  The gradients do not change."""
+    g = torch.Generator().manual_seed(10)
+    x = _randn(g, 2, 37, 8, 64, dtype=BF16).cuda().requires_grad_()
+    w = (1 + 0.3 * _randn(g, 64)).cuda().requires_grad_()
+    table = fa.rotary_table(37, 64).cuda()
+    gq, gk = _randn(g, 2, 4, 37, 64, dtype=BF16).cuda(), _randn(g, 2, 2, 37, 64, dtype=BF16).cuda()
+
+    def step():
+        q, k = x[:, :, :4].transpose(1, 2), x[:, :, 4:6].transpose(1, 2)
+        z = fa.qk_norm_rotary(q, k, table, query_weight=w, key_weight=w)
+        return torch.autograd.grad(z, (x, w), (gq, gk))
+
+    def contiguous(t):
+        return t.detach().clone(memory_format=torch.contiguous_format)
+
+    def shifted(t):
+        if t.ndim < 4:
+            return contiguous(t)
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        return room[1:].view(t.shape).copy_(t.detach())
+
+    want = step()
+    for hooks in (torch.autograd.graph.saved_tensors_hooks(contiguous, lambda t: t),
+                  torch.autograd.graph.saved_tensors_hooks(shifted, lambda t: t),
+                  torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True)):
+        with hooks:
+            got = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

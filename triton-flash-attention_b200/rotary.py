@@ -219,7 +219,8 @@ def _contiguous_like(t):
 
 def _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved):
     """The forward's launch; besides the outputs what the backward's takes of
-    it: the rows as they were read and the arguments both have."""
+    it: the rows as they were read, the sizes, and the arguments both have of the
+    outputs' and of positions."""
     q, qp, qs = row_arg(q)
     k, kp, ks = row_arg(k)
     b, hq, hkv, n, d = _sizes(q, k)
@@ -231,22 +232,25 @@ def _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved)
     _, kop, kos = row_arg(ko)
     launch(q, "fa_qk_norm_rotary", q.dtype, qp, kp, qop, kop, table.data_ptr(), _ptr(positions), _ptr(query_weight),
            _ptr(key_weight), b, hq, hkv, n, d, max_positions, rd, interleaved, fp32, qs, ks, qos, kos, per_batch, eps)
-    return qo, ko, q, k, (b, hq, hkv, n, d, max_positions, rd, interleaved, fp32), (qs, ks, qos, kos, per_batch, eps)
+    return qo, ko, q, k, (b, hq, hkv, n, d, max_positions, rd, interleaved, fp32), (qos, kos, per_batch, eps)
 
 
 def _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, sizes, rest, weight_grads):
-    """The backward's launch, for q and k as ``_forward`` gave them back.  (It
+    """The backward's launch, with ``sizes`` and ``rest`` of ``_forward``.  (It
     runs on autograd's own thread, where host work costs more: what the
-    forward worked out is not worked out again.)"""
+    forward worked out is not worked out again.  The rows' strides are: a hook
+    on saved tensors may give them back laid out otherwise.)"""
+    q, qp, qs = row_arg(q)
+    k, kp, ks = row_arg(k)
     grad_q, gqp, gqs = row_arg(grad_q)
     grad_k, gkp, gks = row_arg(grad_k)
-    qs, ks, qos, kos, per_batch, eps = rest
+    qos, kos, per_batch, eps = rest
     dq, dk = _contiguous_like(q), _contiguous_like(k)
     dwq = dwk = part = None
     if weight_grads:
         dwq, dwk = torch.empty_like(query_weight), torch.empty_like(key_weight)
         part = table.new_empty(ROTARY_PARTIALS * sizes[4])
-    launch(q, "fa_qk_norm_rotary_bwd", q.dtype, q.data_ptr(), k.data_ptr(), gqp, gkp, dq.data_ptr(), dk.data_ptr(),
+    launch(q, "fa_qk_norm_rotary_bwd", q.dtype, qp, kp, gqp, gkp, dq.data_ptr(), dk.data_ptr(),
            _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight),
            *sizes, qs, ks, gqs, gks, qos, kos, per_batch, eps)
     return dq, dk, dwq, dwk
@@ -261,14 +265,12 @@ def qk_norm_rotary_backward(q, k, grad_q, grad_k, table, positions, query_weight
                             interleaved: bool, weight_grads: bool = True):
     """dQ, dK and, with weights and ``weight_grads``, the weights' gradients
     (else None).  Gradients repeat bit for bit."""
-    q, _, qs = row_arg(q)
-    k, _, ks = row_arg(k)
     qos, kos = _contiguous_strides(q.shape), _contiguous_strides(k.shape)
     sizes = (*_sizes(q, k), *table.shape, interleaved,
              query_weight is not None and query_weight.dtype == torch.float32)
     per_batch = sizes[3] if positions is not None and positions.ndim == 2 else 0
     return _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, sizes,
-                     (qs, ks, qos, kos, per_batch, eps), weight_grads and query_weight is not None)
+                     (qos, kos, per_batch, eps), weight_grads and query_weight is not None)
 
 
 class B200QKNormRotary(torch.autograd.Function):
