@@ -182,7 +182,9 @@ int launch_sparse_decode(SparseArgs a, const CUtensorMap& k, const CUtensorMap& 
 // stream is still ending (programmatic dependent launch): that hides 1 to 3 us
 // of a launch.  Each calls begin_after_previous(), in every thread and before
 // it reads or writes any global memory: it waits until all earlier kernels of
-// the stream are done and their writes are seen.
+// the stream are done and their writes are seen.  (Their loads are plain ones:
+// read-only loads, __ldg and __restrict__ to const, promise data that nobody
+// writes while the kernel lives, which starts before that wait.)
 __device__ __forceinline__ void begin_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the stream's next kernel come on once every block has called it, not
 // when the last one has ended.  The kernels of a serving step call it at once

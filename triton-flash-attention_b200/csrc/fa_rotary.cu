@@ -147,8 +147,8 @@ __device__ __forceinline__ Run<C> load_w(const void* w, int w_fp32, int c) {
   Run<C> f;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    f.v[i] = w_fp32 ? __ldg(static_cast<const float*>(w) + c + i)
-                    : unpack2<DT>(uint32_t(__ldg(static_cast<const uint16_t*>(w) + c + i))).x;
+    f.v[i] = w_fp32 ? *(static_cast<const float*>(w) + c + i)
+                    : unpack2<DT>(uint32_t(*(static_cast<const uint16_t*>(w) + c + i))).x;
   }
   return f;
 }
@@ -160,7 +160,7 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 __device__ __forceinline__ int raw_pos(const RotaryArgs& a, int b, int n) {
-  return a.pos ? __ldg(a.pos + (long long)b * a.pos_sb + n) : n;
+  return a.pos ? a.pos[(long long)b * a.pos_sb + n] : n;
 }
 // The position, or -1 (with the device status word set) when it has no row in
 // the table.
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(cons
     wa = load_w<DT, C>(kind == 0 ? a.wq : a.wk, a.w_fp32, c.a);
     wb = load_w<DT, C>(kind == 0 ? a.wq : a.wk, a.w_fp32, c.b);
   }
-  int slot = cached ? __ldg(a.slots + range.n) : 0;
+  int slot = cached ? a.slots[range.n] : 0;
   int n = range.n;
   uint32_t here = mem;
   for (int left = range.count; left > 0; --left) {
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(cons
         st_run<C>(p, ra);
         st_run<C>(p + ab, rb);
       }
-      if (left > 1) slot = __ldg(a.slots + ++n);
+      if (left > 1) slot = a.slots[++n];
     } else {
       if (valid) {
         st_run<C>(const_cast<uint16_t*>(dst.p), ra);
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) fa_rotary_bwd_kernel(cons
 // partial sums (y = 0) or the key blocks' (y = 1), 32 rows of them a pass, in
 // a fixed order.
 template <int DT>
-__global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const float* __restrict__ part, int D, int q_ctas, int ctas,
+__global__ void __launch_bounds__(1024) fa_rotary_dw_kernel(const float* part, int D, int q_ctas, int ctas,
                                                             void* dwq, void* dwk, int w_fp32) {
   __shared__ float sums[32][33];
   const int first = blockIdx.y == 0 ? 0 : q_ctas;

@@ -23,13 +23,13 @@ namespace {
 
 // Sequence of packed row t: the last b with cu[b] <= t, by 32 probes a step.
 // Every lane of the warp calls and gets it.
-__device__ __forceinline__ int warp_find_seq(const int* __restrict__ cu, int B, int t) {
+__device__ __forceinline__ int warp_find_seq(const int* cu, int B, int t) {
   const int lane = threadIdx.x & 31;
   int lo = 0, len = B;
   while (len > 1) {
     const int step = (len + 31) / 32;
     const int i = lane * step;
-    const bool ok = i < len && __ldg(cu + lo + i) <= t;
+    const bool ok = i < len && cu[lo + i] <= t;
     const int c = __popc(__ballot_sync(0xffffffffu, ok));
     const int at = c > 0 ? (c - 1) * step : 0;
     lo += at;
@@ -64,35 +64,35 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
   const int P = 1 << a.page_log2;
   let_next_begin();
   begin_after_previous();
-  units = min(units, (__ldg(a.cu + a.B) >> a.page_log2) + a.B);  // the step's own rows
+  units = min(units, (a.cu[a.B] >> a.page_log2) + a.B);  // the step's own rows
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     // last b with off(b) <= u.  A decode step's first guess is b = u, loaded at
     // once; the search with its dependent loads is for other batches
     int b = min(u, a.B - 1);
-    int q0 = __ldg(a.cu + b), q1 = __ldg(a.cu + b + 1), nk = __ldg(a.seqlens + b);
+    int q0 = a.cu[b], q1 = a.cu[b + 1], nk = a.seqlens[b];
     if ((q0 >> a.page_log2) + b > u || (b + 1 < a.B && (q1 >> a.page_log2) + b + 1 <= u)) {
       const int lane = threadIdx.x & 31;
       int lo = 0, len = a.B;
       while (len > 1) {
         const int step = (len + 31) / 32;
         const int i = lane * step;
-        const bool ok = i < len && (__ldg(a.cu + lo + i) >> a.page_log2) + lo + i <= u;
+        const bool ok = i < len && (a.cu[lo + i] >> a.page_log2) + lo + i <= u;
         const int c = __popc(__ballot_sync(0xffffffffu, ok));
         const int at = c > 0 ? (c - 1) * step : 0;
         lo += at;
         len = min(step, len - at);
       }
       b = lo;
-      q0 = __ldg(a.cu + b);
-      q1 = __ldg(a.cu + b + 1);
-      nk = __ldg(a.seqlens + b);
+      q0 = a.cu[b];
+      q1 = a.cu[b + 1];
+      nk = a.seqlens[b];
     }
     const int nq = q1 - q0;
     if (nq <= 0 || nk <= 0) continue;
     const int from = max(nk - nq, 0) >> a.page_log2;
     const long long p = (long long)from + (u - ((q0 >> a.page_log2) + b));
     if (p < from || p >= (nk >> a.page_log2) || p >= a.width) continue;  // uniform in the block
-    const int id = __ldg(a.table + (long long)b * a.width + p);
+    const int id = a.table[(long long)b * a.width + p];
     if (id < 0 || id >= a.num_pages) {
       if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
       continue;
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
       if (mine) {
 #pragma unroll 8
         for (int r = g; r < P; r += groups) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + (long long)r * a.Hkv * a.D) + c);
+          const uint4 v = *(reinterpret_cast<const uint4*>(src + (long long)r * a.Hkv * a.D) + c);
           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -188,12 +188,12 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
   // a decode step brings one row a sequence: that guess is loaded at once,
   // and the search with its dependent loads is for other batches
   r.b = min(t, B - 1);
-  int q0 = __ldg(cu + r.b), q1 = __ldg(cu + r.b + 1), nk = __ldg(seqlens + r.b);
+  int q0 = cu[r.b], q1 = cu[r.b + 1], nk = seqlens[r.b];
   if (t < q0 || t >= q1) {
     r.b = warp_find_seq(cu, B, t);
-    q0 = __ldg(cu + r.b);
-    q1 = __ldg(cu + r.b + 1);
-    nk = __ldg(seqlens + r.b);
+    q0 = cu[r.b];
+    q1 = cu[r.b + 1];
+    nk = seqlens[r.b];
   }
   const long long pos = (long long)nk - (q1 - t);  // the rows are the sequence's last
   const bool too_long = nk > key_cap;  // its table row cannot hold it
@@ -375,7 +375,7 @@ __device__ __forceinline__ uint32_t exact_key(const SelectArgs& a, const float4*
   const uint16_t* k = static_cast<const uint16_t*>(a.means) + ((long long)id * a.Hkv + h) * D + d0;
   double kd[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) kd[i] = double(to_f32<DT>(__ldg(k + i)));
+  for (int i = 0; i < N; ++i) kd[i] = double(to_f32<DT>(k[i]));
   // where columns d0 .. d0 + N - 1 of head 0 lie in qf (N divides 4)
   const float* q = reinterpret_cast<const float*>(qf + (d0 / (8 * LP) * 2 + d0 / 4 % 2) * LP + d0 / 8 % LP) + d0 % 4;
   float best = -INFINITY;
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
     const int g = i / (D / 4), d = i % (D / 4) * 4;  // columns d .. d + 3: chunk, half and lane
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
     if (g < G) {
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(q + g * a.q_sh + d));
+      const uint2 w = *(reinterpret_cast<const uint2*>(q + g * a.q_sh + d));
       const float2 x = unpack2<DT>(w.x), y = unpack2<DT>(w.y);
       f = make_float4(x.x, x.y, y.x, y.y);
     }
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   const int p0 = rank * share, pn = max(0, min(share, M - p0));
   const int* pages = a.table + (long long)row.b * a.width + a.sink;
   for (int i = threadIdx.x; i < pn; i += SEL_THREADS) {
-    const int id = __ldg(pages + p0 + i);
+    const int id = pages[p0 + i];
     const bool ok = id >= 0 && id < a.num_pages;
     if (!ok && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
     ids[i] = ok ? id : -1;
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   const float sizes = __uint_as_float(q_size) * __uint_as_float(size);
   const float slack = q_size == 0u || size == 0u ? 0.f : sizes * (24.f / 16777216.f) + 1e-43f;
   auto rescore = [&](int p) {
-    const int id = __ldg(pages + p);
+    const int id = pages[p];
     return id >= 0 && id < a.num_pages ? exact_key<D, DT>(a, qf, h, G, id) : 0u;
   };
   out += a.sink;
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
   // lane j: piece j % PT of tile t0 + j / PT of the block's
   auto list_entry = [&](int t0) {
     const int piece = ((t0 + lane / PT) * S + rank) * PT + lane % PT;
-    return piece < pieces ? __ldg(list + (piece >> sub_log2)) : -1;
+    return piece < pieces ? list[piece >> sub_log2] : -1;
   };
   int entry = warp >= DEC_WARPS ? list_entry(0) : -1;
   const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
@@ -863,7 +863,7 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
       if (entry >= 0 && entry < a.width) {
         const int first = (entry << a.page_log2) + sub * DEC_TILE;
         if (first <= pos) {
-          const int id = __ldg(a.table + (long long)row.b * a.width + entry);
+          const int id = a.table[(long long)row.b * a.width + entry];
           if (id >= 0 && id < a.num_pages) {
             base = first;
             at = (id << a.page_log2) + sub * DEC_TILE;
@@ -924,7 +924,7 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           qf[ks][j] =
-              g8 < rows && pos >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(q + ks * 16 + j * 8 + t4 * 2)) : 0u;
+              g8 < rows && pos >= 0 ? *(reinterpret_cast<const uint32_t*>(q + ks * 16 + j * 8 + t4 * 2)) : 0u;
     }
     // the warp's 16 rows: their piece, and their place in it
     const uint32_t box = uint32_t(PR) * 128u;

@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(THREADS) fa_extend_table_kernel(const __grid_c
     const int m = min(THREADS, a.requests - r0);
     long long c = 0, f = 0;
     if (r < a.requests) {
-      c = max(0, __ldg(a.cached + r));
-      f = max(0, __ldg(a.fresh + r));
+      c = max(0, a.cached[r]);
+      f = max(0, a.fresh[r]);
     }
     long long toks, pages;
     const long long t_end = tok_base + block_scan(f, warp_sums, &toks);
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(THREADS) fa_extend_table_kernel(const __grid_c
       if (fit[i]) {
         const int lp = int(pos >> a.page_log2);
         const int id = lp < have[i] ? a.table[(long long)(r0 + i) * a.width + lp]
-                                    : __ldg(a.free_pages + start + first[i] + (lp - have[i]));
+                                    : a.free_pages[start + first[i] + (lp - have[i])];
         slot = (long long)id * page + (pos & (page - 1));
         if (id < 0 || slot > 0x7fffffffLL) slot = -1;
       }
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) fa_extend_table_kernel(const __grid_c
     for (long long p = page_base + blockIdx.x * THREADS + tid; p < p_last; p += (long long)gridDim.x * THREADS) {
       const int i = upper(page_end, m, int(p));
       if (i < m && fit[i])
-        a.table[(long long)(r0 + i) * a.width + have[i] + (p - first[i])] = __ldg(a.free_pages + start + p);
+        a.table[(long long)(r0 + i) * a.width + have[i] + (p - first[i])] = a.free_pages[start + p];
     }
     tok_base += toks;
     page_base += pages;
