@@ -603,6 +603,13 @@ FA_API int fa_fwd_paged_sparse_bf16(const void* q, const void* k_cache, const vo
                         int max_pages_per_seq, int top, float softmax_scale, const int64_t* q_strides,
                         void* stream);
 
+/* For callers to whom every argument of a foreign call costs time: the address
+ * of an int (*)(const void* words) that calls the entry `name` ("fa_paged_append",
+ * ...; those from fa_qk_norm_rotary to here) with its arguments as consecutive
+ * 8-byte words, in order: pointers, ints as int64_t (one that is no int:
+ * FA_ERR_BAD_SHAPE), float as double.  NULL for any other name. */
+FA_API void* fa_packed_entry(const char* name);
+
 /* Reads (and with reset != 0 clears) the device status word that kernels set
  * when a bounded wait gives up or an index is out of range: 0 = healthy, else
  * FA_ERR_DEVICE_TIMEOUT or FA_ERR_BAD_INDEX in the low byte and the site in

@@ -16,6 +16,8 @@ Scores are fp32 sums of exact products: up to D 2^-23 of their terms' sum, some
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -738,3 +740,36 @@ def test_many_rows_a_sequence():
     want = fa.scaled_dot_product_attention_paged(q, kc, vc, table.clamp(min=0), cu, lens, 700, 1000, is_causal=True,
                                                  enable_gqa=True)
     assert float((got.float() - want.float()).abs().max()) <= 4e-3  # each within 2e-3 of float64
+
+
+PACKED = ["fa_qk_norm_rotary", "fa_qk_norm_rotary_bwd", "fa_paged_append", "fa_extend_block_table",
+          "fa_page_means", "fa_select_pages", "fa_fwd_paged_sparse"]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("name", PACKED)
+def test_packed_entries_answer_as_the_entries_do(name, dtype):
+    """Arguments that every entry refuses before any CUDA call: null pointers
+    (after the head dim and sizes have passed), a head dim, an int of more
+    than 32 bits."""
+    dtype = None if name == "fa_extend_block_table" else dtype
+    entry = _abi.entry(name, dtype)
+    call, pack = _abi.packed_entry(name, dtype)
+    kinds = _abi.SIGNATURES[entry.__name__][1]
+    for ints in (64, 0, 48, 1 << 30):
+        args = [ints if t is ctypes.c_int else 1e-6 if t is ctypes.c_float else 0 for t in kinds]
+        alone = [None if t not in (ctypes.c_int, ctypes.c_float, ctypes.c_int64) else v for v, t in zip(args, kinds)]
+        rc = entry(*alone)
+        assert rc in (_abi.FA_ERR_BAD_SHAPE, _abi.FA_ERR_UNSUPPORTED_HEAD_DIM)
+        assert call(pack(*args)) == rc
+    wide = [(1 << 32) + 64 if t is ctypes.c_int else 1e-6 if t is ctypes.c_float else 0 for t in kinds]
+    assert call(pack(*wide)) == _abi.FA_ERR_BAD_SHAPE
+    assert call(None) == _abi.FA_ERR_BAD_SHAPE
+
+
+def test_packed_entry_of_another_name():
+    assert not _abi.lib().fa_packed_entry(b"fa_fwd") and not _abi.lib().fa_packed_entry(None)
+    with pytest.raises(RuntimeError, match="packed"):
+        _abi.packed_entry("fa_fwd", torch.float16)
+    s = _abi.strides_of((1, 2, 3))
+    assert s.at == ctypes.addressof(s) and list(s) == [1, 2, 3]

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libfa_b200.so")
@@ -94,6 +95,7 @@ SIGNATURES.update({
                                   _s, _s, _s, _s, _s, _s, _s, _s, _f, _i, _p]),
     "fa_device_status": (_i, [_i]),
     "fa_status_string": (ctypes.c_char_p, [_i]),
+    "fa_packed_entry": (_p, [ctypes.c_char_p]),
     "fa_version": (_i, []),
 })
 
@@ -138,6 +140,27 @@ def entry(name: str, dtype) -> ctypes._CFuncPtr:
     return fn
 
 
+_packed_entries: dict = {}
+_PackedEntry = ctypes.CFUNCTYPE(_i, ctypes.c_char_p)
+
+
+def packed_entry(name: str, dtype) -> tuple:
+    """The entry ``name`` as ``entry`` finds it (None: it has no type), called
+    with its arguments packed to bytes, and what packs them: ints, floats,
+    addresses (0 for NULL) and, for strides, the array's ``at``.  ctypes
+    takes 0.15 us an argument: a refused call of 25 is 3.8 us, this way 0.9."""
+    key = (name, dtype)
+    got = _packed_entries.get(key)
+    if got is None:
+        symbol = entry(name, dtype).__name__
+        at = lib().fa_packed_entry(symbol.encode())
+        if not at:
+            raise RuntimeError(f"{symbol} has no packed form")
+        words = "".join({_f: "d", _i: "q", ctypes.c_int64: "q"}.get(t, "P") for t in SIGNATURES[symbol][1])
+        got = _packed_entries[key] = (_PackedEntry(at), struct.Struct(words).pack)
+    return got
+
+
 def status_string(code: int) -> str:
     return lib().fa_status_string(int(code)).decode()
 
@@ -147,7 +170,14 @@ def check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} failed: {status_string(rc)} (code {rc})")
 
 
-_Strides3 = ctypes.c_int64 * 3
+class _Strides3(ctypes.c_int64 * 3):
+    """Three strides, and their address: ``at``, good while the array lives."""
+
+    def __init__(self, *strides):
+        super().__init__(*strides)
+        self.at = ctypes.addressof(self)
+
+
 _strides_cache: dict = {}
 
 

@@ -3,6 +3,10 @@
 // (include/fa_b200.h).  As in fa_capi.cu: arguments are checked before any
 // CUDA call, nothing is thrown, and every entry returns an FA_ERR_* code.
 #include <cmath>
+#include <cstring>
+#include <tuple>
+#include <type_traits>
+#include <utility>
 
 #include "fa_kernels.h"
 
@@ -355,3 +359,57 @@ FA_SELECT(fa_select_pages_bf16, DT_BF16)
   }
 FA_SPARSE(fa_fwd_paged_sparse, DT_F16)
 FA_SPARSE(fa_fwd_paged_sparse_bf16, DT_BF16)
+
+namespace fa {
+namespace {
+
+// One argument from its 8-byte word; an int that is none clears ok.
+template <class T>
+T from_word(uint64_t w, bool* ok) {
+  if constexpr (std::is_pointer_v<T>) {
+    return reinterpret_cast<T>(uintptr_t(w));
+  } else if constexpr (std::is_same_v<T, float>) {
+    double d;
+    std::memcpy(&d, &w, sizeof d);
+    return float(d);
+  } else {
+    const int64_t v = int64_t(w);
+    if (int64_t(T(v)) != v) *ok = false;
+    return T(v);
+  }
+}
+template <class... A, size_t... I>
+int call_words(int (*fn)(A...), const void* words, std::index_sequence<I...>) {
+  if (!words) return FA_ERR_BAD_SHAPE;
+  uint64_t w[sizeof...(A)];
+  std::memcpy(w, words, sizeof w);
+  bool ok = true;
+  const std::tuple<A...> args{from_word<A>(w[I], &ok)...};
+  return ok ? fn(std::get<I>(args)...) : FA_ERR_BAD_SHAPE;
+}
+template <class... A>
+constexpr std::index_sequence_for<A...> indices(int (*)(A...)) {
+  return {};
+}
+template <auto* Fn>
+int packed(const void* words) {
+  return call_words(Fn, words, indices(Fn));
+}
+
+#define FA_PACKED(NAME) {#NAME, packed<&NAME>}
+#define FA_PACKED2(NAME) FA_PACKED(NAME), FA_PACKED(NAME##_bf16)
+const struct {
+  const char* name;
+  int (*call)(const void*);
+} packed_entries[] = {FA_PACKED2(fa_qk_norm_rotary), FA_PACKED2(fa_qk_norm_rotary_bwd), FA_PACKED2(fa_paged_append),
+                      FA_PACKED(fa_extend_block_table), FA_PACKED2(fa_page_means), FA_PACKED2(fa_select_pages),
+                      FA_PACKED2(fa_fwd_paged_sparse)};
+
+}  // namespace
+}  // namespace fa
+
+extern "C" void* fa_packed_entry(const char* name) {
+  for (const auto& e : packed_entries)
+    if (name && std::strcmp(e.name, name) == 0) return reinterpret_cast<void*>(e.call);
+  return nullptr;
+}

@@ -195,7 +195,7 @@ def paged_append(query, key, value, k_cache, v_cache, slot_mapping, table, posit
     launch(q, "fa_paged_append", q.dtype, qp, kp, vp, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
            slots.data_ptr(), table.data_ptr(), pos.data_ptr(), _ptr(query_weight), _ptr(key_weight), total, hq, hkv, d,
            pages * page_size, *table.shape, interleaved,
-           query_weight is not None and query_weight.dtype == torch.float32, qs, ks, vs, float(eps))
+           query_weight is not None and query_weight.dtype == torch.float32, qs.at, ks.at, vs.at, float(eps))
     return out
 
 
@@ -302,7 +302,7 @@ def select_pages(query, page_means, block_table, cu_seqlens_q, seqlens_k, *, pag
     out = block_table.new_empty((total, hkv, num_selected))
     launch(q, "fa_select_pages", q.dtype, qp, page_means.data_ptr(), table.data_ptr(), cu.data_ptr(), lens.data_ptr(),
            out.data_ptr(), batch, hq, hkv, d, total, page_means.shape[0], page_size, width, num_selected, sink_pages,
-           local_pages, qs)
+           local_pages, qs.at)
     return out
 
 
@@ -355,5 +355,5 @@ def scaled_dot_product_attention_paged_sparse(query, k_cache, v_cache, block_tab
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     launch(q, "fa_fwd_paged_sparse", q.dtype, qp, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
            table.data_ptr(), cu.data_ptr(), lens.data_ptr(), pages.data_ptr(), batch, hq, hkv, d, total, num_pages,
-           page_size, width, n, float(scale) if scale is not None else d ** -0.5, qs)
+           page_size, width, n, float(scale) if scale is not None else d ** -0.5, qs.at)
     return out

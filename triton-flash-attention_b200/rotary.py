@@ -68,13 +68,13 @@ def launch(tensor: torch.Tensor, what: str, dtype, *args) -> None:
     no type) with ``args`` and the tensor's device's current stream, on that
     device.  (Calls of a few microseconds of GPU time are bound by their host
     side: this asks for no more than it has to.)"""
-    fn = _abi.entry(what, dtype)
+    fn, pack = _abi.packed_entry(what, dtype)
     index = tensor.get_device()
     if torch._C._cuda_getDevice() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(pack(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(pack(*args, torch._C._cuda_getCurrentRawStream(index)))
     if rc:
         _abi.check(rc, what)
 
@@ -210,7 +210,7 @@ def _contiguous_strides(shape):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _contiguous_like(t):
@@ -231,7 +231,8 @@ def _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved)
     _, qop, qos = row_arg(qo)
     _, kop, kos = row_arg(ko)
     launch(q, "fa_qk_norm_rotary", q.dtype, qp, kp, qop, kop, table.data_ptr(), _ptr(positions), _ptr(query_weight),
-           _ptr(key_weight), b, hq, hkv, n, d, max_positions, rd, interleaved, fp32, qs, ks, qos, kos, per_batch, eps)
+           _ptr(key_weight), b, hq, hkv, n, d, max_positions, rd, interleaved, fp32, qs.at, ks.at, qos.at,
+           kos.at, per_batch, eps)
     return qo, ko, q, k, (b, hq, hkv, n, d, max_positions, rd, interleaved, fp32), (qos, kos, per_batch, eps)
 
 
@@ -252,7 +253,7 @@ def _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, 
         part = table.new_empty(ROTARY_PARTIALS * sizes[4])
     launch(q, "fa_qk_norm_rotary_bwd", q.dtype, qp, kp, gqp, gkp, dq.data_ptr(), dk.data_ptr(),
            _ptr(dwq), _ptr(dwk), _ptr(part), table.data_ptr(), _ptr(positions), _ptr(query_weight), _ptr(key_weight),
-           *sizes, qs, ks, gqs, gks, qos, kos, per_batch, eps)
+           *sizes, qs.at, ks.at, gqs.at, gks.at, qos.at, kos.at, per_batch, eps)
     return dq, dk, dwq, dwk
 
 
