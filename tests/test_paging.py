@@ -439,6 +439,31 @@ def test_selection_with_queries_and_means_at_the_edges(what):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group", [1, 5, 8, 9, 17, 40])
+def test_selection_groups_and_scores_in_heaps(group):
+    """Groups on both sides of 8 heads; then a few scores a million times the
+    others', and scores in two heaps, so that nearly all lie close together."""
+    page, n = 16, 1500
+    for d, dt in ((32, F16), (64, BF16), (128, F16)):
+        c = Case([1], [page * n - 3], page, 2 * group, 2, d, dt, group + d, junk=0.0)
+        q, kc, _, table, cu, lens = c.cuda()
+        g = torch.Generator().manual_seed(group * d)
+        means = _randn(g, kc.shape[0], 2, d, dtype=dt).cuda() * 0.125
+        for what in ("plain", "outliers", "heaps"):
+            if what == "outliers":
+                means[:: means.shape[0] // 5] *= 2.0 ** 14
+                means *= 2.0 ** -6
+            elif what == "heaps":
+                means = (means[:1] * 2.0 ** -8).expand(means.shape).clone()
+                means[: means.shape[0] // 2] *= -1.0
+                means[:, :, 0] += (torch.arange(means.shape[0]) % 16 * 2.0 ** -6).to(means)[:, None]
+            for top in (3, 64, 700, n - 1):
+                got = fa.select_pages(q, means, table, cu, lens, page_size=page, num_selected=top)
+                want = orc.select_pages_reference(_f64(q), _f64(means), c.table, c.cu, c.lens, page, top, 1, 1)
+                assert np.array_equal(got.cpu().numpy(), want), (d, what, top)
+
+
+@pytest.mark.gpu
 def test_selection_over_the_widest_table():
     n = 16384
     c = Case([1], [16 * n], 16, 2, 1, 32, F16, 4, junk=0.0)

@@ -43,6 +43,19 @@ __device__ __forceinline__ float to_f32(uint16_t v) {
   return unpack2<DT>(uint32_t(v)).x;
 }
 
+template <int DT>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == 0) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Means of completed pages.
 //
@@ -207,184 +220,146 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
 // block scores its share of the pages into the first block's shared memory,
 // which then finds the top ones.
 //
-// Scoring: a few lanes own a page, 16 columns a lane (8 of D = 32), SEL_PAGES
-// pages at once; asynchronous copies to the lane's own places in shared memory
-// bring the next batch meanwhile.  The group's queries lie in shared memory
-// and are taken SEL_HEADS heads at a time.  Lanes swap halves of their page
-// sums until each holds whole ones.  The sums are fp32, of exact products: 16
-// roundings in a lane and up to 3 between lanes, each at most 2^-24 of the
-// sum of sizes |q| . |k| <= ||q||_1 max |k|.
+// Scoring: matrix instructions, 16 pages a warp as their rows, 8 of the group's
+// heads as columns.  A lane's share of a row are 8 neighbouring columns at a
+// time, straight from global memory to registers (a second set of registers for
+// the pages to come gained nothing); the queries lie in shared memory.  The
+// products are exact and PTX has their sums in at least single precision, so
+// that a score is off by at most 5/4 D 2^-23 of the sum of sizes |q| . |k|,
+// which the same instructions give.
 //
 // Selection: keys are the scores' bits in an order that whole numbers have,
-// neighbouring keys a thread.  T, the kk-th largest, is found two bits a
-// round by block-wide counts of the keys at and above three candidates, and
-// once few keys can still be it, by counting those that go before each of
-// them.  If more than one key lies so near T that its score's roundings may
-// decide, the pages of all such keys are scored again in 64 bits, and T is
-// found again.  The pages above T, and of those at T the first ones, are
-// written in order of their index.
+// neighbouring keys a thread.  T, the kk-th largest, is found by counting the
+// keys in bins of equal width and ranking those of its bin; where scores lie
+// in heaps, two bits a round by counts of the keys at and above three
+// candidates.  If more than one key lies so near T that its score's roundings
+// may decide, the pages of all such keys are scored again in 64 bits.  The
+// pages above T, and of those at T the first ones, are written in order of
+// their index.
 //
-// Bound: issued instructions of the scores, then the latency of the rounds.
-// 64 (token, K/V head) units of 2,048 pages, 4 heads each, D 128: 21 us, of
-// which the scores take 8 and finding T and writing 6 (the means' bytes alone
-// take 5); 128 units of 128 pages: 7.4 us, nearly all of it start and
-// latency.  64-bit sums throughout (64 products a clock and SM, 16
-// conversions) took 15 us for the scores, and larger groups in proportion.
+// Bound: latency.  64 (token, K/V head) units of 2,048 pages, 4 heads each,
+// D 128: 15.5 us, of which 2 go before the first page, 4 for the scores (the
+// means' bytes alone take 5 from HBM, here they lie in L2), 1 to meet, 2.5 for
+// T, 1 for the pages near it and 1 to write; 128 units of 128 pages: 7.2 us.
+// fp32 multiply-adds took 8 us for the scores (they are short of shared memory
+// bandwidth for the queries), 64-bit ones 15, and rounds of two bits alone 5
+// for T.
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
-constexpr int SEL_PAGES = 4;
-constexpr int SEL_HEADS = 4;
+constexpr int SEL_STEP = SEL_WARPS * 16;  // pages of the block's step
 template <int D>
-constexpr int sel_cols() {  // of a lane
-  return D == 32 ? 8 : 16;
-}
-template <int D>
-constexpr int sel_ring() {  // bytes of the two batches
-  return 2 * SEL_PAGES * SEL_THREADS * sel_cols<D>() * 2;
+constexpr int sel_pitch() {  // bytes of a query's row in shared memory: two neighbours on different banks
+  return D == 32 ? 64 : 2 * D + 64;
 }
 
 __device__ __forceinline__ uint32_t order_key(float f) {
   if (f != f) return 0u;  // NaN: behind everything
-  const uint32_t u = __float_as_uint(f);
+  const uint32_t u = __float_as_uint(f + 0.f);  // zeros are equal
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float key_score(uint32_t k) {  // of a key that is not 0
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
+
 // fp32 scores of the block's pn pages, as keys to keys_at.  ids holds their
 // pages and may be where the keys go: a page's key replaces its id, which is
-// read by then.  Returns the largest |k| of the pages this thread has seen.
+// read by then.  Returns the bits of the largest |q| . |k| that this thread has
+// seen (NaN is the largest), 0 only where every k is 0.
 template <int D, int DT>
-__device__ __forceinline__ float score_pages(const SelectArgs& a, const float4* qf, const int* ids, uint32_t ring,
-                                             int h, int G, int pn, uint32_t keys_at) {
-  constexpr int CH = sel_cols<D>() / 8;  // 16-byte chunks of a lane
-  constexpr int LP = D / (8 * CH);       // lanes of a page
-  constexpr int SUBS = SEL_THREADS / LP;
-  constexpr int BATCH = SUBS * SEL_PAGES;  // pages of the block's step
-  constexpr uint32_t PIECE = SEL_THREADS * 16, STAGE = SEL_PAGES * CH * PIECE;
-  const int lane = threadIdx.x & 31;
-  const int l = threadIdx.x % LP;
-  // chunk c of lane l: columns 8 (c LP + l) .. + 7
-  const uint16_t* means = static_cast<const uint16_t*>(a.means) + (long long)h * D + 8 * l;
+__device__ __forceinline__ uint32_t score_pages(const SelectArgs& a, const unsigned char* qs, const int* ids, int h,
+                                                int G, int pn, uint32_t keys_at) {
+  constexpr int CH = D / 32;  // 16-byte chunks of a lane and row
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g8 = lane >> 2, t4 = lane & 3;
+  const uint16_t* means = static_cast<const uint16_t*>(a.means) + (long long)h * D + 8 * t4;
   const long long page_stride = (long long)a.Hkv * D;
-  const uint32_t mine_at = ring + threadIdx.x * 16;
-  auto fetch = [&](int first, uint32_t to) {
-#pragma unroll
-    for (int i = 0; i < SEL_PAGES; ++i) {
-      const int id = first + i < pn ? ids[first + i] : -1;
-      if (id >= 0)
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (i * CH + c) * PIECE),
-                       "l"(means + id * page_stride + c * (8 * LP))
-                       : "memory");
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+  // 16 pages of the warp: rows g8 and g8 + 8 are this lane's, its chunk c of
+  // them columns 32 c + 8 t4 .. + 7
+  struct Pages {
+    uint4 v[2][CH];
+    bool ok[2];
   };
-  int first = (threadIdx.x / LP) * SEL_PAGES;
-  fetch(first, mine_at);
-  uint32_t stage = 0;
-  float top = 0.f;
-  // the trip count is the warp's, for the shuffles
-  for (int base = (threadIdx.x - lane) / LP * SEL_PAGES; base < pn; base += BATCH, first += BATCH) {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    const uint32_t from = mine_at + stage;
-    stage = STAGE - stage;
-    fetch(first + BATCH, mine_at + stage);  // where the batch before was, which this lane has read
-    float best = -INFINITY;
-    bool nan = false;
-    for (int g0 = 0; g0 < G; g0 += SEL_HEADS) {
-      float s[SEL_HEADS][SEL_PAGES], size[SEL_PAGES];
+  auto load = [&](Pages& x, int base) {
 #pragma unroll
-      for (int i = 0; i < SEL_PAGES; ++i) {
-        size[i] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int at = base + g8 + 8 * i;
+      const int id = at < pn ? ids[at] : -1;
+      x.ok[i] = id >= 0;
 #pragma unroll
-        for (int g = 0; g < SEL_HEADS; ++g) s[g][i] = 0.f;
-      }
+      for (int c = 0; c < CH; ++c)
+        x.v[i][c] = id >= 0 ? *reinterpret_cast<const uint4*>(means + id * page_stride + c * 32)
+                            : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  constexpr uint32_t ABS = 0x7fff7fffu;
+  float most = 0.f;
+  uint32_t any = 0u;  // of k, whose products may all be too small to see
+  Pages here;
+  load(here, warp * 16);
+  for (int base = warp * 16; base < pn; base += SEL_STEP) {
+    float best[2] = {-INFINITY, -INFINITY};
+    for (int g0 = 0; g0 < G; g0 += 8) {
+      float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f}, size[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        float k[SEL_PAGES][8];  // what no page was copied to gives a sum that nobody looks at
-#pragma unroll
-        for (int i = 0; i < SEL_PAGES; ++i) {
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(from + (i * CH + c) * PIECE)
-                       : "memory");
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack2<DT>(w[j]);
-            k[i][2 * j] = f.x;
-            k[i][2 * j + 1] = f.y;
-            size[i] = fmax3(size[i], fabsf(f.x), fabsf(f.y));
-          }
-        }
-#pragma unroll
-        for (int g = 0; g < SEL_HEADS; ++g) {
-          const float4 lo = qf[((g0 + g) * (2 * CH) + c * 2) * LP + l];
-          const float4 hi = qf[((g0 + g) * (2 * CH) + c * 2 + 1) * LP + l];
-#pragma unroll
-          for (int i = 0; i < SEL_PAGES; ++i) {
-            float t = s[g][i];
-            t = fmaf(lo.x, k[i][0], t), t = fmaf(lo.y, k[i][1], t);
-            t = fmaf(lo.z, k[i][2], t), t = fmaf(lo.w, k[i][3], t);
-            t = fmaf(hi.x, k[i][4], t), t = fmaf(hi.y, k[i][5], t);
-            t = fmaf(hi.z, k[i][6], t), t = fmaf(hi.w, k[i][7], t);
-            s[g][i] = t;
-          }
-        }
+        // a sum does not care which column is which k: both operands take the
+        // lane's 8 neighbouring ones as two products' shares
+        const uint4 q = *reinterpret_cast<const uint4*>(qs + (g0 + g8) * sel_pitch<D>() + c * 64 + t4 * 16);
+        const uint4 r0 = here.v[0][c], r1 = here.v[1][c];
+        const uint32_t lo[4] = {r0.x, r1.x, r0.y, r1.y}, hi[4] = {r0.z, r1.z, r0.w, r1.w};
+        mma16816<DT>(even, lo, q.x, q.y);
+        mma16816<DT>(odd, hi, q.z, q.w);
+        const uint32_t lo_abs[4] = {lo[0] & ABS, lo[1] & ABS, lo[2] & ABS, lo[3] & ABS};
+        const uint32_t hi_abs[4] = {hi[0] & ABS, hi[1] & ABS, hi[2] & ABS, hi[3] & ABS};
+        mma16816<DT>(size, lo_abs, q.x & ABS, q.y & ABS);
+        mma16816<DT>(size, hi_abs, q.z & ABS, q.w & ABS);
+        any |= lo_abs[0] | lo_abs[1] | lo_abs[2] | lo_abs[3] | hi_abs[0] | hi_abs[1] | hi_abs[2] | hi_abs[3];
       }
-      // 4 page sums over LP lanes: keep 2, then 1, then add it up
-      const bool up0 = (l & (LP / 2)) != 0, up1 = (l & (LP / 4)) != 0;
 #pragma unroll
-      for (int g = 0; g < SEL_HEADS; ++g) {
-        if (g0 + g >= G) break;  // uniform
-        float e0 = up0 ? s[g][2] : s[g][0], e1 = up0 ? s[g][3] : s[g][1];
-        e0 += __shfl_xor_sync(0xffffffffu, up0 ? s[g][0] : s[g][2], LP / 2);
-        e1 += __shfl_xor_sync(0xffffffffu, up0 ? s[g][1] : s[g][3], LP / 2);
-        float e = up1 ? e1 : e0;
-        e += __shfl_xor_sync(0xffffffffu, up1 ? e0 : e1, LP / 4);
-#pragma unroll
-        for (int m = LP / 8; m > 0; m >>= 1) e += __shfl_xor_sync(0xffffffffu, e, m);
-        nan |= e != e;
-        best = fmaxf(best, e);
-      }
-      if (g0 == 0)
-#pragma unroll
-        for (int i = 0; i < SEL_PAGES; ++i)
-          if (first + i < pn && ids[first + i] >= 0) top = fmaxf(top, size[i]);
+      for (int j = 0; j < 4; ++j)  // page g8 + 8 (j / 2), head g0 + 2 t4 + j % 2
+        if (g0 + 2 * t4 + j % 2 < G) best[j / 2] = max_nan(best[j / 2], even[j] + odd[j]);
+      most = max_nan(most, max_nan(max_nan(size[0], size[1]), max_nan(size[2], size[3])));
     }
-    __syncwarp();  // the batch's ids are read
-    // this lane's page of the four
-    const int mine = first + ((l & (LP / 2)) ? 2 : 0) + ((l & (LP / 4)) ? 1 : 0);
-    if ((l & (LP / 4 - 1)) == 0 && mine < pn)
-      st_cluster_u32(keys_at + 4u * uint32_t(mine), ids[mine] < 0 || nan ? 0u : order_key(best));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      best[i] = max_nan(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
+      best[i] = max_nan(best[i], __shfl_xor_sync(0xffffffffu, best[i], 2));
+    }
+    const int mine = base + g8 + 8 * t4;  // of lanes t4 = 0 and 1
+    const bool ok = t4 ? here.ok[1] : here.ok[0];
+    load(here, base + SEL_STEP);
+    __syncwarp();  // the step's ids are read
+    if (t4 < 2 && mine < pn)
+      st_cluster_u32(keys_at + 4u * uint32_t(mine), ok ? order_key(t4 ? best[1] : best[0]) : 0u);
   }
-  return top;
+  return max(__float_as_uint(most) & 0x7fffffffu, any != 0u ? 1u : 0u);
 }
 
 // The score of page `id` by its definition: 64-bit sums, rounded to fp32.  One
 // warp; a lane's D / 32 neighbouring columns against the queries in shared
 // memory, which hold the operands exactly.
 template <int D, int DT>
-__device__ __forceinline__ uint32_t exact_key(const SelectArgs& a, const float4* qf, int h, int G, int id) {
-  constexpr int CH = sel_cols<D>() / 8, LP = D / (8 * CH);
+__device__ __forceinline__ uint32_t exact_key(const SelectArgs& a, const unsigned char* qs, int h, int G, int id) {
   constexpr int N = D / 32;
   const int d0 = (threadIdx.x & 31) * N;
   const uint16_t* k = static_cast<const uint16_t*>(a.means) + ((long long)id * a.Hkv + h) * D + d0;
   double kd[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) kd[i] = double(to_f32<DT>(k[i]));
-  // where columns d0 .. d0 + N - 1 of head 0 lie in qf (N divides 4)
-  const float* q = reinterpret_cast<const float*>(qf + (d0 / (8 * LP) * 2 + d0 / 4 % 2) * LP + d0 / 8 % LP) + d0 % 4;
   float best = -INFINITY;
   bool nan = false;
 #pragma unroll 4
   for (int g = 0; g < G; ++g) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(qs + g * sel_pitch<D>()) + d0;
     double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s = fma(double(q[g * D + i]), kd[i], s);
+    for (int i = 0; i < N; ++i) s = fma(double(to_f32<DT>(q[i])), kd[i], s);
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
     const float f = __double2float_rn(s);
@@ -401,6 +376,7 @@ struct SelectShared {
   int pages[SEL_THREADS];
   uint32_t found;
   int listed;
+  int bin, above, active;
 };
 
 // The rank-th largest (from 1) of n <= SEL_THREADS values; v has zeros up to a
@@ -462,23 +438,70 @@ __device__ __forceinline__ uint2 block_counts(SelectShared& sh, int turn, uint32
   return make_uint2(x, y);
 }
 
+// The rank-th largest of the n <= SEL_THREADS held keys that `in` picks.  All
+// threads.
+template <int E, class In>
+__device__ __forceinline__ uint32_t ranked_of(SelectShared& sh, const Held<E>& held, int n, int rank, In in) {
+  if (threadIdx.x == 0) sh.listed = 0;
+  sh.list[threadIdx.x] = 0u;
+  __syncthreads();
+  held.each([&](int, uint32_t k) {
+    if (in(k)) sh.list[atomicAdd(&sh.listed, 1)] = k;
+  });
+  __syncthreads();
+  return ranked(sh, sh.list, n, rank);
+}
+
 // The kk-th largest of the M keys (below 2^16 of them).
 template <int E>
 __device__ __forceinline__ uint32_t kth_largest(SelectShared& sh, const Held<E>& held, int M, int kk) {
+  // SEL_THREADS bins of equal width between the smallest and the largest
+  // score: a larger score's bin is never below a smaller one's, whatever the
+  // roundings, so a count of each finds T's, and its few keys are ranked
+  uint32_t lo = 0xffffffffu, hi = 0u;
+  held.each([&](int, uint32_t k) { lo = k != 0u ? min(lo, k) : lo, hi = max(hi, k); });
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) sh.counts[0][warp] = make_uint2(lo, hi);
+  sh.list[threadIdx.x] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < SEL_WARPS; ++w) lo = min(lo, sh.counts[0][w].x), hi = max(hi, sh.counts[0][w].y);
+  if (lo < hi && fabsf(key_score(lo)) < INFINITY && fabsf(key_score(hi)) < INFINITY) {  // uniform
+    const float low = key_score(lo), scale = (SEL_THREADS - 0.5f) / (key_score(hi) - low);
+    auto bin_of = [&](uint32_t k) {
+      return k == 0u ? 0 : min(SEL_THREADS - 1, int((key_score(k) - low) * scale));
+    };
+    held.each([&](int, uint32_t k) { atomicAdd(&sh.list[bin_of(k)], 1u); });
+    __syncthreads();
+    const int bin = SEL_THREADS - 1 - int(threadIdx.x);  // from the top
+    const int n = int(sh.list[bin]);
+    int sum = n;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, m);
+      if (lane >= m) sum += x;
+    }
+    if (lane == 31) sh.counts[1][warp].x = uint32_t(sum);
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SEL_WARPS; ++w) sum += w < warp ? int(sh.counts[1][w].x) : 0;
+    if (sum - n < kk && kk <= sum) sh.bin = bin, sh.above = sum - n, sh.active = n;
+    __syncthreads();
+    if (sh.active <= SEL_THREADS) {
+      const int mine = sh.bin;
+      return ranked_of(sh, held, sh.active, kk - sh.above, [&](uint32_t k) { return bin_of(k) == mine; });
+    }
+  }
+  // scores that lie in heaps: two bits of T a round
   uint32_t T = 0;
   int above = 0, active = M;  // keys above T's range, keys in it
 #pragma unroll 1
   for (int bit = 30; bit >= 0; bit -= 2) {
     if (bit <= 20 && active <= SEL_THREADS) {  // few keys agree with T so far
       const uint32_t low = bit + 1 >= 31 ? 0xffffffffu : (4u << bit) - 1u;
-      if (threadIdx.x == 0) sh.listed = 0;
-      sh.list[threadIdx.x] = 0u;
-      __syncthreads();
-      held.each([&](int, uint32_t k) {
-        if ((k & ~low) == T) sh.list[atomicAdd(&sh.listed, 1)] = k;
-      });
-      __syncthreads();
-      return ranked(sh, sh.list, active, kk - above);
+      return ranked_of(sh, held, active, kk - above, [&](uint32_t k) { return (k & ~low) == T; });
     }
     const uint32_t t1 = T | (1u << bit), t2 = T | (2u << bit), t3 = T | (3u << bit);
     uint32_t c12 = 0, c3 = 0;
@@ -586,35 +609,28 @@ template <int D, int DT>
 __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const __grid_constant__ SelectArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ SelectShared sh;
-  __shared__ uint32_t q_size, k_size, k_sizes[MAX_CLUSTER];  // ||q||_1; max |k| of the block; of all blocks
-  constexpr int CH = sel_cols<D>() / 8, LP = D / (8 * CH);
+  __shared__ uint32_t size, sizes[MAX_CLUSTER];  // largest |q| . |k| of the block; of all blocks
+  constexpr int PITCH = sel_pitch<D>();
   const int S = a.cluster;
   const int rank = S > 1 ? int(cluster_rank()) : 0;
   const int unit = blockIdx.x / S;
   const int t = unit / a.Hkv, h = unit - t * a.Hkv;
   const int G = a.Hq / a.Hkv;
   const int lane = threadIdx.x & 31;
-  // the group's queries in fp32, [head][2 CH][LP] fours of columns, zeros up to
-  // a whole SEL_HEADS; then the ring; then page ids and keys
-  const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
-  float4* qf = reinterpret_cast<float4*>(smem);
-  const uint32_t ring = smem_u32(smem + size_t(G4) * D * 4);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(smem + size_t(G4) * D * 4 + sel_ring<D>());
+  // the group's queries, zeros up to a whole 8 of them; then page ids and keys
+  const int G8 = (G + 7) / 8 * 8;
+  unsigned char* qs = smem;
+  uint32_t* keys = reinterpret_cast<uint32_t*>(smem + size_t(G8) * PITCH);
   int* ids = reinterpret_cast<int*>(keys);  // until their scores are known
-  if (threadIdx.x == 0) q_size = k_size = 0u;
+  if (threadIdx.x == 0) size = 0u;
   let_next_begin();
   begin_after_previous();
 
   const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + (long long)h * G * a.q_sh;
-  for (int i = threadIdx.x; i < G4 * D / 4; i += SEL_THREADS) {
-    const int g = i / (D / 4), d = i % (D / 4) * 4;  // columns d .. d + 3: chunk, half and lane
-    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (g < G) {
-      const uint2 w = *(reinterpret_cast<const uint2*>(q + g * a.q_sh + d));
-      const float2 x = unpack2<DT>(w.x), y = unpack2<DT>(w.y);
-      f = make_float4(x.x, x.y, y.x, y.y);
-    }
-    qf[(g * (2 * CH) + d / (8 * LP) * 2 + d / 4 % 2) * LP + d / 8 % LP] = f;
+  for (int i = threadIdx.x; i < G8 * (D / 8); i += SEL_THREADS) {
+    const int g = i / (D / 8), d = i % (D / 8) * 8;
+    *reinterpret_cast<uint4*>(qs + g * PITCH + d * 2) =
+        g < G ? *reinterpret_cast<const uint4*>(q + g * a.q_sh + d) : make_uint4(0u, 0u, 0u, 0u);
   }
   const RowPlace row = place_row(a.cu, a.seqlens, a.B, t, a.width << a.page_log2, a.status);
   int* out = a.out + (long long)unit * a.top;
@@ -645,24 +661,14 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   }
   if (S > 1) cluster_sync();  // and the first block has begun, so that its shared memory may be written
   else __syncthreads();
-  if (rank == 0)  // as bits: of sizes, these have the floats' order, and NaN is the largest
-    for (int g = threadIdx.x >> 5; g < G; g += SEL_WARPS) {
-      const float* row_of = reinterpret_cast<const float*>(qf + g * (D / 4));
-      float s = 0.f;
-#pragma unroll
-      for (int d = 0; d < D; d += 32) s += fabsf(row_of[d + lane]);
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-      if (lane == 0) atomicMax(&q_size, __float_as_uint(s) & 0x7fffffffu);
-    }
   const uint32_t keys0 = smem_u32(keys) + 4u * uint32_t(p0);
-  const float top = score_pages<D, DT>(a, qf, ids, ring, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
-  const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-  if (lane == 0) atomicMax(&k_size, top_bits);
+  const uint32_t top = score_pages<D, DT>(a, qs, ids, h, G, pn, S > 1 ? cluster_map(keys0, 0) : keys0);
+  const uint32_t top_bits = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) atomicMax(&size, top_bits);  // sizes' bits have their order
   __syncthreads();
   if (threadIdx.x == 0) {
-    const uint32_t to = smem_u32(k_sizes + rank);
-    st_cluster_u32(S > 1 ? cluster_map(to, 0) : to, k_size);
+    const uint32_t to = smem_u32(sizes + rank);
+    st_cluster_u32(S > 1 ? cluster_map(to, 0) : to, size);
   }
   if (threadIdx.x < 4 && rank == 0 && M + int(threadIdx.x) < (M + 3) / 4 * 4) keys[M + threadIdx.x] = 0u;
   if (S > 1) {
@@ -671,15 +677,20 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   } else {
     __syncthreads();
   }
-  uint32_t size = 0u;
-  for (int i = 0; i < S; ++i) size = max(size, k_sizes[i]);
-  // 19 roundings of a score's sum and the one of its definition, 2^-24 of the
-  // sum of sizes each (and 2^-150 below the normal numbers), rounded up
-  const float sizes = __uint_as_float(q_size) * __uint_as_float(size);
-  const float slack = q_size == 0u || size == 0u ? 0.f : sizes * (24.f / 16777216.f) + 1e-43f;
+  uint32_t bits = 0u;
+  for (int i = 0; i < S; ++i) bits = max(bits, sizes[i]);
+  // D products and D / 16 accumulators are added with at least single
+  // precision, in whatever order and rounding: 2^-23 of the sum of sizes each,
+  // or 2^-126 below the normal numbers; two roundings more join the halves and
+  // are the definition's, and the sum of sizes is as inexact.  5 D / 4 + 1
+  // covers them.  Near the end of the range no bound
+  const float most = __uint_as_float(bits);
+  const float slack = bits == 0u     ? 0.f  // as every k and score is
+                      : most < 1e38f ? most * ((5 * D / 4 + 1) / 8388608.f) + 2e-36f
+                                     : INFINITY;
   auto rescore = [&](int p) {
     const int id = pages[p];
-    return id >= 0 && id < a.num_pages ? exact_key<D, DT>(a, qf, h, G, id) : 0u;
+    return id >= 0 && id < a.num_pages ? exact_key<D, DT>(a, qs, h, G, id) : 0u;
   };
   out += a.sink;
   if (M <= SEL_THREADS) write_top<1>(sh, keys, M, kk, a.sink, out, slack, rescore);
@@ -754,19 +765,6 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-template <int DT>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (DT == 0) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-}
-
 // Byte offset of 16-byte chunk c (8 columns) of row r of 16 rows that start at
 // a multiple of 8 rows of a piece, as the TMA's swizzle leaves it.  box: bytes
 // between the first 64 columns and the last 64 of a piece.
@@ -1120,8 +1118,7 @@ template <int D, int DT>
 int run_select(const SelectArgs& a) {
   auto* kernel = fa_select_pages_kernel<D, DT>;
   const int G = a.Hq / a.Hkv;
-  const int G4 = (G + SEL_HEADS - 1) / SEL_HEADS * SEL_HEADS;
-  const size_t smem = size_t(G4) * D * 4 + sel_ring<D>() + (size_t(a.width) * 4 + 15) / 16 * 16;
+  const size_t smem = size_t((G + 7) / 8 * 8) * sel_pitch<D>() + (size_t(a.width) * 4 + 15) / 16 * 16;
   constexpr size_t most = size_t(220) << 10;  // of an SM's 227 KB, the static part left out
   if (smem > most) return FA_ERR_BAD_SHAPE;
   if (int rc = allow_smem<fa_select_pages_kernel<D, DT>>(int(most))) return rc;
