@@ -798,3 +798,89 @@ def test_packed_entry_of_another_name():
         _abi.packed_entry("fa_fwd", torch.float16)
     s = _abi.strides_of((1, 2, 3))
     assert s.at == ctypes.addressof(s) and list(s) == [1, 2, 3]
+
+
+# ---------------------------------------------------------------- weights, lengths, refused requests
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [3, 4, 5])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+def test_sparse_attention_keeps_its_weights_in_more_bits_than_the_operands(dt, d, group):
+    """Queries and keys of -1, 0 and 1: scores are exact in any order.  With A
+    the attention of |v| and up to 64 keys, a weight is off by the scale's,
+    the product's and the difference's roundings (3 x 2^-24 of at most 8, in
+    base 2) and the exponential's 2^-22: 2^-20; once in the sum and once in
+    the product, which adds 17 values a time at 2^-23 and joins 4 warps:
+    below 2^-17 A in all.  To it come what is lost of a weight held as two
+    numbers of the operand type, the first cut off and the second rounded:
+    2^-10 2^-11 (fp16) or 2^-7 2^-8 (bf16), and the result's own rounding.
+    Weights rounded once to the operand type would be off by 2^-11 or 2^-8."""
+    rng = np.random.default_rng(d)
+    lens = [2, 3, 5, 9, 16, 17, 33, 64]
+    c = Case([1] * len(lens), lens, 16, 2 * group, 2, d, dt, d, junk=0.0)
+    c.q[:] = torch.from_numpy(rng.integers(-1, 2, c.q.shape)).to(dt)
+    c.kc[:] = torch.from_numpy(rng.integers(-1, 2, c.kc.shape)).to(dt)
+    pages = np.tile(np.arange(4, dtype=np.int32), (len(lens), 2, 1))
+    q, kc, vc, table, cu, ln = c.cuda()
+    scale = 0.11 * (32 / d) ** 0.5
+    got = fa.scaled_dot_product_attention_paged_sparse(q, kc, vc, table, cu, ln, _i32(pages).cuda(), scale=scale,
+                                                       enable_gqa=True)
+    o, a = orc.sparse_paged_reference(*c.refs(), pages, scale)
+    split = 2.0 ** -21 if dt == F16 else 2.0 ** -15
+    tol = (torch.finfo(dt).eps / 2 * np.abs(o) * 1.001 + (2.0 ** -17 + split) * a + (2.0 ** -25 if dt == F16 else 0.0))
+    diff = np.abs(_f64(got) - o)
+    assert (diff <= tol).all(), (float((diff - tol).max()), int((diff > tol).sum()))
+
+
+@pytest.mark.gpu
+def test_fp16_weights_far_below_the_largest_are_not_lost():
+    """One key of every 16 has weight 1 and no value, the others 2^-19.84 each
+    and large values.  2^-19.84 by itself lies between fp16's subnormal steps:
+    rounded to one of them it would be off by half a percent."""
+    n = 1001
+    c = Case([1], [n], 16, 1, 1, 64, F16, 41, junk=0.0)
+    c.q[:], c.kc[:], c.vc[:] = 0, 0, 0
+    c.q[0, 0, 0] = 1.0
+    j = np.arange(n)
+    rows = torch.from_numpy(c.table[0, j // 16].astype(np.int64) * 16 + j % 16)
+    c.kc.view(-1, 64)[rows, 0] = -13.75
+    c.vc.view(-1, 64)[rows] = 1000.0
+    c.kc.view(-1, 64)[rows[::16]] = 0.0
+    c.vc.view(-1, 64)[rows[::16]] = 0.0
+    pages = np.arange(63, dtype=np.int32)[None, None]
+    q, kc, vc, table, cu, ln = c.cuda()
+    got = fa.scaled_dot_product_attention_paged_sparse(q, kc, vc, table, cu, ln, _i32(pages).cuda(), scale=1.0)
+    o, _ = orc.sparse_paged_reference(*c.refs(), pages, 1.0)
+    # the result's rounding; the score in base 2 is off by 2 x 2^-24 of 20, the sums by 2^-23 of some hundred terms
+    assert (np.abs(_f64(got) - o) <= (2.0 ** -11 + 2.0 ** -14) * o).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [3, 6])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dt", [F16, BF16], ids=str)
+def test_infinite_values_stay_infinite(dt, d, group):
+    """Values of infinity under weights of 1, of few bits and of many; both
+    signs in one column are no number.  The other columns are as without."""
+    c = Case([1, 1], [40, 7], 16, group, 1, d, dt, d + 1, junk=0.0)
+    c.q[:], c.kc[:] = 0, 0
+    c.q[:, :, 0] = 1.0
+    at = c.table[0, np.arange(40) // 16].astype(np.int64) * 16 + np.arange(40) % 16
+    k, v = c.kc.view(-1, d), c.vc.view(-1, d)
+    # weights (scale ln 2): keys 0 and 5 have 1, 9 has 1/2, 20 has 2^-3.25, 33 has 2^-14.5
+    k[torch.from_numpy(at), 0] = -3.0
+    for j, e in ((0, 0.0), (5, 0.0), (9, -1.0), (20, -3.25), (33, -14.5)):
+        k[at[j], 0] = e
+    pages = np.tile(np.arange(3, dtype=np.int32), (2, 1, 1))
+    want, _ = orc.sparse_paged_reference(*c.refs(), pages, float(np.log(2.0)))
+    inf = float("inf")
+    for j, col, x in ((0, 1, inf), (9, 2, -inf), (20, 3, inf), (33, 4, inf), (5, 5, inf), (20, 5, -inf), (33, 6, -inf)):
+        v[at[j], col] = x
+    q, kc, vc, table, cu, lens = c.cuda()
+    got = fa.scaled_dot_product_attention_paged_sparse(q, kc, vc, table, cu, lens, _i32(pages).cuda(),
+                                                       scale=float(np.log(2.0)), enable_gqa=True)[0]
+    for col, x in ((1, inf), (2, -inf), (3, inf), (4, inf), (6, -inf)):
+        assert (got[:, col] == x).all(), col
+    assert got[:, 5].isnan().all()
+    u = torch.finfo(dt).eps / 2
+    assert (np.abs(_f64(got)[:, 7:] - want[0][:, 7:]) <= u * np.abs(want[0][:, 7:]) * 1.001 + 2.0 ** -13).all()

@@ -713,8 +713,8 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
 //
 // Both products are m16n8k16 matrix instructions.  S = Q K^T has the heads as
 // rows (8 of 16) and the keys as columns; what a thread then holds of the
-// weights is just what it has to hold of P^T as the second operand of
-// O^T = V^T P^T, whose rows are 16 of the D columns and whose columns are the
+// weights is just what it has to hold of P^T, as two numbers of the operand type
+// a weight, as the second operand of O^T = V^T P^T, whose rows are 16 of the D columns and whose columns are the
 // 8 heads.  That takes half of the instructions and accumulators of O = P V
 // with 16 rows of heads.
 //
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
 // be 15 of 16 parts empty for a group's heads.  16 sequences x 8 K/V heads x
 // 2,048 keys at D 128: 27 us (134 MB: 20.5 us of HBM), of which 4 go before the
 // first keys arrive and 2.5 behind the last; without the products it takes 24.
-// 2 sequences x 8 x 8,192 keys in pages of 16: 19 us (10.3 of HBM).
+// 2 sequences x 8 x 8,192 keys in pages of 16: 19.6 us (10.3 of HBM).
 constexpr int DEC_WARPS = 4;
 constexpr int DEC_THREADS = (DEC_WARPS + 2) * 32;
 constexpr int DEC_TILE = 64;
@@ -774,6 +774,34 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c, uint32_t box) {
   else return (D == 128 && (c & 8) ? box : 0u) + uint32_t(r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// Two weights, none negative, as numbers of the operand type whose sum they
+// are: hi, the largest below the weight, and lo, the rest.  A weight is then
+// off by lo's rounding, half a step of a number below 2^-7 (bf16) or 2^-10
+// (fp16) of it: 2^-15 or 2^-21.  Rounded once it would be 2^-8 or 2^-11, which
+// showed in the result (error of 16 x 2,048 keys in fp16 2.5e-4 of the result,
+// 2.1e-4 with fp32 weights and with these).  Neither part of a weight is
+// negative or zero, so that a value of infinity gives infinity.
+template <int DT>
+__device__ __forceinline__ void split_weights(float w0, float w1, uint32_t& hi, uint32_t& lo) {
+  // the fp32 numbers before them, cut off
+  const uint32_t b0 = max(__float_as_uint(w0), 1u) - 1u, b1 = max(__float_as_uint(w1), 1u) - 1u;
+  float2 h;
+  if constexpr (DT == DT_F16) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(__uint_as_float(b1)), "f"(__uint_as_float(b0)));
+    h = unpack2<DT>(hi);
+  } else {
+    hi = __byte_perm(b0, b1, 0x7632);
+    h = make_float2(__uint_as_float(b0 & 0xffff0000u), __uint_as_float(b1 & 0xffff0000u));
+  }
+  lo = pack2<DT>(w0 - h.x, w1 - h.y);
+}
+// The weights' factor, which the result loses with their sum: fp16 has no
+// exponents for weights below 2^-24 of the largest.
+template <int DT>
+constexpr float weight_lift() {
+  return DT == DT_F16 ? 16384.f : 1.f;
+}
+
 // Blocks a SM, with what dec_stages takes of shared memory.  D 64, 4 drafted
 // tokens of 31 sequences (496 units): 4 blocks x 3 stages hold all units at
 // once, 27 us; 3 x 3 35, 2 x 6 33, in two waves.  D 128, 2 blocks: 3 stages
@@ -806,6 +834,11 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
   const int th = unit / hblocks;
   const int t = th / a.Hkv, h = th - t * a.Hkv;
   const int rows = min(8, G - hb * 8);
+  // Up to 4 heads leave columns 4 to 7 of the second product free: those take
+  // the weights' second parts (their heads' queries are there twice), one
+  // product instead of two.  At 4 heads and D 128, 16 x 2,048 keys 27.0
+  // us against 27.1, 2 x 8,192 keys 19.6 against 20.1.
+  const bool few = rows <= 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int PR = min(1 << a.page_log2, DEC_TILE);  // rows of a piece
 
@@ -916,13 +949,14 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
     // ---- consumers: keys 16 warp .. of each tile ----
     uint32_t qf[KS][2];  // head g8's columns 16 ks + 2 t4 and + 8
     {
-      const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + ((long long)h * G + hb * 8 + g8) * a.q_sh;
+      const int head = few ? g8 & 3 : g8;
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + t * a.q_st + ((long long)h * G + hb * 8 + head) * a.q_sh;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           qf[ks][j] =
-              g8 < rows && pos >= 0 ? *(reinterpret_cast<const uint32_t*>(q + ks * 16 + j * 8 + t4 * 2)) : 0u;
+              head < rows && pos >= 0 ? *(reinterpret_cast<const uint32_t*>(q + ks * 16 + j * 8 + t4 * 2)) : 0u;
     }
     // the warp's 16 rows: their piece, and their place in it
     const uint32_t box = uint32_t(PR) * 128u;
@@ -989,14 +1023,18 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          w[j] = ex2(w[j] - ref);
+          w[j] = ex2(w[j] - ref) * weight_lift<DT>();
           l += w[j];
         }
-        // the weights as the second product's operand: rounded to its type,
-        // at most half a step of a value in [0, 1]
-        const uint32_t p0 = pack2<DT>(w[0], w[1]), p1 = pack2<DT>(w[2], w[3]);
+        uint32_t p0, p1, r0, r1;  // the second product's operand, twice
+        split_weights<DT>(w[0], w[1], p0, r0);
+        split_weights<DT>(w[2], w[3], p1, r1);
+        if (few && g8 >= 4) p0 = r0, p1 = r1;
 #pragma unroll
         for (int np = 0; np < D / 16; ++np) mma16816<DT>(o[np], vf[np], p0, p1);
+        if (!few)
+#pragma unroll
+          for (int np = 0; np < D / 16; ++np) mma16816<DT>(o[np], vf[np], r0, r1);
         if (seen < 16) fence_proxy_async_smem();  // zeros written before the next copy lands there
       }
       __syncwarp();
@@ -1037,7 +1075,11 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
     for (int w = 0; w < DEC_WARPS; ++w) {
       const float x = ex2(ml_warp[w * 16 + r] - ref);
       ll += x * ml_warp[w * 16 + 8 + r];
-      const float4 v = *reinterpret_cast<const float4*>(o_warp + (w * 8 + r) * OP + c);
+      float4 v = *reinterpret_cast<const float4*>(o_warp + (w * 8 + r) * OP + c);
+      if (few) {  // the second parts' product
+        const float4 u = *reinterpret_cast<const float4*>(o_warp + (w * 8 + r + 4) * OP + c);
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+      }
       acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
     }
     *reinterpret_cast<float4*>(o_block + r * OP + c) = acc;
