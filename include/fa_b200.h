@@ -563,7 +563,9 @@ FA_API int fa_extend_block_table(int* block_table, const int* cached, const int*
  *
  * fa_page_means: the mean key, summed in 64 bits, of every page that the
  * step's tokens completed, to page_means (num_pages, Hkv, D) in the cache's
- * type; other rows stay as they are. */
+ * type; other rows stay as they are.  A sequence with more keys than its row of
+ * block_table holds has none written, and the device status is
+ * FA_ERR_BAD_INDEX (in the other two calls it has no pages and zeros). */
 FA_API int fa_page_means(const void* k_cache, void* page_means, const int* block_table, const int*
                         cu_seqlens_q, const int* seqlens_k, int B, int Hkv, int D, int num_pages, int
                         page_size, int max_pages_per_seq, int total_q, void* stream);

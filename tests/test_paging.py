@@ -884,3 +884,23 @@ def test_infinite_values_stay_infinite(dt, d, group):
     assert got[:, 5].isnan().all()
     u = torch.finfo(dt).eps / 2
     assert (np.abs(_f64(got)[:, 7:] - want[0][:, 7:]) <= u * np.abs(want[0][:, 7:]) * 1.001 + 2.0 ** -13).all()
+
+
+@pytest.mark.gpu
+def test_page_means_refuse_a_sequence_longer_than_its_table_row():
+    """As the selection and the attention do: nothing of it is written, the
+    device status is set, and the other sequences' means are made."""
+    c = Case([40, 100], [200, 100], 16, 4, 2, 64, F16, 15)
+    _, kc, _, table, _, _ = c.cuda()
+    start = torch.full((kc.shape[0], 2, 64), 0.5, dtype=F16)
+    width = table.shape[1]
+    for nk in (width * 16 + 1, width * 16 + 39, 100_000, 2 ** 31 - 1):
+        means = start.clone().cuda()
+        fa.update_page_means(kc, means, table, _i32(c.cu).cuda(), _i32([nk, 100]).cuda())
+        want = orc.page_means_reference(_f64(c.kc), _f64(start), c.table[1:], [0, 100], [100])
+        assert torch.equal(means.cpu(), _rounded_mean(want, F16)), nk
+        assert _abi.device_status(reset=True) & 0xff == _abi.FA_ERR_BAD_INDEX, nk
+    # as long as its row, and one that brings no rows this step
+    means = start.clone().cuda()
+    fa.update_page_means(kc, means, table.clamp(min=0), _i32([0, 0, 100]).cuda(), _i32([100_000, 100]).cuda())
+    assert _abi.device_status(reset=True) == 0

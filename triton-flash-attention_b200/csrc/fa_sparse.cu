@@ -102,9 +102,13 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
     }
     const int nq = q1 - q0;
     if (nq <= 0 || nk <= 0) continue;
+    if (nk > (a.width << a.page_log2)) {  // its table row cannot hold it: refused whole, as place_row does
+      if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+      continue;
+    }
     const int from = max(nk - nq, 0) >> a.page_log2;
     const long long p = (long long)from + (u - ((q0 >> a.page_log2) + b));
-    if (p < from || p >= (nk >> a.page_log2) || p >= a.width) continue;  // uniform in the block
+    if (p < from || p >= (nk >> a.page_log2)) continue;  // uniform in the block
     const int id = a.table[(long long)b * a.width + p];
     if (id < 0 || id >= a.num_pages) {
       if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);

@@ -221,7 +221,9 @@ def update_page_means(k_cache, page_means, block_table, cu_seqlens_q, seqlens_k,
     ``scaled_dot_product_attention_paged``: the rows of a sequence are its
     last keys.  ``total_q``: rows of the packed batch when the caller has it;
     None takes room for a step that fills the table.  Means are summed in 64
-    bits and do not depend on the order of the sum."""
+    bits and do not depend on the order of the sum.  A sequence with more keys
+    than its row of ``block_table`` holds is refused on the GPU: no mean of it
+    is written."""
     if not isinstance(k_cache, torch.Tensor):
         raise TypeError("k_cache must be a torch.Tensor")
     num_pages, page_size, hkv, d = _check_cache("k_cache", k_cache, k_cache.dtype, k_cache.device)
