@@ -519,8 +519,9 @@ FA_API int fa_qk_norm_rotary_bwd_bf16(const void* q, const void* k, const void* 
  * Hkv, D) by element strides {batch (unused), head, row}; q is written to
  * q_out (total, Hq, D), contiguous, the prepared k and v as it is to row
  * slots[t] of the (num_slots, Hkv, D) caches, contiguous.  slots[t] < 0:
- * nothing of token t is written to the caches; slots[t] >= num_slots: the
- * same, and the device status is FA_ERR_BAD_INDEX.  Slots of one call must
+ * nothing of token t is written to the caches, and its position may lie outside
+ * the table (NaN in q_out, no error); slots[t] >= num_slots: nothing either, and
+ * the device status is FA_ERR_BAD_INDEX.  Slots of one call must
  * differ from each other.  positions is an int32 array of total. */
 FA_API int fa_paged_append(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void*
                         v_cache, const int* slots, const float* table, const int* positions, const void*

@@ -904,3 +904,25 @@ def test_page_means_refuse_a_sequence_longer_than_its_table_row():
     means = start.clone().cuda()
     fa.update_page_means(kc, means, table.clamp(min=0), _i32([0, 0, 100]).cuda(), _i32([100_000, 100]).cuda())
     assert _abi.device_status(reset=True) == 0
+
+
+@pytest.mark.gpu
+def test_a_token_without_a_slot_may_be_at_any_position():
+    """A request that does not fit has slots of -1 and positions that may lie
+    behind the angles' table: no error, and nothing is written for it.  A
+    token with a slot and such a position is one."""
+    g = torch.Generator().manual_seed(3)
+    x = _randn(g, 6, 8, 64, dtype=F16).cuda()
+    kc, vc = (torch.full((3, 16, 2, 64), float("nan"), dtype=F16, device="cuda") for _ in range(2))
+    table = fa.rotary_table(8, 64).cuda()
+    pos, slots = _i32([0, 8, -1, 2 ** 31 - 1, 7, 3]).cuda(), _i32([5, -1, -1, -1, -1, 20]).cuda()
+    q = fa.paged_append(x[:, :4], x[:, 4:6], x[:, 6:], kc, vc, slots, table, pos)
+    assert _abi.device_status(reset=True) == 0
+    assert q[[0, 4, 5]].isfinite().all()
+    assert torch.equal(vc.view(-1, 2, 64)[[5, 20]], x[[0, 5], 6:])
+    left = torch.ones(48, dtype=torch.bool)
+    left[[5, 20]] = False
+    assert kc.view(-1, 2, 64)[left.cuda()].isnan().all() and vc.view(-1, 2, 64)[left.cuda()].isnan().all()
+    slots[2] = 7
+    fa.paged_append(x[:, :4], x[:, 4:6], x[:, 6:], kc, vc, slots, table, pos)
+    assert _abi.device_status(reset=True) & 0xff == _abi.FA_ERR_BAD_INDEX

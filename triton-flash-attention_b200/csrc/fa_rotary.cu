@@ -162,11 +162,13 @@ __device__ __forceinline__ float group_sum(float v) {
 __device__ __forceinline__ int raw_pos(const RotaryArgs& a, int b, int n) {
   return a.pos ? a.pos[(long long)b * a.pos_sb + n] : n;
 }
-// The position, or -1 (with the device status word set) when it has no row in
-// the table.
-__device__ __forceinline__ int checked_pos(const RotaryArgs& a, int p) {
+// The position, or -1 when it has no row in the table: an error (the device
+// status word is set), but for an appended token without a slot, as those of a
+// request are that found no room.
+template <bool APPEND>
+__device__ __forceinline__ int checked_pos(const RotaryArgs& a, int p, int n) {
   if (p >= 0 && p < a.max_pos) return p;
-  if (a.status) atomicCAS(a.status, 0, (FA_SITE_POSITION << 8) | FA_ERR_BAD_INDEX);
+  if (a.status && !(APPEND && a.slots[n] < 0)) atomicCAS(a.status, 0, (FA_SITE_POSITION << 8) | FA_ERR_BAD_INDEX);
   return -1;
 }
 constexpr int THREADS = 128;
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(cons
     if (to_come > 0) {
       copy_run<C>(to + lane * R::RUN, src.p, valid);
       copy_run<C>(to + (32 + lane) * R::RUN, src.p + ab, valid);
-      if (!APPEND || kind != 2) fetch_angles<D, C>(a, to + R::ANGLES, checked_pos(a, pos), lane);
+      if (!APPEND || kind != 2) fetch_angles<D, C>(a, to + R::ANGLES, checked_pos<APPEND>(a, pos, src_n), lane);
       const bool ends = src_n + 1 == a.N;
       src.next(ends);
       src_n = ends ? 0 : src_n + 1;
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) fa_rotary_bwd_kernel(cons
         copy_run<C>(to + (32 + lane) * R::RUN, gp.p + ab, valid);
         copy_run<C>(to + (64 + lane) * R::RUN, xp.p, NORM && valid);
         copy_run<C>(to + (96 + lane) * R::RUN, xp.p + ab, NORM && valid);
-        fetch_angles<D, C>(a, to + R::ANGLES, checked_pos(a, pos), lane);
+        fetch_angles<D, C>(a, to + R::ANGLES, checked_pos<false>(a, pos, src_n), lane);
         const bool ends = src_n + 1 == a.N;
         gp.next(ends);
         xp.next(ends);

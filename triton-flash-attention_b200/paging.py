@@ -153,8 +153,9 @@ def paged_append(query, key, value, k_cache, v_cache, slot_mapping, table, posit
     views of a fused projection are read in place.  ``k_cache``, ``v_cache``:
     contiguous ``(num_pages, page_size, Hkv, D)``, written in place at row
     ``slot_mapping[t]`` (int32, ``page * page_size + row``) of their
-    ``num_pages * page_size`` rows; a slot of -1 writes nothing.  Slots of one
-    call must differ.  ``positions``: int32 ``(total,)``.  The weights, ``eps``
+    ``num_pages * page_size`` rows; a slot of -1 writes nothing,
+    and the token may be at any position (its query is NaN where the table
+    has no row for it).  Other slots of one call must differ.  ``positions``: int32 ``(total,)``.  The weights, ``eps``
     and ``interleaved`` as in ``qk_norm_rotary``."""
     for name, t in (("query", query), ("key", key), ("value", value)):
         if not isinstance(t, torch.Tensor):
