@@ -926,3 +926,57 @@ def test_a_token_without_a_slot_may_be_at_any_position():
     slots[2] = 7
     fa.paged_append(x[:, :4], x[:, 4:6], x[:, 6:], kc, vc, slots, table, pos)
     assert _abi.device_status(reset=True) & 0xff == _abi.FA_ERR_BAD_INDEX
+
+
+@pytest.mark.gpu
+def test_a_step_with_requests_that_do_not_fit():
+    """One request is too long for its row (its positions pass the angles'
+    table), one finds no page.  With ``seqlens_attended`` for the calls behind
+    the append their rows see no key and complete no page, nothing is an
+    error, and the others get what they get when those two bring nothing."""
+    def attend(sv, x, s, lens):
+        q = fa.paged_append(x[:, :sv.hq], x[:, sv.hq:-sv.hkv], x[:, -sv.hkv:], sv.kc, sv.vc, s.slot_mapping, sv.rope,
+                            s.positions, query_weight=sv.w, key_weight=sv.w)
+        fa.update_page_means(sv.kc, sv.means, sv.bt, s.cu_seqlens_q, lens)
+        pages = fa.select_pages(q, sv.means, sv.bt, s.cu_seqlens_q, lens, page_size=sv.page, num_selected=3)
+        o = fa.scaled_dot_product_attention_paged_sparse(q, sv.kc, sv.vc, sv.bt, s.cu_seqlens_q, lens, pages,
+                                                         enable_gqa=True)
+        dense = fa.scaled_dot_product_attention_paged(q, sv.kc, sv.vc, sv.bt, s.cu_seqlens_q, lens, 1000, 24 * 16,
+                                                      is_causal=True, enable_gqa=True)
+        return pages, o, dense
+
+    def served(new, rows):
+        sv = Server(4, pool=12)
+        for t in (sv.kc, sv.vc):  # the dense call wants finite rows behind a sequence's end
+            t.zero_()
+        x0 = sv.x(100)
+        sv.step(_i32([40, 33, 20, 7]).cuda(), x0)  # 3 + 3 + 2 + 1 pages of 12
+        before = sv.kc.clone(), sv.means.clone(), sv.bt.clone()
+        x = _randn(torch.Generator().manual_seed(1), 512, sv.hq + 2 * sv.hkv, sv.d, dtype=sv.dtype).cuda()[rows]
+        s = fa.extend_block_table(sv.bt, sv.lens, _i32(new).cuda(), sv.free, sv.start, page_size=sv.page,
+                                  total_q=x.shape[0])
+        return sv, before, x, s
+
+    assert _abi.device_status(reset=True) == 0
+    # request 1 has room in its row for 24 pages only, request 3 lacks pages; requests 0 and 2 need one page each
+    first = [*range(9), *range(9, 409), *range(409, 422), *range(422, 512)]
+    sv, before, x, s = served([9, 400, 13, 90], first)
+    assert s.fits.tolist() == [True, False, True, False]
+    assert s.seqlens_attended.tolist() == [49, 0, 33, 0] and s.seqlens_attended.dtype == torch.int32
+    pages, o, dense = attend(sv, x, s, s.seqlens_attended)
+    assert _abi.device_status(reset=True) == 0
+    refused = [*range(9, 409), *range(422, 512)]
+    assert (pages[refused] == -1).all() and (o[refused] == 0).all() and (dense[refused] == 0).all()
+    kept = [*range(9), *range(409, 422)]
+    sv2, _, x2, s2 = served([9, 0, 13, 0], kept)
+    pages2, o2, dense2 = attend(sv2, x2, s2, s2.seqlens_attended)
+    assert s2.fits.all() and s2.seqlens_attended.tolist() == s2.seqlens_k.tolist()[:1] + [33, 33, 7]
+    assert torch.equal(pages[kept], pages2) and torch.equal(o[kept], o2) and torch.equal(sv.kc, sv2.kc)
+    assert torch.equal(sv.means, sv2.means) and torch.equal(sv.bt, sv2.bt)
+    assert float((dense[kept].float() - dense2.float()).abs().max()) <= 4e-3  # other tiles: each within 2e-3
+    # the refused ones' history is as it was
+    for r, n in ((1, 33), (3, 7)):
+        for p in range(-(-n // 16)):
+            page = int(sv.bt[r, p])
+            assert page == int(before[2][r, p]) and torch.equal(sv.kc[page], before[0][page])
+            assert torch.equal(sv.means[page], before[1][page])

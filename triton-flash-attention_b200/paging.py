@@ -6,7 +6,8 @@ No counterpart in the reference, which has no cache.  In the order of a step:
   positions and offsets, on the GPU, from the requests' lengths;
 * ``paged_append`` norms and rotates the new queries and keys
   (``rotary.py``) and writes keys and values into the cache;
-* then ``scaled_dot_product_attention_paged`` (``varlen.py``) over all of the
+* then, with the step's ``seqlens_attended``,
+  ``scaled_dot_product_attention_paged`` (``varlen.py``) over all of the
   cache, or attention over a part of it: ``update_page_means`` keeps the mean
   key of every full page, ``select_pages`` scores the pages by it for each
   token and K/V head, and ``scaled_dot_product_attention_paged_sparse``
@@ -86,6 +87,14 @@ class PagedStep(NamedTuple):
     fits: torch.Tensor
     free_next: torch.Tensor
 
+    @property
+    def seqlens_attended(self) -> torch.Tensor:
+        """``seqlens_k`` for the calls behind the append: 0 where the request
+        does not fit, so that its rows, which are in the batch all the same,
+        see no key and complete no page.  (One small launch a use; a step
+        whose requests are known to fit can pass ``seqlens_k``.)"""
+        return self.seqlens_k * self.fits
+
 
 def extend_block_table(block_table, seqlens_cached, seqlens_new, free_pages, free_start, *, page_size: int,
                        total_q: int) -> PagedStep:
@@ -104,7 +113,10 @@ def extend_block_table(block_table, seqlens_cached, seqlens_new, free_pages, fre
     A request that needs more pages than its row has, or rows behind
     ``total_q``, takes nothing; when the free pages run out, the request that
     lacks them and all after it take nothing.  Such a request has ``fits``
-    False, slots of -1 and the ``seqlens_k`` it had."""
+    False, slots of -1 and the ``seqlens_k`` it had, and its rows stay in the
+    batch: the calls behind ``paged_append`` take ``seqlens_attended`` of the
+    result, with ``seqlens_k`` those rows would stand at the positions of the
+    request's last cached tokens."""
     if not isinstance(block_table, torch.Tensor):
         raise TypeError("block_table must be a torch.Tensor")
     dev = block_table.device
