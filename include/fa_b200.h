@@ -613,10 +613,12 @@ FA_API int fa_fwd_paged_sparse_bf16(const void* q, const void* k_cache, const vo
  * FA_ERR_BAD_SHAPE), float as double.  NULL for any other name. */
 FA_API void* fa_packed_entry(const char* name);
 
-/* Reads (and with reset != 0 clears) the device status word that kernels set
- * when a bounded wait gives up or an index is out of range: 0 = healthy, else
- * FA_ERR_DEVICE_TIMEOUT or FA_ERR_BAD_INDEX in the low byte and the site in
- * bits 8..15.  Synchronises the device. */
+/* Reads (and with reset != 0 clears) the current device's status, which kernels
+ * set when a bounded wait gives up or an index is out of range: 0 = healthy,
+ * else FA_ERR_DEVICE_TIMEOUT or FA_ERR_BAD_INDEX in the low byte and the site of
+ * the first such error in bits 8..23.  Neither hides the other: where both have
+ * come up those are the timeout's, and bits 24..31, else 0, the refused index's
+ * site.  Synchronises the device. */
 FA_API int fa_device_status(int reset);
 
 /* Human-readable text of an FA_ERR_* code. */

@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import subprocess
 
 import pytest
 
@@ -131,3 +132,23 @@ def test_varlen_and_paged_entry_points_reject_before_any_cuda_call():
     assert lib.fa_combine_splits(p, p, p, p, 65, 2, 4, 64, None) == _abi.FA_ERR_BAD_SHAPE
     assert lib.fa_combine_splits(p, p, p, p, 2, 2, 4, 48, None) == _abi.FA_ERR_UNSUPPORTED_HEAD_DIM
     assert lib.fa_combine_splits(p, p, 18, p, 2, 2, 4, 64, None) == _abi.FA_ERR_MISALIGNED
+
+
+def test_a_refused_index_does_not_hide_a_timeout(tmp_path):
+    """The device status has a word for each and joins them: the header that
+    says how, in a program of its own."""
+    csrc = os.path.join(os.path.dirname(_abi.__file__), "csrc")
+    src, exe = tmp_path / "joined.cc", tmp_path / "joined"
+    src.write_text("""
+#include <cstdio>
+#include "fa_status.h"
+int main() {
+  const int words[4][2] = {{0, 0}, {0x0507, 0}, {0, 0xe00c}, {0x14a07, 0xe20c}};
+  for (auto& w : words) std::printf("%x ", unsigned(fa::joined_status(w)));
+  std::printf("%d %d\\n", fa::STATUS_TIMEOUT, fa::STATUS_REFUSED);
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-I", csrc, str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+    assert out == ["0", "507", "e00c", "e2014a07", "0", "1"]
+    assert "out of range" in _abi.status_string(int(out[2], 16)) and "timed out" in _abi.status_string(int(out[3], 16))

@@ -203,6 +203,7 @@ def strides_of(key: tuple) -> ctypes.Array:
 
 
 def device_status(reset: bool = False) -> int:
-    """The device status word (0 = healthy; its low byte is an ``FA_ERR_*``
-    code); synchronises the device."""
-    return int(lib().fa_device_status(1 if reset else 0))
+    """The current device's status (0 = healthy; the low byte is an ``FA_ERR_*``
+    code; with a timeout and a refused index both it is the timeout's, and
+    bits 24 to 31 are the latter's site); synchronises the device."""
+    return int(lib().fa_device_status(1 if reset else 0)) & 0xffffffff

@@ -13,7 +13,7 @@
 namespace fa {
 namespace {
 
-__device__ int g_device_status;  // one word per device (each device loads its own copy)
+__device__ int g_device_status[STATUS_WORDS];  // of each device (which loads its own copy)
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -32,7 +32,7 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// Device address of this device's status word (looked up once per device).
+// Device address of this device's status words (looked up once per device).
 int* status_ptr() {
   static int* ptrs[64] = {nullptr};
   static std::mutex mu;
@@ -703,7 +703,7 @@ int bwd_dense_impl(const void* q, const void* k, const void* v, const void* o, c
 
 }  // namespace
 
-int* device_status_word() { return status_ptr(); }
+int* device_status_words() { return status_ptr(); }
 int make_cache_map(CUtensorMap* map, const void* cache, int cache_rows, int Hkv, int D, int rows, int dtype) {
   // as make_map, with the runs of 64 columns as the third dimension and the
   // heads as the fourth
@@ -919,13 +919,13 @@ extern "C" int fa_combine_splits_bf16(const void* o_part, const float* lse_part,
 
 extern "C" int fa_device_status(int reset) {
   if (cudaDeviceSynchronize() != cudaSuccess) return FA_ERR_LAUNCH;
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)) != cudaSuccess) return FA_ERR_LAUNCH;
+  int v[STATUS_WORDS] = {};
+  if (cudaMemcpyFromSymbol(v, g_device_status, sizeof v) != cudaSuccess) return FA_ERR_LAUNCH;
   if (reset) {
-    const int zero = 0;
-    if (cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)) != cudaSuccess) return FA_ERR_LAUNCH;
+    const int zero[STATUS_WORDS] = {};
+    if (cudaMemcpyToSymbol(g_device_status, zero, sizeof zero) != cudaSuccess) return FA_ERR_LAUNCH;
   }
-  return v;
+  return joined_status(v);
 }
 
 namespace fa {

@@ -8,6 +8,7 @@
 
 #include "../../include/fa_b200.h"
 #include "fa_common.cuh"
+#include "fa_status.h"
 
 namespace fa {
 
@@ -95,9 +96,12 @@ int launch_merge_partial(float* o_acc, float* lse_acc, const void* o_part, const
 // Query/key preparation and the paged cache (fa_rotary.cu, fa_tables.cu,
 // fa_sparse.cu; no counterpart in the reference).
 
-// Sites of FA_ERR_BAD_INDEX in the device status word (bits 8..15): a
+// Sites of FA_ERR_BAD_INDEX in the device status (bits 8..15 of its word): a
 // position, a slot, a page or a length that a kernel refused.
 enum : int { FA_SITE_POSITION = 224, FA_SITE_SLOT = 225, FA_SITE_PAGE = 226 };
+__device__ __forceinline__ void refuse_index(int* status, int site) {
+  if (status) atomicCAS(status + STATUS_REFUSED, 0, (site << 8) | FA_ERR_BAD_INDEX);
+}
 
 struct RowStrides {
   long long b, h, n;  // elements
@@ -215,11 +219,11 @@ int launch_early(void (*kernel)(Params...), dim3 blocks, unsigned threads, size_
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
-// The device status word, and a tensor map over a (num_pages, page_size, Hkv,
+// The device status words, and a tensor map over a (num_pages, page_size, Hkv,
 // D) cache whose box is `rows` rows of one head, all D columns: dimensions
 // {min(D, 64) columns, cache rows, D / 64 runs of columns, heads}, so that one
 // copy leaves a row's runs of 64 columns behind each other (fa_capi.cu).
-int* device_status_word();
+int* device_status_words();
 int make_cache_map(CUtensorMap* map, const void* cache, int cache_rows, int Hkv, int D, int rows, int dtype);
 
 // Query-tile / key-tile sizes the host needs for TMA box shapes.

@@ -163,12 +163,12 @@ __device__ __forceinline__ int raw_pos(const RotaryArgs& a, int b, int n) {
   return a.pos ? a.pos[(long long)b * a.pos_sb + n] : n;
 }
 // The position, or -1 when it has no row in the table: an error (the device
-// status word is set), but for an appended token without a slot, as those of a
+// status is set), but for an appended token without a slot, as those of a
 // request are that found no room.
 template <bool APPEND>
 __device__ __forceinline__ int checked_pos(const RotaryArgs& a, int p, int n) {
   if (p >= 0 && p < a.max_pos) return p;
-  if (a.status && !(APPEND && a.slots[n] < 0)) atomicCAS(a.status, 0, (FA_SITE_POSITION << 8) | FA_ERR_BAD_INDEX);
+  if (!(APPEND && a.slots[n] < 0)) refuse_index(a.status, FA_SITE_POSITION);
   return -1;
 }
 constexpr int THREADS = 128;
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(cons
     }
     if (cached) {
       const bool in = slot >= 0 && slot < a.n_slots;
-      if (slot >= a.n_slots && a.status) atomicCAS(a.status, 0, (FA_SITE_SLOT << 8) | FA_ERR_BAD_INDEX);
+      if (slot >= a.n_slots) refuse_index(a.status, FA_SITE_SLOT);
       uint16_t* p = const_cast<uint16_t*>(dst.p) + (in ? (long long)slot * (a.Hkv * D) : 0);
       if (valid && in) {
         st_run<C>(p, ra);

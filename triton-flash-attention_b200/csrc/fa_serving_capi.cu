@@ -58,7 +58,7 @@ int rotary_common(RotaryArgs* a, const float* table, const int* positions, const
   a->Hq = Hq;
   a->Hkv = Hkv;
   a->dtype = dtype;
-  a->status = device_status_word();
+  a->status = device_status_words();
   a->stream = static_cast<cudaStream_t>(stream);
   return FA_OK;
 }
@@ -168,7 +168,7 @@ int means_impl(const void* k_cache, void* means, const int* table, const int* cu
   a.page_log2 = pl;
   a.width = width;
   a.dtype = dtype;
-  a.status = device_status_word();
+  a.status = device_status_words();
   a.stream = static_cast<cudaStream_t>(stream);
   return launch_page_means(a, total_q);
 }
@@ -211,7 +211,7 @@ int select_impl(const void* q, const void* means, const int* table, const int* c
   a.sink = sink;
   a.local = local;
   a.dtype = dtype;
-  a.status = device_status_word();
+  a.status = device_status_words();
   a.stream = static_cast<cudaStream_t>(stream);
   return launch_select_pages(a, D);
 }
@@ -246,7 +246,7 @@ int sparse_impl(const void* q, const void* k_cache, const void* v_cache, void* o
   a.top = top;
   a.dtype = dtype;
   a.scale_log2 = float(double(softmax_scale) * 1.4426950408889634);
-  a.status = device_status_word();
+  a.status = device_status_words();
   a.stream = static_cast<cudaStream_t>(stream);
   return launch_sparse_decode(a, mk, mv, D);
 }

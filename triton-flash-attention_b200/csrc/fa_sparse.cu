@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
     const int nq = q1 - q0;
     if (nq <= 0 || nk <= 0) continue;
     if (nk > (a.width << a.page_log2)) {  // its table row cannot hold it: refused whole, as place_row does
-      if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+      if (threadIdx.x == 0) refuse_index(a.status, FA_SITE_PAGE);
       continue;
     }
     const int from = max(nk - nq, 0) >> a.page_log2;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(MEAN_THREADS) fa_page_means_kernel(const __gri
     if (p < from || p >= (nk >> a.page_log2)) continue;  // uniform in the block
     const int id = a.table[(long long)b * a.width + p];
     if (id < 0 || id >= a.num_pages) {
-      if (threadIdx.x == 0 && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+      if (threadIdx.x == 0) refuse_index(a.status, FA_SITE_PAGE);
       continue;
     }
     const uint16_t* src = static_cast<const uint16_t*>(a.k_cache) + (long long)id * P * a.Hkv * a.D;
@@ -214,7 +214,7 @@ __device__ __forceinline__ RowPlace place_row(const int* cu, const int* seqlens,
   }
   const long long pos = (long long)nk - (q1 - t);  // the rows are the sequence's last
   const bool too_long = nk > key_cap;  // its table row cannot hold it
-  if (too_long && status) atomicCAS(status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+  if (too_long) refuse_index(status, FA_SITE_PAGE);
   r.pos = (t < q0 || t >= q1 || too_long) ? -1 : int(pos < 0 ? -1 : pos);
   return r;
 }
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) fa_select_pages_kernel(const _
   for (int i = threadIdx.x; i < pn; i += SEL_THREADS) {
     const int id = pages[p0 + i];
     const bool ok = id >= 0 && id < a.num_pages;
-    if (!ok && a.status) atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+    if (!ok) refuse_index(a.status, FA_SITE_PAGE);
     ids[i] = ok ? id : -1;
   }
   if (S > 1) cluster_sync();  // and the first block has begun, so that its shared memory may be written
@@ -902,8 +902,8 @@ __global__ void __launch_bounds__(DEC_THREADS, dec_per_sm<D>())
           if (id >= 0 && id < a.num_pages) {
             base = first;
             at = (id << a.page_log2) + sub * DEC_TILE;
-          } else if (a.status) {
-            atomicCAS(a.status, 0, (FA_SITE_PAGE << 8) | FA_ERR_BAD_INDEX);
+          } else {
+            refuse_index(a.status, FA_SITE_PAGE);
           }
         }
       }

@@ -71,7 +71,8 @@ struct CtaCtl {
   int* status;
 };
 
-// Records a timeout: the first failing site wins the device status word.
+// Records a timeout: the first failing site wins the device status' first word
+// (fa_status.h).
 __device__ __forceinline__ void report_timeout(volatile CtaCtl* ctl, int site) {
   int* status = ctl->status;
   if (status) atomicCAS(status, 0, (site << 8) | 7 /* FA_ERR_DEVICE_TIMEOUT */);
