@@ -480,7 +480,8 @@ FA_API int fa_bwd_dropout_bf16(const void* q, const void* k, const void* v, cons
  * rotary_dim / 2 cosines, then as many sines, of each position.  positions is
  * int32, positions[b * pos_batch_stride + n]; NULL: token n is at position n.
  * A position outside the table gives NaN in the turned columns and sets the
- * device status to FA_ERR_BAD_INDEX.  Arithmetic is fp32, rounded once.
+ * device status to FA_ERR_BAD_INDEX.  Arithmetic is fp32, rounded once; rows
+ * whose squares leave its range are scaled by a power of two first.
  * q, q_out: (B, Hq, N, D), k, k_out: (B, Hkv, N, D) by element strides
  * {batch, head, seq} (inputs may have zero strides); packed (total, H, D)
  * tensors are B = 1, N = total.  rotary_dim is a multiple of 16, at most D. */

@@ -446,3 +446,71 @@ def test_saved_tensors_may_come_back_laid_out_otherwise():
         with hooks:
             got = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------- the ends of the range
+def _edge_check(x, w, table, pos, eps, z, gz, dx, dw):
+    """As ``_check`` for bf16 rows of any size: a result below 2^-126 is also
+    off by half of bf16's smallest step, 2^-134, and of fp32's on the way."""
+    x64, gz64, w64 = _f64(x), _f64(gz), _f64(w)
+    rd = table.shape[1]
+    ref = orc.norm_rotary_reference(x64, w64, table.cpu().numpy(), pos, eps, False, gz64)
+    r = 1 / np.sqrt((x64 ** 2).mean(-1, keepdims=True) + eps)
+    dy = _pair_size(gz64, rd, False)
+    g = dy * np.abs(w64)
+    size = r * (g + np.abs(x64) * r * r * (g * np.abs(x64)).mean(-1, keepdims=True))
+    for what, got, want, slack in (("z", z, ref["z"], 2.0 ** -19 * _pair_size(x64 * r * w64, rd, False)),
+                                   ("dx", dx, ref["dx"], 2.0 ** -18 * size)):
+        tol = 2.0 ** -8 * np.abs(want) * 1.001 + slack + 2.0 ** -133
+        diff = np.abs(_f64(got) - want)
+        assert (diff <= tol).all(), (what, np.argwhere(~(diff <= tol))[:4].tolist(), int((~(diff <= tol)).sum()))
+    _assert_close(dw, ref["dw"], 2.0 ** -16 * (dy * np.abs(x64) * r).sum((0, 1)), dw.dtype, "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("eps,powers", [(1e-6, [0, 40, 49, 50, 51, 60, 63, 64, 65, 90, 110, 125]),
+                                        (0.0, [0, -40, -49, -50, -51, -60, -64, -75, -90, -110, -120])])
+def test_bf16_rows_whose_squares_leave_the_fp32_range(d, eps, powers):
+    """Rows of size 2^p: from p = 64 on their squares pass the fp32 range, and
+    without an eps below p = -64 they vanish in it.  The norm is the row's all
+    the same, and so are the gradients."""
+    g = torch.Generator().manual_seed(d)
+    n, h = 3 * len(powers), 3
+    x = _randn(g, n, h, d).clamp(-4, 4)
+    x *= torch.tensor([2.0 ** p for p in powers], dtype=F32).repeat(3)[:, None, None]
+    x[0, 1] *= 2.0 ** (20 if powers[1] > 0 else -20)  # rows of one token in and out of the range
+    x[len(powers) - 1, 2] *= 2.0 ** (-80 if powers[1] > 0 else 80)
+    x = x.to(BF16)
+    x[-1, 0, 5:] = 0  # few values
+    w = (1 + 0.3 * _randn(g, d)).cuda().requires_grad_()
+    gz = _randn(g, n, h, d, dtype=BF16).cuda()
+    table = fa.rotary_table(n, d).cuda()
+    pos = torch.arange(n, dtype=torch.int32)
+    xq = x.cuda().requires_grad_()
+    z, _ = fa.qk_norm_rotary(xq, xq.detach(), table, pos.cuda(), query_weight=w, key_weight=w.detach(), eps=eps)
+    dx, dw = torch.autograd.grad(z, (xq, w), gz)
+    _edge_check(x, w, table, pos.numpy(), eps, z, gz, dx, dw)
+    kc = torch.zeros(-(-n // 16), 16, h, d, dtype=BF16, device="cuda")
+    q = fa.paged_append(xq.detach(), xq.detach(), xq.detach(), kc, kc.clone(), pos.cuda(), table, pos.cuda(),
+                        query_weight=w.detach(), key_weight=w.detach(), eps=eps)
+    assert torch.equal(q, z.detach()) and torch.equal(kc.view(-1, h, d)[:n], q)
+
+
+@pytest.mark.gpu
+def test_rows_with_infinities_zeros_and_the_largest_value():
+    table = fa.rotary_table(4, 32).cuda()
+    q = torch.zeros(4, 2, 64, dtype=BF16).cuda()
+    q[0, 0] = 3e38
+    q[0, 1] = torch.finfo(BF16).max
+    q[1, :, 3] = float("inf")
+    q[1, :, 40] = 5.0
+    pos, w = torch.zeros(4, dtype=torch.int32).cuda(), torch.ones(64).cuda()
+    z, _ = fa.qk_norm_rotary(q, q, table, pos, query_weight=w, key_weight=w)
+    assert (z[0] == 1).all()
+    # an infinity over an infinite norm, also in its pair's other column; everything else vanishes
+    assert z[1, :, [3, 19]].isnan().all() and (z[1, :, 32:] == 0).all() and (z[1, :, [0, 15, 31]] == 0).all()
+    assert (z[2:] == 0).all()
+    z, _ = fa.qk_norm_rotary(q, q, table, pos, query_weight=w, key_weight=w, eps=0.0)
+    assert (z[0] == 1).all() and z[2:].isnan().all()  # 0 / 0
+    assert _abi.device_status() == 0

@@ -159,6 +159,29 @@ __device__ __forceinline__ float group_sum(float v) {
   for (int m = L / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   return v;
 }
+// bf16 rows reach from 2^-133 to 2^128, and their squares past both ends of
+// fp32.  A root r = rsqrt(mean(x^2) + eps) below 2^-50 or above 2^50 tells (0
+// and infinity do too; NaN stays what it is).  fp16 rows stay within.
+template <int DT>
+__device__ __forceinline__ bool out_of_range(float r) {
+  constexpr uint32_t lo = (127u - 50u) << 23, hi = (127u + 50u) << 23;
+  return DT == DT_BF16 && __float_as_uint(r) - lo > hi - lo;
+}
+// Brings such a row (of a warp's rows those that are; all lanes call) by a power
+// of two, 2^-72 or 2^72, to where its squares are normal numbers, with eps
+// alike; returns the power.  r becomes the scaled row's.
+template <int DT, int D, int L, int C>
+__device__ __forceinline__ float bring_in_range(Run<C>& x, Run<C>& y, float& r, float eps) {
+  const float k = !out_of_range<DT>(r) ? 1.f : r > 1.f ? 0x1p72f : 0x1p-72f;
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    x.v[j] *= k, y.v[j] *= k;
+    ss = fmaf(x.v[j], x.v[j], fmaf(y.v[j], y.v[j], ss));
+  }
+  r = rsqrtf(group_sum<L>(ss) * (1.f / D) + eps * k * k);
+  return k;
+}
 __device__ __forceinline__ int raw_pos(const RotaryArgs& a, int b, int n) {
   return a.pos ? a.pos[(long long)b * a.pos_sb + n] : n;
 }
@@ -320,7 +343,8 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS) fa_rotary_fwd_kernel(cons
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int j = 0; j < C; ++j) s0 = fmaf(x.v[j], x.v[j], s0), s1 = fmaf(y.v[j], y.v[j], s1);
-        const float r = rsqrtf(group_sum<L>(s0 + s1) * (1.f / D) + a.eps);
+        float r = rsqrtf(group_sum<L>(s0 + s1) * (1.f / D) + a.eps);
+        if (__any_sync(0xffffffffu, out_of_range<DT>(r))) bring_in_range<DT, D, L, C>(x, y, r, a.eps);
 #pragma unroll
         for (int j = 0; j < C; ++j) x.v[j] *= r * wa.v[j], y.v[j] *= r * wb.v[j];
       }
@@ -418,8 +442,8 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) fa_rotary_bwd_kernel(cons
       Run<C> yb = widen<DT, C>(ld_run<C>(here + (32 + lane) * R::RUN));
       if (c.turned) turn<INTER, true, C>(ya, yb, read_angles<D, C>(here + R::ANGLES, l));
       if (NORM) {
-        const Run<C> x = widen<DT, C>(ld_run<C>(here + (64 + lane) * R::RUN));
-        const Run<C> y = widen<DT, C>(ld_run<C>(here + (96 + lane) * R::RUN));
+        Run<C> x = widen<DT, C>(ld_run<C>(here + (64 + lane) * R::RUN));
+        Run<C> y = widen<DT, C>(ld_run<C>(here + (96 + lane) * R::RUN));
         float ss = 0.f, gx = 0.f;
         Run<C> ta, tb;  // dy w
 #pragma unroll
@@ -429,17 +453,24 @@ __global__ void __launch_bounds__(THREADS, BWD_BLOCKS) fa_rotary_bwd_kernel(cons
           ss = fmaf(x.v[j], x.v[j], fmaf(y.v[j], y.v[j], ss));
           gx = fmaf(ta.v[j], x.v[j], fmaf(tb.v[j], y.v[j], gx));
         }
-        ss = group_sum<L>(ss);
+        float r = rsqrtf(group_sum<L>(ss) * (1.f / D) + a.eps);
+        float k = 1.f;  // what the row is scaled by, and its gradient then too
+        if (__any_sync(0xffffffffu, out_of_range<DT>(r))) {
+          k = bring_in_range<DT, D, L, C>(x, y, r, a.eps);
+          gx = 0.f;
+#pragma unroll
+          for (int j = 0; j < C; ++j) gx = fmaf(ta.v[j], x.v[j], fmaf(tb.v[j], y.v[j], gx));
+        }
         gx = group_sum<L>(gx);
-        const float r = rsqrtf(ss * (1.f / D) + a.eps);
-        const float m = -gx * (1.f / D) * r * r;
+        const float rk = r * k;
+        const float m = -gx * (1.f / D) * r * rk;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
           const float xr = x.v[j] * r, yr = y.v[j] * r;
           dwa.v[j] = fmaf(ya.v[j], xr, dwa.v[j]);
           dwb.v[j] = fmaf(yb.v[j], yr, dwb.v[j]);
-          ya.v[j] = fmaf(xr, m, ta.v[j] * r);
-          yb.v[j] = fmaf(yr, m, tb.v[j] * r);
+          ya.v[j] = fmaf(xr, m, ta.v[j] * rk);
+          yb.v[j] = fmaf(yr, m, tb.v[j] * rk);
         }
       }
       if (valid) {

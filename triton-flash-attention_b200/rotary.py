@@ -10,7 +10,7 @@ enter the product (triton_flash_attention/attention.py:584-626).  For a row
 
 for the column pairs ``(a, b)`` of the first ``rotary_dim`` columns; columns
 behind them keep ``y``.  Both steps run in fp32 and the result is rounded
-once.  ``qk_norm_rotary`` supports autograd; ``paged_append`` (``paging.py``)
+once (bf16 rows whose squares leave fp32's range are scaled first).  ``qk_norm_rotary`` supports autograd; ``paged_append`` (``paging.py``)
 is the same preparation for serving, with keys and values written to a paged
 cache.
 """
