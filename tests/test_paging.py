@@ -980,3 +980,26 @@ def test_a_step_with_requests_that_do_not_fit():
             page = int(sv.bt[r, p])
             assert page == int(before[2][r, p]) and torch.equal(sv.kc[page], before[0][page])
             assert torch.equal(sv.means[page], before[1][page])
+
+
+@pytest.mark.gpu
+def test_a_sequence_next_to_a_refused_one_is_the_reference():
+    """Bad pages, lengths past the table and lengths below the rows' in one
+    sequence: the other one's pages and output are float64's."""
+    c = Case([1, 1], [200, 100], 16, 4, 2, 64, F16, 15)
+    pages = _random_pages(c, 5, 1)
+    o, a = orc.sparse_paged_reference(*c.refs(), pages, c.d ** -0.5)
+    tol = (2.0 ** -11 * (a + np.abs(o)) * 1.01 + 2e-4 * a + 80 * 2.0 ** -25 * 5 + 2.0 ** -25)[1]
+    q, kc, vc, table, cu, lens = c.cuda()
+    means = torch.zeros(kc.shape[0], 2, 64, dtype=F16, device="cuda")
+    fa.update_page_means(kc, means, table, _i32([0, 200, 300]).cuda(), lens)
+    sel = orc.select_pages_reference(_f64(c.q), _f64(means), c.table, c.cu, c.lens, 16, 4, 1, 1)
+    assert _abi.device_status(reset=True) == 0
+    bad = [(torch.cat([torch.full_like(table[:1], b), table[1:]]), lens) for b in (-1, -2 ** 31, kc.shape[0], 2 ** 31 - 1)]
+    bad += [(table, _i32([n, 100]).cuda()) for n in (100_000, 2 ** 31 - 1, -3, 0)]
+    for t, ln in bad:
+        out = fa.scaled_dot_product_attention_paged_sparse(q, kc, vc, t, cu, ln, _i32(pages).cuda(), enable_gqa=True)
+        assert (out[0] == 0).all() and (np.abs(_f64(out[1]) - o[1]) <= tol).all()
+        got = fa.select_pages(q, means, t, cu, ln, page_size=16, num_selected=4)
+        assert np.array_equal(got[1].cpu().numpy(), sel[1])
+        _abi.device_status(reset=True)

@@ -514,3 +514,63 @@ def test_rows_with_infinities_zeros_and_the_largest_value():
     z, _ = fa.qk_norm_rotary(q, q, table, pos, query_weight=w, key_weight=w, eps=0.0)
     assert (z[0] == 1).all() and z[2:].isnan().all()  # 0 / 0
     assert _abi.device_status() == 0
+
+
+# ---------------------------------------------------------------- many tokens a warp
+LONG = [
+    # b, n, hq, hkv, d, rd, interleaved, norm, weights, dtype
+    (3, 1367, 32, 8, 128, 128, False, True, F32, BF16),
+    (3, 1367, 32, 8, 128, 64, False, False, None, F16),
+    (3, 2221, 16, 16, 64, 64, True, True, F16, F16),
+    (3, 2221, 16, 16, 64, 32, True, False, None, BF16),
+    (5, 2665, 8, 8, 32, 32, False, True, BF16, BF16),
+    (5, 2665, 8, 8, 32, 16, True, False, None, F16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,n,hq,hkv,d,rd,interleaved,norm,wdt,dt", LONG)
+def test_ranges_of_many_tokens_that_cross_batches(b, n, hq, hkv, d, rd, interleaved, norm, wdt, dt):
+    """A warp takes 10 to 18 tokens of its heads here (148 SMs), several turns
+    of its ring, and ranges run over the ends of batches of odd length."""
+    g = torch.Generator().manual_seed(n + d + rd)
+    table = fa.rotary_table(n + 40, rd).cuda()
+    weights = [(1 + 0.5 * _randn(g, d)).to(wdt).cuda().requires_grad_() if norm else None for _ in range(2)]
+    x = _randn(g, b, n, hq + hkv, d, dtype=dt).cuda()
+    q, k = (t.transpose(1, 2).detach().requires_grad_() for t in (x[:, :, :hq], x[:, :, hq:]))
+    gz = [_randn(g, b, h, n, d, dtype=dt).cuda() for h in (hq, hkv)]
+    pos = torch.stack([torch.randperm(n + 40, generator=g)[:n] for _ in range(b)]).int()
+    z = fa.qk_norm_rotary(q, k, table, pos.cuda(), query_weight=weights[0], key_weight=weights[1], eps=1e-5,
+                          interleaved=interleaved)
+    grads = torch.autograd.grad(z, [q, k] + [w for w in weights if norm], gz)
+    for i, src in enumerate((q, k)):
+        _check(_packed(src.detach()), weights[i], table, pos.reshape(-1).numpy(), 1e-5, interleaved, _packed(z[i]),
+               _packed(gz[i]), _packed(grads[i]), grads[2 + i] if norm else None)
+    assert _abi.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("total,hq,hkv,d,dt", [(9174, 8, 2, 64, BF16), (9001, 3, 1, 128, F16), (15013, 4, 4, 32, F16)])
+def test_append_of_many_tokens(total, hq, hkv, d, dt):
+    """As above for the cache: 10 to 16 tokens a warp, some without a slot,
+    against float64."""
+    g = torch.Generator().manual_seed(total)
+    page, n_pages = 16, total // 16 + 4
+    x = _randn(g, total, hq + 2 * hkv, d, dtype=dt).cuda()
+    q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+    table = fa.rotary_table(total + 3, d).cuda()
+    pos = torch.randperm(total + 3, generator=g)[:total].int()
+    slots = torch.randperm(n_pages * page, generator=g)[:total].int()
+    slots[torch.randperm(total, generator=g)[:total // 7]] = -1
+    wq, wk = ((1 + 0.5 * _randn(g, d)).cuda() for _ in range(2))
+    kc, vc = (torch.full((n_pages, page, hkv, d), float("nan"), dtype=dt, device="cuda") for _ in range(2))
+    out = fa.paged_append(q, k, v, kc, vc, slots.cuda(), table, pos.cuda(), query_weight=wq, key_weight=wk)
+    _check(q, wq, table, pos.numpy(), 1e-6, False, out)
+    has = slots >= 0
+    at = slots[has].long().cuda()
+    _check(k[has.cuda()], wk, table, pos[has].numpy(), 1e-6, False, kc.view(-1, hkv, d)[at])
+    assert torch.equal(vc.view(-1, hkv, d)[at], v[has.cuda()])
+    rest = torch.ones(n_pages * page, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert kc.view(-1, hkv, d)[rest].isnan().all() and vc.view(-1, hkv, d)[rest].isnan().all()
+    assert _abi.device_status() == 0
