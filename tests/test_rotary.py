@@ -574,3 +574,46 @@ def test_append_of_many_tokens(total, hq, hkv, d, dt):
     rest[at] = False
     assert kc.view(-1, hkv, d)[rest].isnan().all() and vc.view(-1, hkv, d)[rest].isnan().all()
     assert _abi.device_status() == 0
+
+
+# ---------------------------------------------------------------- the launches by themselves
+def test_launches_refuse_what_they_would_misread():
+    """The forward's and backward's launches check what ``qk_norm_rotary``
+    does, and the gradients."""
+    q, k = torch.randn(5, 4, 32).half(), torch.randn(5, 2, 32).half()
+    t, p, w = fa.rotary_table(8, 32), torch.arange(5, dtype=torch.int32), torch.ones(32)
+    fwd = [q, k, t, p, w, w, 1e-6, False]
+    bwd = [q, k, q.clone(), k.clone(), t, p, w, w, 1e-6, False]
+    for call, args, rest in ((fa.qk_norm_rotary_forward, fwd, 2), (fa.qk_norm_rotary_backward, bwd, 4)):
+        with pytest.raises(RuntimeError, match="requires a CUDA tensor"):
+            call(*args)
+        for at, bad, message in [(rest + 1, p.long(), "int32"), (rest + 1, p[:4], "int32"), (rest, t[:, :16], "contiguous"),
+                                 (rest + 2, w[:16], "head_dim weights"), (rest + 3, None, "both"),
+                                 (rest + 4, -1.0, "eps"), (1, k[:4], None)]:
+            with pytest.raises(ValueError, match=message):
+                call(*[bad if j == at else x for j, x in enumerate(args)])
+    for at, bad in ((2, q[:4]), (2, q.float()), (3, q)):
+        with pytest.raises(ValueError, match="shape, dtype and device"):
+            fa.qk_norm_rotary_backward(*[bad if j == at else x for j, x in enumerate(bwd)])
+    with pytest.raises(TypeError, match="grad_q"):
+        fa.qk_norm_rotary_backward(q, k, None, *bwd[3:])
+
+
+@pytest.mark.gpu
+def test_launches_take_positions_and_weights_of_any_stride():
+    g = torch.Generator().manual_seed(11)
+    q, k, gq, gk = (_randn(g, 40, h, 64, dtype=F16).cuda() for h in (4, 2, 4, 2))
+    table, pos, w = fa.rotary_table(90, 64).cuda(), torch.arange(40, dtype=torch.int32).cuda() * 2, torch.rand(64).cuda()
+    wide = torch.full((40, 3), 1 << 30, dtype=torch.int32, device="cuda")
+    wide[:, 1] = pos
+    ww = torch.full((64, 2), float("nan"), device="cuda")
+    ww[:, 0] = w
+    one = torch.full((1,), 7, dtype=torch.int32, device="cuda").expand(40)
+    for p, v in ((pos, w), (wide[:, 1], ww[:, 0]), (one, w)):
+        z = fa.qk_norm_rotary_forward(q, k, table, p, v, v, 1e-6, False)
+        d = fa.qk_norm_rotary_backward(q, k, gq, gk, table, p, v, v, 1e-6, False)
+        pc, vc = p.contiguous(), v.contiguous()
+        want = (fa.qk_norm_rotary_forward(q, k, table, pc, vc, vc, 1e-6, False)
+                + fa.qk_norm_rotary_backward(q, k, gq, gk, table, pc, vc, vc, 1e-6, False))
+        assert all(torch.equal(a, b) for a, b in zip(z + d, want))
+    assert _abi.device_status() == 0

@@ -10,9 +10,9 @@ enter the product (triton_flash_attention/attention.py:584-626).  For a row
 
 for the column pairs ``(a, b)`` of the first ``rotary_dim`` columns; columns
 behind them keep ``y``.  Both steps run in fp32 and the result is rounded
-once (bf16 rows whose squares leave fp32's range are scaled first).  ``qk_norm_rotary`` supports autograd; ``paged_append`` (``paging.py``)
-is the same preparation for serving, with keys and values written to a paged
-cache.
+once (bf16 rows whose squares leave fp32's range are scaled first).
+``qk_norm_rotary`` supports autograd; ``paged_append`` (``paging.py``) is the
+same preparation for serving, with keys and values written to a paged cache.
 """
 
 from __future__ import annotations
@@ -257,8 +257,14 @@ def _backward(q, k, grad_q, grad_k, table, positions, query_weight, key_weight, 
     return dq, dk, dwq, dwk
 
 
+def _contiguous(*tensors):
+    return [None if t is None else t.contiguous() for t in tensors]
+
+
 def qk_norm_rotary_forward(q, k, table, positions, query_weight, key_weight, eps: float, interleaved: bool):
     """Launch the forward: contiguous outputs in the inputs' layout."""
+    _validate(q, k, table, positions, query_weight, key_weight, eps, interleaved)
+    positions, query_weight, key_weight = _contiguous(positions, query_weight, key_weight)
     return _forward(q, k, table, positions, query_weight, key_weight, eps, interleaved)[:2]
 
 
@@ -266,6 +272,13 @@ def qk_norm_rotary_backward(q, k, grad_q, grad_k, table, positions, query_weight
                             interleaved: bool, weight_grads: bool = True):
     """dQ, dK and, with weights and ``weight_grads``, the weights' gradients
     (else None).  Gradients repeat bit for bit."""
+    for name, g, t in (("grad_q", grad_q, q), ("grad_k", grad_k, k)):
+        if not isinstance(g, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if isinstance(t, torch.Tensor) and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device):
+            raise ValueError(f"{name} must have the shape, dtype and device of its output")
+    _validate(q, k, table, positions, query_weight, key_weight, eps, interleaved)
+    positions, query_weight, key_weight = _contiguous(positions, query_weight, key_weight)
     qos, kos = _contiguous_strides(q.shape), _contiguous_strides(k.shape)
     sizes = (*_sizes(q, k), *table.shape, interleaved,
              query_weight is not None and query_weight.dtype == torch.float32)
@@ -314,8 +327,5 @@ def qk_norm_rotary(query, key, table, positions=None, *, query_weight=None, key_
     A position outside the table is found on the GPU: its turned columns are
     NaN and the device status (``_abi.device_status``) names the error."""
     _validate(query, key, table, positions, query_weight, key_weight, eps, interleaved)
-    if positions is not None:
-        positions = positions.contiguous()
-    if query_weight is not None:
-        query_weight, key_weight = query_weight.contiguous(), key_weight.contiguous()
+    positions, query_weight, key_weight = _contiguous(positions, query_weight, key_weight)
     return B200QKNormRotary.apply(query, key, table, positions, query_weight, key_weight, float(eps), interleaved)
