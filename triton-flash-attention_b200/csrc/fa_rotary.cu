@@ -19,20 +19,25 @@
 // both halves of its pairs: the rotation needs no exchange and the mean of
 // squares log2(D / 2 C) shuffles.  A warp takes GW = 64 C / D neighbouring
 // heads of all tokens of a range, one token a step, so that its weights and
-// strides stay in registers and a step adds to its pointers and no more: these
-// kernels run out of issued instructions before they run out of bytes, and
-// what is worked out for a token or a kind of row costs as much as its
-// arithmetic.  Asynchronous copies bring the next steps' rows and angles into
-// a ring of the warp's own in shared memory, so that no register waits for
-// them.
+// strides stay in registers and a step adds to its pointers and no more.  At
+// D 128 that takes two thirds of the issue slots; forms that worked out a
+// token's place or a kind of row at every step had 260 to 305 instructions in
+// it and ran out of them first.  Asynchronous copies bring the next steps' rows
+// and angles into a ring of the warp's own in shared memory, so that no
+// register waits for them.  B2 H32/8 N8191 D128 bf16: forward 58 us (51 of
+// HBM), backward 88 with the weights' sums (77); without a norm 57 and 61 (51
+// each).  Further from their bytes: D 32 (B4 H32/8 N8191) 39 and 60 us (26 and
+// 38), whose copies are 8 bytes a lane, and interleaved pairs (B8 H16 N4097
+// D64) 73 and 118 us (41 and 62; halves 50 and 73): a lane's two runs lie beside
+// each other there, an access of the warp touches half of every 32 bytes, and
+// the memory pipe is what it waits for.
 #include "fa_kernels.h"
 
 namespace fa {
 namespace {
 
-// A lane's run of C columns in fp32.  (Packed pairs, f32x2, were slower: the
-// kernel is bound by issued instructions before it is by bytes, and pairs cost
-// more moves than they save.)
+// A lane's run of C columns in fp32.  (Packed pairs, f32x2, were slower: they
+// cost more moves than they save.)
 template <int C>
 struct Run {
   float v[C];
@@ -200,6 +205,7 @@ constexpr int WARPS = THREADS / 32;
 // alone takes 51 and 77 us): forward 4 steps x 5 blocks 58 us, 6 x 4 60, 5 x 6
 // 59; backward 3 x 4 85 us, 4 x 4 87, 4 x 3 87 (and 113 with C = 4).
 constexpr int FWD_STEPS = 4, FWD_BLOCKS = 5;
+// One backward form (D 64, bf16, halves) spills 12 bytes a thread.
 constexpr int BWD_STEPS = 3, BWD_BLOCKS = 4;
 template <int D>
 constexpr int run_cols() {  // C: of narrow rows fewer, so that a step is 8 rows at most
